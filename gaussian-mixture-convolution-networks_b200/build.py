@@ -22,6 +22,8 @@ COMMON_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-I", I
 # compiled with IEEE arithmetic and without FMA contraction.
 FAST_MATH = ["--use_fast_math"]
 IEEE_FILES = {"lbvh.cu", "mhem_fit.cu", "convolution_fitting.cu"}
+# Compiled with neither: they choose approximate functions one by one and rely on signed zeros, infinities and NaN.
+PLAIN_FILES = {"log_probabilities.cu"}
 
 
 def _sources():
@@ -50,7 +52,7 @@ def _compile(src, verbose, bounds_check=False):
         flags += ["-DGMC_BOUNDS_CHECK"]
     if src in IEEE_FILES:
         flags += ["--fmad=false"]
-    else:
+    elif src not in PLAIN_FILES:
         flags += FAST_MATH
     if verbose:
         flags += ["-Xptxas", "-v"]

@@ -41,6 +41,7 @@ static __device__ int g_device_check_word;
 enum DeviceCheck : int {
     CHECK_MBARRIER_TIMEOUT = 1,     // a bounded wait for a bulk copy ran out
     CHECK_INDEX_RANGE = 4,          // GMC_BOUNDS_CHECK builds only: a data-dependent index left its array
+    CHECK_CLASS_RANGE = 8,          // a target is neither a class nor the ignored value
 };
 
 __device__ __forceinline__ void report_check(int code) { atomicOr(&g_device_check_word, code); }

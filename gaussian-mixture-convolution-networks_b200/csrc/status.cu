@@ -16,6 +16,7 @@ int gmc_tu_check_mhem_fit(int* word);
 int gmc_tu_check_convolution(int* word);
 int gmc_tu_check_convolution_fitting(int* word);
 int gmc_tu_check_relu_fixed_point(int* word);
+int gmc_tu_check_log_probabilities(int* word);
 
 extern "C" const char* gmc_status_string(int status) {
     switch (status) {
@@ -63,5 +64,6 @@ static int read_all_check_words(int* word_out) {
     if (int s = gmc_tu_check_convolution(word_out)) return s;
     if (int s = gmc_tu_check_convolution_fitting(word_out)) return s;
     if (int s = gmc_tu_check_relu_fixed_point(word_out)) return s;
+    if (int s = gmc_tu_check_log_probabilities(word_out)) return s;
     return GMC_OK;
 }

@@ -76,6 +76,11 @@ _declare("gmc_symeig", [_c_float_p] * 3 + [ctypes.c_longlong, _c_int, _c_void_p]
 _declare("gmc_integrate", [_c_float_p] * 2 + [ctypes.c_longlong, _c_int, _c_int, _c_void_p])
 _declare("gmc_trace_scale", [_c_float_p] * 3 + [ctypes.c_longlong, _c_int, _c_int, _c_void_p])
 _declare("gmc_spatial_scale", [_c_float_p] * 3 + [ctypes.c_longlong, _c_int, _c_int, _c_void_p])
+_c_long = ctypes.c_longlong
+_declare("gmc_log_probabilities_forward", [_c_void_p, _c_int, _c_void_p] + [_c_long] * 3 + [ctypes.c_float, _c_long, _c_int]
+         + [_c_void_p] * 6)
+_declare("gmc_log_probabilities_backward", [_c_void_p, _c_int] + [_c_void_p] * 8 + [_c_long] * 3
+         + [ctypes.c_float, _c_long, _c_int, _c_void_p])
 _declare("gmc_input_normalise", [_c_float_p, _c_void_p, _c_float_p, _c_float_p, ctypes.c_longlong, _c_int, _c_int, _c_int,
                                  _c_void_p, _c_void_p, _c_void_p])
 
@@ -121,6 +126,19 @@ def require_cuda_f32(t: torch.Tensor, name: str) -> None:
         raise GmcError(f"{name} must be float32 (got {t.dtype})")
     if not t.is_contiguous():
         raise GmcError(f"{name} must be contiguous")
+
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def dtype_code(t: torch.Tensor, name: str) -> int:
+    """Element type of an operator that takes 32 and 16 bits (enum gmc_dtype)."""
+    if not t.is_cuda:
+        raise GmcError(f"{name} must be a CUDA tensor: this library has no CPU implementation")
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise GmcError(f"{name} must be float32, bfloat16 or float16 (got {t.dtype})")
+    return code
 
 
 def sync_and_check(device=None) -> None:

@@ -8,6 +8,7 @@ from torch import Tensor
 import torch.nn as nn
 import torch.nn.functional as F
 
+import gmc.classification
 import gmc.mixture as gm
 import gmc.modules
 
@@ -206,8 +207,19 @@ class Net(nn.Module):
                 x, x_const = self.norms[i]((x, x_const))
         return gm.integrate(x)
 
-    def forward(self, in_x: Tensor, tensorboard=None) -> Tensor:
+    def logits(self, in_x: Tensor, tensorboard=None) -> Tensor:
+        """The class scores [n_batch, n_classes] that forward() normalises."""
         x = self.normX(self.features(in_x, tensorboard))
         if self.mlp is not None:
             x = self.mlp(x)
-        return F.log_softmax(x, dim=1).view(in_x.shape[0], self.config.n_classes)
+        return x
+
+    def forward(self, in_x: Tensor, tensorboard=None) -> Tensor:
+        return F.log_softmax(self.logits(in_x, tensorboard), dim=1).view(in_x.shape[0], self.config.n_classes)
+
+    def log_probabilities(self, in_x: Tensor, targets: typing.Optional[Tensor] = None, n_top: int = 0,
+                          temperature: float = 1.0) -> gmc.classification.LogProbabilities:
+        """Log-probability of each sample's target class, entropy of its distribution and its n_top likeliest classes in
+        one pass (gmc.classification.log_probabilities). -result.target.mean() is the loss that nll_loss(forward(x), targets)
+        computes."""
+        return gmc.classification.log_probabilities(self.logits(in_x), targets, n_top, temperature)

@@ -47,6 +47,9 @@ enum gmc_status {
     GMC_ERR_BUILTIN_SCRATCH = 9  /* problem larger than the built-in scratch of a *_noalloc entry point */
 };
 
+/* Element types of the entry points that take a `dtype` (the others are fp32). */
+enum gmc_dtype { GMC_FLOAT32 = 0, GMC_BFLOAT16 = 1, GMC_FLOAT16 = 2 };
+
 /* Human-readable text for a status code (static storage, never NULL). */
 const char* gmc_status_string(int status);
 /* cudaGetErrorString of the last CUDA error this library saw on the calling thread ("" if none). */
@@ -55,7 +58,8 @@ const char* gmc_last_cuda_error(void);
 const char* gmc_version(void);
 /* Reads and clears the device-side check word of the current device (synchronises the WHOLE device).
  * 0 = no kernel reported a problem since the last call. Bit 1: a bounded wait for a bulk copy ran out (the kernel
- * wrote NaN to the outputs it could not compute); bit 4: an index check of a bounds-checked build failed. */
+ * wrote NaN to the outputs it could not compute); bit 4: an index check of a bounds-checked build failed; bit 8: a
+ * target class was out of range (its outputs are NaN). */
 int gmc_device_check_word(int* word_out);
 /* Waits for `stream` and returns GMC_ERR_DEVICE_CHECK if any kernel of this library reported a problem since the last
  * check (the word is cleared), GMC_OK otherwise. Call it wherever the host synchronises anyway: device-side give-ups
@@ -326,6 +330,34 @@ int gmc_convolution_fitting_backward(const float* grad, const float* data, const
                                      const float* cached_pos_covs, const int32_t* nodesobjs,
                                      const int32_t* fitting_subtrees, float* grad_data, float* grad_kernels,
                                      void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Log-probabilities of given classes, entropy and the likeliest classes of rows of logits z (the classifier's answer and
+ * its loss; the reference's network ends in log_softmax + nll_loss, src/gmc/model.py):
+ *   log p_j = z_j / T - log sum_i exp(z_i / T)
+ *   target[r]  = log p of class targets[r]; 0 where targets[r] == ignore_index; NaN and check bit 8 where targets[r] is
+ *                neither that nor in [0, n_classes). targets and target may both be NULL.
+ *   entropy[r] = -sum_j p_j log p_j
+ *   top[r, i], top_indices[r, i], i < n_top: log p and class of the n_top largest logits, largest first, equal logits by
+ *                the lower class; NaN logits rank behind -inf. n_top <= min(32, n_classes); 0 = none.
+ *   stats[r, 2] = max z, log sum exp((z - max) / T): input of the backward; may be NULL.
+ * Masked classes (-inf) have probability 0. A row with nothing but -inf: log p = -inf, entropy 0, gradient 0. A row with
+ * NaN or +inf: NaN log-probabilities, entropy and gradient. logits is [n_rows, n_classes] of `dtype` with unit class
+ * stride and row_stride elements between rows (0 = one row for all); T in [1e-6, 1e6]; n_rows <= 2^27,
+ * n_classes <= 2^30. Sums are fp32; outputs are fp32. Results do not depend on the launch order (no atomics).
+ *
+ * Backward: dz_j = 1/T [ grad_target d(t, j) + sum_i grad_top[i] d(top_i, j) - p_j (grad_target + sum_i grad_top[i])
+ *                        - p_j grad_entropy (log p_j + entropy) ]
+ * Each incoming gradient (fp32, shaped like its output) may be NULL = zero. grad_logits is [n_rows, n_classes] contiguous,
+ * of `dtype`, fully overwritten; it must not overlap the logits.
+ * ---------------------------------------------------------------------------------------------- */
+int gmc_log_probabilities_forward(const void* logits, int dtype, const long long* targets, long long n_rows, long long n_classes,
+                                  long long row_stride, float temperature, long long ignore_index, int n_top, float* target,
+                                  float* entropy, float* stats, float* top, long long* top_indices, void* stream);
+int gmc_log_probabilities_backward(const void* logits, int dtype, const long long* targets, const long long* top_indices,
+                                   const float* stats, const float* entropy, const float* grad_target, const float* grad_entropy,
+                                   const float* grad_top, void* grad_logits, long long n_rows, long long n_classes,
+                                   long long row_stride, float temperature, long long ignore_index, int n_top, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * gmc_mhem_fit_forward for callers that have no scratch memory to give. (No counterpart in the reference, which
