@@ -23,7 +23,7 @@ COMMON_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-I", I
 FAST_MATH = ["--use_fast_math"]
 IEEE_FILES = {"lbvh.cu", "mhem_fit.cu", "convolution_fitting.cu"}
 # Compiled with neither: they choose approximate functions one by one and rely on signed zeros, infinities and NaN.
-PLAIN_FILES = {"log_probabilities.cu"}
+PLAIN_FILES = {"log_probabilities.cu", "newton_schulz.cu"}
 
 
 def _sources():

@@ -17,6 +17,7 @@ int gmc_tu_check_convolution(int* word);
 int gmc_tu_check_convolution_fitting(int* word);
 int gmc_tu_check_relu_fixed_point(int* word);
 int gmc_tu_check_log_probabilities(int* word);
+int gmc_tu_check_newton_schulz(int* word);
 
 extern "C" const char* gmc_status_string(int status) {
     switch (status) {
@@ -30,6 +31,7 @@ extern "C" const char* gmc_status_string(int status) {
         case GMC_ERR_BUILTIN_SCRATCH:
             return "problem exceeds the built-in scratch of the no-allocation entry point (n_mixtures * n_components > "
                    "2^20); use the entry point that takes caller scratch";
+        case GMC_ERR_WORKSPACE: return "the workspace is smaller than the entry point's ..._workspace_bytes asks for";
         default: return "unknown status";
     }
 }
@@ -65,5 +67,6 @@ static int read_all_check_words(int* word_out) {
     if (int s = gmc_tu_check_convolution_fitting(word_out)) return s;
     if (int s = gmc_tu_check_relu_fixed_point(word_out)) return s;
     if (int s = gmc_tu_check_log_probabilities(word_out)) return s;
+    if (int s = gmc_tu_check_newton_schulz(word_out)) return s;
     return GMC_OK;
 }

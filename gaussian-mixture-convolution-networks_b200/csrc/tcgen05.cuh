@@ -1,0 +1,66 @@
+// 5th-generation tensor core helpers (tcgen05, one CTA): descriptors of 128-byte-swizzled fp16 tiles in shared memory,
+// tensor memory, and the instructions' wrappers.
+#pragma once
+
+#include "common.cuh"
+
+namespace gmc {
+
+// A tile is stored in rows of 64 fp16 elements (128 bytes); the 16-byte chunk c of row r sits at chunk c ^ (r & 7), groups
+// of eight rows are 1024 bytes apart, and tiles start on 1024-byte boundaries. The same tile is read along its rows
+// (K contiguous: `k_major`) or across them (rows are the K axis: `mn_major`).
+__device__ __forceinline__ uint32_t swizzled_offset(int row, int chunk) {
+    return uint32_t(row) * 128u + (uint32_t(chunk ^ (row & 7)) << 4);
+}
+constexpr uint64_t kDescriptorBase = (uint64_t(1) << 46) | (uint64_t(2) << 61) | (uint64_t(1024 >> 4) << 32);
+__device__ __forceinline__ uint64_t k_major_descriptor(uint32_t smem) {
+    return kDescriptorBase | (uint64_t(1) << 16) | ((smem >> 4) & 0x3fffu);
+}
+// column_group_bytes: distance between neighbouring groups of 64 columns.
+__device__ __forceinline__ uint64_t mn_major_descriptor(uint32_t smem, uint32_t column_group_bytes) {
+    return kDescriptorBase | (uint64_t((column_group_bytes >> 4) & 0x3fffu) << 16) | ((smem >> 4) & 0x3fffu);
+}
+// fp16 x fp16 -> fp32, A along K, B along K or across it.
+__host__ __device__ constexpr uint32_t f16_instruction(int m, int n, bool b_mn_major) {
+    return (1u << 4) | (b_mn_major ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void tmem_alloc(uint32_t* address_smem, uint32_t columns) {       // one warp
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(address_smem)), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_free(uint32_t address, uint32_t columns) {              // the same warp
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(address), "r"(columns));
+}
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(instruction),
+        "r"(uint32_t(accumulate))
+        : "memory");
+}
+// `bar` gets one arrival when every MMA this thread has issued is complete.
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// 32 fp32 columns of the warp's 32 lanes (the thread's lane); complete on return.
+__device__ __forceinline__ void tmem_load32(uint32_t address, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+          "=r"(r[31])
+        : "r"(address)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+}  // namespace gmc

@@ -5,6 +5,7 @@ import fails, and a tensor that does not live on a CUDA device is rejected.
 """
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -83,6 +84,18 @@ _declare("gmc_log_probabilities_backward", [_c_void_p, _c_int] + [_c_void_p] * 8
          + [ctypes.c_float, _c_long, _c_int, _c_void_p])
 _declare("gmc_input_normalise", [_c_float_p, _c_void_p, _c_float_p, _c_float_p, ctypes.c_longlong, _c_int, _c_int, _c_int,
                                  _c_void_p, _c_void_p, _c_void_p])
+
+
+
+
+# struct gmc_matrix of the header: update, momentum, out, rows, cols, update_stride, out_stride, rate
+matrix_struct = struct.Struct("@PPPqqqqf4x")
+lib.gmc_orthogonalise_workspace_bytes.restype = ctypes.c_size_t
+lib.gmc_orthogonalise_workspace_bytes.argtypes = [_c_void_p, _c_int]
+_declare("gmc_orthogonalise", [_c_void_p] + [_c_int] * 3 + [ctypes.c_float] * 4
+         + [_c_void_p, ctypes.c_size_t, _c_void_p])
+_declare("gmc_muon_update", [_c_void_p] + [_c_int] * 3 + [ctypes.c_float] * 5 + [_c_int, ctypes.c_float]
+         + [_c_void_p, ctypes.c_size_t, _c_void_p])
 
 
 class GmcError(RuntimeError):

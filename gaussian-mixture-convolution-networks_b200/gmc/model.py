@@ -136,6 +136,14 @@ class Net(nn.Module):
         for g in self.gmcs:
             g.learn_covariances = flag
 
+    def matrix_parameters(self) -> typing.List[torch.nn.Parameter]:
+        """The parameters that mix features, as gmc.optimisation.Muon takes them: the kernel weights of the convolutions
+        ([n_out, n_in, n_kernel_components, 1], a matrix of n_out rows) and the matrices of the head's linear layers. Kernel
+        positions, covariance factors, normalisations and biases are not matrices of this kind: give them to another
+        optimiser."""
+        return ([g.weights for g in self.gmcs]
+                + ([m.weight for m in self.mlp if isinstance(m, nn.Linear)] if self.mlp is not None else []))
+
     def weight_decay_loss(self) -> Tensor:
         loss = torch.zeros(1, device=next(self.parameters()).device, dtype=torch.float)
         for g in self.gmcs:

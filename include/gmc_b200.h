@@ -44,7 +44,8 @@ enum gmc_status {
     GMC_ERR_UNSUPPORTED = 4,     /* e.g. reduction_n not in {2,4}                                     */
     GMC_ERR_CUDA = 6,            /* a CUDA runtime call failed (see gmc_last_cuda_error)              */
     GMC_ERR_DEVICE_CHECK = 7,    /* a kernel-side bounded wait or self check gave up                  */
-    GMC_ERR_BUILTIN_SCRATCH = 9  /* problem larger than the built-in scratch of a *_noalloc entry point */
+    GMC_ERR_BUILTIN_SCRATCH = 9, /* problem larger than the built-in scratch of a *_noalloc entry point */
+    GMC_ERR_WORKSPACE = 10       /* the workspace is smaller than ..._workspace_bytes asks for        */
 };
 
 /* Element types of the entry points that take a `dtype` (the others are fp32). */
@@ -358,6 +359,35 @@ int gmc_log_probabilities_backward(const void* logits, int dtype, const long lon
                                    const float* stats, const float* entropy, const float* grad_target, const float* grad_entropy,
                                    const float* grad_top, void* grad_logits, long long n_rows, long long n_classes,
                                    long long row_stride, float temperature, long long ignore_index, int n_top, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Orthogonalisation of updates by Newton-Schulz products and the Muon update around it (training glue; no reference
+ * counterpart, its trainers use Adam). Per matrix U [rows, cols]:
+ *   X = U / (|U|_F + epsilon), transposed if rows > cols; `steps` times: A = X X^T, X <- a X + (b A + c A A) X;
+ *   out = X, transposed back. Singular values of U / |U| end up near 1 for (a, b, c) = (3.4445, -4.7750, 2.0315), 5 steps.
+ * gmc_muon_update first updates the running average (fp32), m <- momentum m + (1 - momentum) U, takes U <- (nesterov) ?
+ * (1 - momentum) U + momentum m : m, and then out <- decay out - rate X: out holds the parameters.
+ * `matrices` is a HOST array; update, out are of `dtype` with unit column stride, *_stride elements (>= cols) between rows;
+ * momentum is contiguous fp32. Matrices may differ in shape; 1 <= rows, cols <= 32768. A zero matrix gives zero; NaN or
+ * infinity in a matrix makes that matrix NaN. out may be update (the same address and stride), no other overlap is allowed
+ * within a call, and no matrix may appear twice. Products are accurate to fp32 rounding whatever `dtype`.
+ * 1 <= steps <= 32; coefficients whose iterates leave |X| < 1.4, |b A + c A A| < 3.9 for singular values in [0, 1] are
+ * refused (GMC_ERR_UNSUPPORTED); 1e-30 <= epsilon <= 1e30; 0 <= momentum < 1.
+ * workspace: gmc_orthogonalise_workspace_bytes (0 = sizes out of range; depends on the shapes only), aligned to 1024 bytes,
+ * content undefined before and after; concurrent calls need one each. Nothing is allocated, kept or synchronised.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct gmc_matrix {
+    const void* update;
+    float* momentum;            /* gmc_muon_update only */
+    void* out;
+    long long rows, cols, update_stride, out_stride;
+    float rate;                 /* gmc_muon_update only */
+} gmc_matrix;
+size_t gmc_orthogonalise_workspace_bytes(const gmc_matrix* matrices, int n_matrices);
+int gmc_orthogonalise(const gmc_matrix* matrices, int n_matrices, int dtype, int steps, float a, float b, float c, float epsilon,
+                      void* workspace, size_t workspace_bytes, void* stream);
+int gmc_muon_update(const gmc_matrix* matrices, int n_matrices, int dtype, int steps, float a, float b, float c, float epsilon,
+                    float momentum, int nesterov, float decay, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * gmc_mhem_fit_forward for callers that have no scratch memory to give. (No counterpart in the reference, which

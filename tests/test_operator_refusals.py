@@ -45,3 +45,44 @@ def test_log_probabilities_refuses_what_it_cannot_do():
         log_probabilities(torch.zeros(2, 0))
     with pytest.raises(GmcError, match="at least one class"):
         log_probabilities([1.0, 2.0])
+
+
+def test_orthogonalise_argument_checks():
+    from gmc import _native
+    address = 1024
+
+    def run(rows=4, cols=5, us=5, os_=5, update=16, out=16, momentum=16, dtype=0, steps=5, abc=(3.4445, -4.775, 2.0315), eps=1e-7,
+            n=1, work=address, size=1 << 30, muon=False, beta=0.9):
+        m = _native.matrix_struct.pack(update, momentum, out, rows, cols, us, os_, 0.1)
+        if muon:
+            return _native.lib.gmc_muon_update(m, n, dtype, steps, *abc, eps, beta, 1, 1.0, work, size, NULL)
+        return _native.lib.gmc_orthogonalise(m, n, dtype, steps, *abc, eps, work, size, NULL)
+
+    assert run(rows=0) == 1 and run(cols=0) == 1 and run(rows=32769) == 1 and run(us=4) == 1 and run(os_=4) == 1 and run(n=-1) == 1
+    assert run(dtype=3) == 4 and run(steps=0) == 4 and run(steps=33) == 4 and run(eps=0.0) == 4 and run(eps=float("nan")) == 4
+    assert run(abc=(10.0, 0.0, 0.0)) == 4 and run(abc=(float("nan"), 0.0, 0.0)) == 4 and run(abc=(1.0, -4.0, 0.0)) == 4
+    assert run(update=0) == 3 and run(out=0) == 3 and run(work=0) == 3 and run(work=address + 16) == 4
+    assert run(size=64) == 10 and run(n=0, update=0) == 0
+    assert run(muon=True, momentum=0) == 3 and run(muon=True, beta=1.0) == 4 and run(muon=True, beta=-0.1) == 4
+    m = _native.matrix_struct.pack(16, 0, 16, 300, 500, 500, 500, 0.0)
+    assert _native.lib.gmc_orthogonalise_workspace_bytes(m, 1) > 0
+    assert _native.lib.gmc_orthogonalise_workspace_bytes(_native.matrix_struct.pack(16, 0, 16, 0, 5, 5, 5, 0.0), 1) == 0
+
+
+def test_optimisation_refuses_what_it_cannot_do():
+    from gmc._native import GmcError
+    from gmc.optimisation import Muon, muon_update, orthogonalise
+    t = torch.zeros(3, 4)
+    with pytest.raises(GmcError, match="no CPU implementation"):
+        orthogonalise(t)
+    with pytest.raises(GmcError, match="three numbers"):
+        orthogonalise(t, coefficients=(1.0, 2.0))
+    with pytest.raises(GmcError, match="one entry per parameter"):
+        muon_update([t], [t], [], 0.1)
+    with pytest.raises(GmcError, match="finite"):
+        muon_update([t], [t], [t], float("nan"))
+    with pytest.raises(GmcError, match="no CPU implementation"):
+        muon_update([t], [t], [t], 0.1)
+    with pytest.raises(GmcError, match="two or more axes"):
+        Muon([torch.nn.Parameter(torch.zeros(5))])
+    muon_update([], [], [], 0.1)

@@ -1,0 +1,294 @@
+"""GPU: orthogonalisation by Newton-Schulz products and the Muon update against 64-bit restatements.
+
+Error bound. The operands carry 22 bits where a 32-bit evaluation carries 24, and the polynomial amplifies either by the same
+factors: the error (2-norm over the matrix) may be 2^2 times that of the plain 32-bit evaluation of the same formula on the
+same input, plus 2^-20 of the result's norm for inputs on which the plain one is exact by luck, plus half a step of the
+output's type on every value."""
+import copy
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _plain(u, steps, coefficients, epsilon):
+    a, b, c = coefficients
+    tall = u.shape[-2] > u.shape[-1]
+    x = u.mT if tall else u
+    x = x / (x.square().sum(dim=(-1, -2), keepdim=True).sqrt() + epsilon)
+    for _ in range(steps):
+        g = x @ x.mT
+        x = a * x + (b * g + c * (g @ g)) @ x
+    return x.mT if tall else x
+
+
+def _check(got, u, steps=5, coefficients=COEFFICIENTS, epsilon=1e-7):
+    ref = _plain(u.double(), steps, coefficients, epsilon)
+    plain = _plain(u.float(), steps, coefficients, epsilon).double()
+    assert got.shape == u.shape and got.dtype == u.dtype
+    norm = lambda t: torch.linalg.matrix_norm(t)  # noqa: E731
+    half = torch.finfo(u.dtype).eps / 2 if u.dtype != torch.float32 else 0.0
+    bound = 4 * norm(plain - ref) + (2.0 ** -20 + half) * norm(ref) + torch.finfo(u.dtype).tiny * math.sqrt(u.shape[-1] * u.shape[-2])
+    off = norm(got.double() - ref)
+    assert (off <= bound).all(), f"{(off / norm(ref)).max().item():.3e} against {(bound / norm(ref)).min().item():.3e}"
+
+
+def _update(*shape, seed=0, dtype=torch.float32):
+    """A few strong directions over noise, as gradients have them."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    *lead, m, n = shape
+    rank = max(1, min(m, n, 12) // 2)
+    strong = (torch.randn(*lead, m, rank, device="cuda", generator=g) * torch.exp(-0.5 * torch.arange(rank, device="cuda"))) \
+        @ torch.randn(*lead, rank, n, device="cuda", generator=g)
+    return (1e-3 * (strong + 0.3 * torch.randn(*shape, device="cuda", generator=g))).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n", [(1, 1), (1, 7), (9, 1), (5, 5), (16, 40), (64, 64), (64, 160), (65, 63), (127, 129), (128, 128),
+                                 (129, 127), (130, 600), (257, 64), (64, 2000), (3000, 17), (300, 1000), (1000, 300), (513, 769),
+                                 (1025, 1031)])
+def test_orthogonalise(m, n, dtype):
+    from gmc.optimisation import orthogonalise
+    u = _update(m, n, seed=m * 7 + n, dtype=dtype)
+    before = u.clone()
+    _check(orthogonalise(u), u)
+    assert torch.equal(u, before)
+
+
+def test_a_long_inner_axis():
+    """The sums of X X^T over 20000 columns, all of one sign on the diagonal."""
+    from gmc.optimisation import orthogonalise
+    u = _update(200, 20000, seed=5)
+    _check(orthogonalise(u), u)
+
+
+@pytest.mark.parametrize("m,n", [(20, 50), (200, 333)])
+def test_inputs_at_the_edges(m, n):
+    """Rank one, nearly rank one, one element, equal elements, very small and very large values, orthogonal rows."""
+    from gmc.optimisation import orthogonalise
+    g = torch.Generator(device="cuda").manual_seed(1)
+    left, right = torch.randn(m, 1, device="cuda", generator=g), torch.randn(1, n, device="cuda", generator=g)
+    one = torch.zeros(m, n, device="cuda")
+    one[m // 2, n // 3] = -2.5
+    inputs = [left @ right, left @ right + 1e-4 * torch.randn(m, n, device="cuda", generator=g), one,
+              torch.full((m, n), 3.0, device="cuda"), torch.linalg.qr(torch.randn(n, m, device="cuda", generator=g))[0].mT.contiguous()]
+    for u in inputs:
+        _check(orthogonalise(u), u)
+    for scale in (1e-22, 1e22):                                  # squares beyond fp32: the norm is a 64-bit sum
+        u = scale * inputs[1]
+        got, want = orthogonalise(u, epsilon=1e-30), orthogonalise(inputs[1], epsilon=1e-30)
+        # the input is rounded by the scaling (2^-24 a value), and its error grows at most 4^5 times
+        assert torch.linalg.matrix_norm(got - want) <= 4 ** 5 * 2.0 ** -23 * torch.linalg.matrix_norm(want)
+    assert (orthogonalise(torch.zeros(m, n, device="cuda")) == 0).all()
+
+
+@pytest.mark.parametrize("m,n", [(12, 30), (140, 260)])
+def test_nan_and_infinity_stay_in_their_matrix(m, n):
+    from gmc.optimisation import orthogonalise
+    u = _update(4, m, n)
+    clean = orthogonalise(u)
+    u[1, m - 1, n - 1] = math.nan
+    u[2, 0, 0] = math.inf
+    got = orthogonalise(u)
+    assert got[1].isnan().all() and got[2].isnan().all()
+    assert torch.equal(got[[0, 3]], clean[[0, 3]])
+
+
+@pytest.mark.parametrize("steps,coefficients", [(1, COEFFICIENTS), (8, COEFFICIENTS), (6, (1.875, -1.25, 0.375)), (7, (1.5, -0.5, 0.0))])
+@pytest.mark.parametrize("m,n", [(24, 70), (150, 200)])
+def test_steps_and_coefficients(m, n, steps, coefficients):
+    from gmc.optimisation import orthogonalise
+    u = _update(m, n, seed=3)
+    _check(orthogonalise(u, steps=steps, coefficients=coefficients), u, steps, coefficients)
+
+
+@pytest.mark.parametrize("m,n", [(48, 100), (400, 256)])
+def test_singular_values_end_near_one(m, n):
+    from gmc.optimisation import orthogonalise
+    u = torch.randn(m, n, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))
+    s = torch.linalg.svdvals(orthogonalise(u).double())
+    # the smallest singular value of these inputs is above 0.01 of the norm: five steps bring it into the band
+    assert s.max() < 1.21 and s.min() > 0.3
+
+
+def test_batches_lists_and_strides():
+    from gmc.optimisation import orthogonalise
+    u = _update(3, 2, 70, 90)
+    got = orthogonalise(u)
+    _check(got, u)
+    for i in range(3):
+        for j in range(2):
+            assert torch.equal(got[i, j], orthogonalise(u[i, j]))
+    many = _update(101, 10, 12)
+    assert torch.equal(orthogonalise(many)[77], orthogonalise(many[77]))
+    many = _update(50, 130, 70)
+    got = orthogonalise(many)
+    assert torch.equal(got[49], orthogonalise(many[49])) and torch.equal(got[0], orthogonalise(many[0]))
+    shapes = [(30, 40), (300, 140), (1, 9), (130, 700), (64, 64)]
+    mixed = [_update(m, n, seed=i) for i, (m, n) in enumerate(shapes)]
+    for o, t in zip(orthogonalise(mixed), mixed):
+        assert torch.equal(o, orthogonalise(t))
+    for size in (40, 200):
+        wide = _update(size, 3 * size + 5)
+        for view in (wide[:, 3:3 + size], wide[::2, 1:size], wide[:, :size].t(), wide[:1].expand(size, -1)):
+            assert torch.equal(orthogonalise(view), orthogonalise(view.contiguous()))
+    assert orthogonalise(torch.zeros(0, 4, 5, device="cuda")).shape == (0, 4, 5)
+    assert orthogonalise(torch.zeros(4, 0, device="cuda")).shape == (4, 0) and orthogonalise([]) == []
+
+
+def _muon_reference(p, g, m, lr, momentum, weight_decay, nesterov):
+    p, g, m = p.double(), g.double(), m.double()
+    m = momentum * m + (1 - momentum) * g
+    u = (1 - momentum) * g + momentum * m if nesterov else m
+    rows, cols = p.shape[0], p[0].numel()
+    x = _plain(u.view(rows, cols), 5, COEFFICIENTS, 1e-7).view(p.shape)
+    return (1 - lr * weight_decay) * p - lr * math.sqrt(max(1.0, rows / cols)) * x, m
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nesterov", [True, False])
+@pytest.mark.parametrize("shapes", [[(8, 1, 5, 1), (16, 8, 5, 1), (64, 32, 5, 1), (40, 64)], [(300, 129), (129, 400), (20, 7)], [(640, 2)]])
+def test_muon_update(shapes, nesterov, dtype):
+    from gmc.optimisation import muon_update
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    params = [torch.randn(s, device="cuda", generator=gen).to(dtype) for s in shapes]
+    grads = [_update(s[0], math.prod(s[1:]), seed=i, dtype=dtype).view(s) for i, s in enumerate(shapes)]
+    momenta = [_update(s[0], math.prod(s[1:]), seed=50 + i).view(s) for i, s in enumerate(shapes)]
+    lr, momentum, weight_decay = 0.05, 0.9, 0.1
+    want = [_muon_reference(p, g, m, lr, momentum, weight_decay, nesterov) for p, g, m in zip(params, grads, momenta)]
+    before, versions = [p.clone() for p in params], [p._version for p in params]
+    muon_update(params, grads, momenta, lr, momentum, weight_decay, nesterov)
+    for p, m, (wp, wm), old, version in zip(params, momenta, want, before, versions):
+        assert p._version > version
+        # momentum: three roundings of fp32
+        assert ((m.double() - wm).abs() <= 3 * 2.0 ** -24 * (wm.abs() + 0.01)).all()
+        # parameter: its own rounding, and an update of lr sqrt(..) times an orthogonal matrix whose relative error is below
+        # 4^5 times the three roundings of the momentum (the polynomial's largest slope is below 4) and 2^-12 for the products
+        half = torch.finfo(dtype).eps / 2
+        step = torch.linalg.vector_norm(wp - old.double())
+        assert torch.linalg.vector_norm(p.double() - wp) <= (2 * half + 3 * 2.0 ** -24) * torch.linalg.vector_norm(wp) \
+            + (4 ** 5 * 3 * 2.0 ** -24 + 2.0 ** -12) * step
+
+
+def test_optimiser_steps_and_state():
+    """Three steps of the class on an fp32 and a bf16 parameter against the restatement; the state survives a save and load in
+    32 bits; parameters without a gradient are left alone."""
+    from gmc.optimisation import Muon
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    params = [torch.nn.Parameter(torch.randn(48, 96, device="cuda", generator=gen)),
+              torch.nn.Parameter(torch.randn(130, 200, device="cuda", generator=gen).bfloat16()),
+              torch.nn.Parameter(torch.randn(10, 10, device="cuda", generator=gen))]
+    opt = Muon(params, lr=0.03, momentum=0.8, weight_decay=0.05)
+    idle = params[2].detach().clone()
+    mom = [torch.zeros_like(p, dtype=torch.float32) for p in params[:2]]
+    for step in range(3):
+        for i, p in enumerate(params[:2]):
+            p.grad = _update(*p.shape, seed=10 * step + i, dtype=p.dtype)
+        want = [_muon_reference(p.detach(), p.grad, m, 0.03, 0.8, 0.05, True) for p, m in zip(params, mom)]
+        if step == 2:
+            other = Muon(params, lr=1.0)
+            other.load_state_dict(copy.deepcopy(opt.state_dict()))
+            opt = other
+            for p, m in zip(params, mom):
+                assert opt.state[p]["momentum_buffer"].dtype == torch.float32 and torch.equal(opt.state[p]["momentum_buffer"], m)
+        opt.step()
+        mom = [opt.state[p]["momentum_buffer"].clone() for p in params[:2]]
+        for p, m, (wp, wm) in zip(params, mom, want):
+            assert torch.linalg.vector_norm(m.double() - wm) <= 2.0 ** -22 * torch.linalg.vector_norm(wm)
+            half = torch.finfo(p.dtype).eps / 2
+            assert torch.linalg.vector_norm(p.detach().double() - wp) <= (2 * half + 2.0 ** -16) * torch.linalg.vector_norm(wp)
+    assert torch.equal(params[2], idle) and params[2] not in opt.state
+
+
+def test_captured_and_replayed_on_another_stream():
+    from gmc.optimisation import muon_update, orthogonalise
+    shapes = [(20, 45), (200, 150)]
+    params = [torch.randn(s, device="cuda") for s in shapes]
+    grads = [_update(*s, seed=1) for s in shapes]
+    momenta = [torch.zeros(s, device="cuda") for s in shapes]
+    start = [t.clone() for t in params + momenta]
+    eager = []
+    for _ in range(2):
+        muon_update(params, grads, momenta, 0.02)
+        eager.append([t.clone() for t in params + momenta])
+    graphs, outs = [], []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        muon_update(params, grads, momenta, 0.02)
+        orthogonalise(grads)
+    torch.cuda.current_stream().wait_stream(side)
+    for _ in range(2):                                              # two graphs, each with its own workspace
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            muon_update(params, grads, momenta, 0.02)
+            outs.append(orthogonalise(grads))
+        graphs.append(graph)
+    for t, s in zip(params + momenta, start):
+        t.copy_(s)
+    want = orthogonalise(grads)
+    for i, graph in enumerate(graphs):
+        graph.replay()
+        for t, e in zip(params + momenta, eager[i]):
+            assert torch.equal(t, e)
+        for a, b in zip(outs[i], want):
+            assert torch.equal(a, b)
+
+
+def test_two_calls_at_once():
+    from gmc.optimisation import orthogonalise
+    u = [_update(300, 500, seed=i) for i in range(2)]
+    want = [orthogonalise(v) for v in u]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in u], []
+    for s, v in zip(streams, u):
+        with torch.cuda.stream(s):
+            got.append(orthogonalise(v))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_training_step_of_the_network():
+    """Loss, gradient and both optimisers together: log_probabilities -> backward -> Muon on the matrices, Adam on the rest.
+    The matrices move by the restatement's update of the gradients that the backward pass left."""
+    import gmc.model as model
+    import synthetic_inputs as synthetic
+    from gmc.optimisation import Muon
+    cfg = model.Config(n_dims=2)
+    cfg.layers = [model.Layer(4, 1, 24, 12), model.Layer(10, 1, 16, 8)]
+    cfg.mlp = [24, 10]
+    torch.manual_seed(11)
+    net = model.Net(config=cfg).cuda().train()
+    x = synthetic.fit_target_2d(6, 1, 20, 5)
+    x[..., 0] = x[..., 0].abs() + 0.1
+    x, t = x.cuda(), torch.arange(6, device="cuda") % 10
+    matrices = net.matrix_parameters()
+    assert len(matrices) == 4
+    chosen = {id(p) for p in matrices}
+    optimisers = [Muon(matrices, lr=0.01, momentum=0.9), torch.optim.Adam([p for p in net.parameters() if id(p) not in chosen], lr=1e-3)]
+    for _ in range(2):
+        for o in optimisers:
+            o.zero_grad()
+        r = net.log_probabilities(x, t)
+        (-r.target.mean() - 0.01 * r.entropy.mean()).backward()
+        before = [(p.detach().clone(), p.grad.clone(), optimisers[0].state[p].get("momentum_buffer", torch.zeros_like(p)).clone())
+                  for p in matrices]
+        for o in optimisers:
+            o.step()
+        for p, (old, g, m) in zip(matrices, before):
+            assert torch.isfinite(p).all() and (g != 0).any()
+            want, _ = _muon_reference(old, g, m, 0.01, 0.9, 0.0, True)
+            bound = 2.0 ** -23 * torch.linalg.vector_norm(want) + (4 ** 5 * 3 * 2.0 ** -24 + 2.0 ** -12) * torch.linalg.vector_norm(want - old)
+            assert torch.linalg.vector_norm(p.detach().double() - want) <= bound
+    net.eval()
+    with torch.no_grad():
+        kernels = net.gmcs[0].kernels()
+        before = kernels.clone()
+        matrices[0].grad = torch.ones_like(matrices[0])
+        optimisers[0].step()
+        assert not torch.equal(net.gmcs[0].kernels(), before)          # the cached kernel mixture sees the update
