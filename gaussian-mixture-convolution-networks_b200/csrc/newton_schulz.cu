@@ -12,6 +12,7 @@
 // shared memory (128-byte swizzle), padded with zeros: loading an operand tile is one contiguous bulk copy, whatever the
 // matrix's shape, and X serves both as rows (X X^T, K = columns) and across (B X, K = rows) without a transposed copy.
 // A and A A are symmetric: only tiles on and below the diagonal are computed, their mirror images are stored with them.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -20,13 +21,15 @@
 namespace gmc {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kMaxMatrices = 48;                 // descriptors of one launch (kernel parameter)
 constexpr int kBlockBytes = 128 * 64 * 2;        // one block of one plane
 constexpr int kStageBytes = 4 * kBlockBytes;     // hi and lo of both operands, 64 wide in K
 constexpr int kStages = 3;
 constexpr int kProductSmem = kStages * kStageBytes + 1024;
 constexpr float kScaleX = 32768.f, kScaleA = 32768.f, kScaleB = 16384.f;
-constexpr int kNormElements = 16384;             // elements of a matrix per CTA of the norm
+constexpr int kNormElements = 4096;              // elements of a matrix per CTA of the norm
 
 // The matrices of a launch. Wide form: m <= n after the transposition.
 struct Matrix {
@@ -72,14 +75,18 @@ __global__ void __launch_bounds__(256) norm_kernel(const __grid_constant__ Batch
     const Matrix& m = b.m[which];
     const long long total = (long long)m.rows * m.cols;
     const long long first = (long long)(int(blockIdx.x) - m.norm_first) * kNormElements;
-    const long long end = min(total, first + kNormElements);
+    const int count = int(min((long long)kNormElements, total - first));
+    const int row0 = int(first / m.cols), col0 = int(first - (long long)row0 * m.cols);
     double s = 0.;
-    for (long long i = first + threadIdx.x; i < end; i += 256) {
-        const long long r = i / m.cols, c = i - r * m.cols;
-        float u = load_float<T>(m.update, r * m.update_stride + c);
+    const unsigned cols = unsigned(m.cols);
+#pragma unroll 4
+    for (int i = threadIdx.x; i < count; i += 256) {
+        const unsigned at = unsigned(col0 + i), r = at / cols;
+        float u = load_float<T>(m.update, (row0 + (long long)r) * m.update_stride + (at - r * cols));
         if constexpr (MUON) {
-            const float now = mo.beta * m.momentum[i] + mo.one_minus_beta * u;
-            m.momentum[i] = now;
+            float* p = m.momentum + first + i;
+            const float now = mo.beta * *p + mo.one_minus_beta * u;
+            *p = now;
             u = mo.nesterov ? mo.one_minus_beta * u + mo.beta * now : now;
         }
         s += double(u) * double(u);
@@ -381,16 +388,212 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
     }
 }
 
+// ---- matrices with a short side: the whole chain in one launch, fp32 -------------------------------------------------
+// One cluster per matrix. Each CTA keeps X for its share of the columns in shared memory over all steps; per step the CTAs
+// add up their shares of X X^T over distributed shared memory (CTA q sums rows q, q + ranks, .. and hands them to all), form
+// b A + c A A (each for itself) and multiply their own columns with it in place. Nothing goes through global memory between
+// the update's elements and the result, there is one launch instead of three per step, and the products are fp32.
+constexpr int kShortThreads = 512;
+constexpr int kShortRows = 64;
+constexpr int kShortPartials = 8448;             // floats: groups x tiles x 16 partial sums of X X^T
+struct ShortBatch {
+    Matrix m[kMaxMatrices];
+};
+__host__ __device__ inline int short_padded_rows(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+__host__ __device__ inline int short_columns(int cols, int ranks) { return ((cols + ranks - 1) / ranks + 3) & ~3; }
+__host__ __device__ inline int short_pitch(int columns) { return ((columns + 27) / 32) * 32 + 4; }       // = 4 mod 32 banks, >= columns
+__host__ __device__ inline size_t short_smem(int rows, int cols, int ranks) {
+    const size_t mp = short_padded_rows(rows);
+    return (mp * short_pitch(short_columns(cols, ranks)) + 2 * mp * (mp + 4) + kShortPartials) * sizeof(float);
+}
+
+template <typename T, bool MUON>
+__global__ void __launch_bounds__(kShortThreads, 1) short_kernel(const __grid_constant__ ShortBatch b, int ranks, Momentum mo, int steps, float ca,
+                                                                 float cb, float cc, float epsilon) {
+    extern __shared__ __align__(16) float smem[];
+    __shared__ double warp_sum[kShortThreads / 32], cta_sum;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const Matrix& m = b.m[blockIdx.x / unsigned(ranks)];
+    const int rank = int(blockIdx.x % unsigned(ranks));
+    const bool tall = m.rows > m.cols;
+    const int wide_rows = tall ? m.cols : m.rows, wide_cols = tall ? m.rows : m.cols;
+    const int mp = short_padded_rows(wide_rows), columns = short_columns(wide_cols, ranks), pitch = short_pitch(columns), gp = mp + 4;
+    const int col0 = rank * columns, here = max(0, min(columns, wide_cols - col0));
+    float* x = smem;
+    float* gram = x + mp * pitch;                // A, complete
+    float* poly = gram + mp * gp;                // the CTA's share of A, then b A + c A A
+    float* partial = poly + mp * gp;
+
+    for (int i = tid; i < mp * pitch; i += kShortThreads) x[i] = 0.f;
+    __syncthreads();
+    double s = 0.;
+    for (int i = tid; i < wide_rows * here; i += kShortThreads) {
+        // neighbouring threads read along a row of the update
+        const int r = tall ? i % wide_rows : i / here, c = tall ? i / wide_rows : i % here;
+        const long long rr = tall ? col0 + c : r, cc_ = tall ? r : col0 + c;
+        float u = load_float<T>(m.update, rr * m.update_stride + cc_);
+        if constexpr (MUON) {
+            float* at = m.momentum + rr * m.cols + cc_;
+            const float now = mo.beta * *at + mo.one_minus_beta * u;
+            *at = now;
+            u = mo.nesterov ? mo.one_minus_beta * u + mo.beta * now : now;
+        }
+        x[r * pitch + c] = u;
+        s += double(u) * double(u);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) warp_sum[warp] = s;
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < kShortThreads / 32; ++w) s += warp_sum[w];
+        cta_sum = s;
+    }
+    cluster.sync();
+    s = 0.;
+    for (int q = 0; q < ranks; ++q) s += *cluster.map_shared_rank(&cta_sum, q);
+    const float norm = float(sqrt(s) + double(epsilon));
+    for (int i = tid; i < wide_rows * here; i += kShortThreads) {
+        const int r = i / here, c = i - r * here;
+        x[r * pitch + c] /= norm;
+    }
+    __syncthreads();
+
+    const int tiles_side = mp / 4, tiles = tiles_side * (tiles_side + 1) / 2;
+    // this thread's 4 x 4 tile on or below the diagonal, and its share of a long axis
+    const int groups = min(kShortThreads / tiles, kShortPartials / (tiles * 16));
+    const int tile = tid % tiles, group = tid / tiles;
+    int ti = 0;
+    while ((ti + 1) * (ti + 2) / 2 <= tile) ++ti;
+    const int tj = tile - ti * (ti + 1) / 2;
+
+    // symmetric product rows x rows^T of `length` columns (a multiple of 4) of `from`; sum over the CTA's groups handed to
+    // store(row, column, value) for each element on or below the diagonal tiles
+    auto symmetric = [&](const float* from, int from_pitch, int length, auto&& store) {
+        if (group < groups) {
+            float acc[4][4] = {};
+            for (int c = group * 4; c < length; c += groups * 4) {
+                float4 p[4], q[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    p[i] = *reinterpret_cast<const float4*>(from + (ti * 4 + i) * from_pitch + c);
+                    q[i] = *reinterpret_cast<const float4*>(from + (tj * 4 + i) * from_pitch + c);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[i][j] += p[i].x * q[j].x + p[i].y * q[j].y + p[i].z * q[j].z + p[i].w * q[j].w;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<float4*>(partial + ((group * tiles + tile) * 4 + i) * 4) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+        }
+        __syncthreads();
+        auto element = [&](int e, float v) {
+            int i = 0;
+            const int t = e >> 4;
+            while ((i + 1) * (i + 2) / 2 <= t) ++i;
+            store(i * 4 + ((e >> 2) & 3), (t - i * (i + 1) / 2) * 4 + (e & 3), v);
+        };
+        if (groups <= 16) {
+            for (int e = tid; e < tiles * 16; e += kShortThreads) {
+                float v = 0.f;
+                for (int g = 0; g < groups; ++g) v += partial[g * tiles * 16 + e];
+                element(e, v);
+            }
+        } else {
+            for (int e = warp; e < tiles * 16; e += kShortThreads / 32) {
+                float v = 0.f;
+                for (int g = lane; g < groups; g += 32) v += partial[g * tiles * 16 + e];
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+                if (lane == 0) element(e, v);
+            }
+        }
+    };
+
+    for (int step = 0; step < steps; ++step) {
+        symmetric(x, pitch, columns, [&](int i, int j, float v) {
+            poly[i * gp + j] = v;
+            poly[j * gp + i] = v;
+        });
+        if (ranks > 1) {
+            cluster.sync();
+            // rows rank, rank + ranks, .. : sum over the CTAs in their order, to all of them
+            const int quads = mp / 4;
+            for (int i = tid; i < ((mp - rank + ranks - 1) / ranks) * quads; i += kShortThreads) {
+                const int r = rank + (i / quads) * ranks, c = (i % quads) * 4;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int q = 0; q < ranks; ++q) {
+                    const float4 w = *reinterpret_cast<const float4*>(cluster.map_shared_rank(poly, q) + r * gp + c);
+                    v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+                }
+                for (int q = 0; q < ranks; ++q) *reinterpret_cast<float4*>(cluster.map_shared_rank(gram, q) + r * gp + c) = v;
+            }
+            cluster.sync();
+        } else {
+            __syncthreads();
+        }
+        const float* full = ranks > 1 ? gram : poly;
+        float* to = ranks > 1 ? poly : gram;
+        symmetric(full, gp, mp, [&](int i, int j, float v) {
+            v = cb * full[i * gp + j] + cc * v;
+            to[i * gp + j] = v;
+            to[j * gp + i] = v;
+        });
+        __syncthreads();
+        // X <- a X + P X in place: a warp holds all rows of 4 * 32 / tiles_side columns, so what it overwrites it alone reads
+        const int col_tiles = 32 / tiles_side, row = (lane % tiles_side) * 4, my_col = (lane / tiles_side) * 4;
+        for (int c0 = warp * col_tiles * 4; c0 < columns; c0 += (kShortThreads / 32) * col_tiles * 4) {
+            const int c = c0 + my_col;
+            const bool in = c < columns;
+            float acc[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float4 v = in ? *reinterpret_cast<const float4*>(x + (row + i) * pitch + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+                acc[i][0] = ca * v.x, acc[i][1] = ca * v.y, acc[i][2] = ca * v.z, acc[i][3] = ca * v.w;
+            }
+            if (in) {
+#pragma unroll 4
+                for (int k = 0; k < mp; ++k) {
+                    const float4 p = *reinterpret_cast<const float4*>(to + k * gp + row);
+                    const float4 v = *reinterpret_cast<const float4*>(x + k * pitch + c);
+                    const float pr[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        acc[i][0] += pr[i] * v.x, acc[i][1] += pr[i] * v.y, acc[i][2] += pr[i] * v.z, acc[i][3] += pr[i] * v.w;
+                    }
+                }
+            }
+            __syncwarp();
+            if (in)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<float4*>(x + (row + i) * pitch + c) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+        }
+        __syncthreads();
+    }
+    T* out = static_cast<T*>(m.out);
+    for (int i = tid; i < wide_rows * here; i += kShortThreads) {
+        const int r = tall ? i % wide_rows : i / here, c = tall ? i / wide_rows : i % here;
+        const long long o = tall ? (col0 + c) * m.out_stride + r : r * m.out_stride + col0 + c;
+        const float v = x[r * pitch + c];
+        out[o] = T(MUON ? float(out[o]) * mo.decay - m.rate * v : v);
+    }
+    cluster.sync();                                                   // no CTA leaves while its shared memory is read or written
+}
+
 // ---- host side -------------------------------------------------------------------------------------------------------
 int ceil_div(long long a, long long b) { return int((a + b - 1) / b); }
 
-int fill(const gmc_matrix* matrices, int n, Batch* batch, size_t* bytes, uint8_t* workspace) {
+void fill(const gmc_matrix* matrices, const int* which, int n, Batch* batch, size_t* bytes, uint8_t* workspace) {
     Batch& b = *batch;
     b.n = n;
     long long x_blocks = 0, gram_blocks = 0;
     b.norm_ctas = b.gram_ctas = b.step_ctas = b.blocks = 0;
     for (int i = 0; i < n; ++i) {
-        const gmc_matrix& g = matrices[i];
+        const gmc_matrix& g = matrices[which[i]];
         Matrix& m = b.m[i];
         const long long wide_rows = g.rows < g.cols ? g.rows : g.cols, wide_cols = g.rows < g.cols ? g.cols : g.rows;
         m.update = g.update;
@@ -429,7 +632,6 @@ int fill(const gmc_matrix* matrices, int n, Batch* batch, size_t* bytes, uint8_t
     b.poly = reinterpret_cast<__half*>(take(size_t(gram_blocks) * kBlockBytes));
     b.partial = reinterpret_cast<double*>(take(size_t(b.norm_ctas) * sizeof(double)));
     *bytes = at;
-    return GMC_OK;
 }
 
 constexpr long long kMaxSide = 32768;
@@ -490,6 +692,96 @@ int run_batch(const Batch& b, int steps, float ca, float cb, float cc, float eps
     return GMC_OK;
 }
 
+// A matrix goes to the one-launch kernel if its short side fits the tile grid and X fits the shared memory of eight CTAs.
+constexpr size_t kShortSmemLimit = 200 * 1024;
+bool is_short(const gmc_matrix& g) {
+    const long long rows = g.rows < g.cols ? g.rows : g.cols, cols = g.rows < g.cols ? g.cols : g.rows;
+    return rows <= kShortRows && short_smem(int(rows), int(cols), 8) <= kShortSmemLimit;
+}
+
+template <typename T, bool MUON>
+int run_short(const gmc_matrix* matrices, const int* which, int n, int steps, float ca, float cb, float cc, float epsilon,
+              const Momentum& mo, cudaStream_t stream) {
+    ShortBatch b;
+    int ranks = 1, device = 0, n_sm = 0;
+    GMC_CUDA_TRY(cudaGetDevice(&device));
+    GMC_CUDA_TRY(cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, device));
+    size_t smem = 0;
+    for (int i = 0; i < n; ++i) {
+        const gmc_matrix& g = matrices[which[i]];
+        Matrix& m = b.m[i];
+        m.update = g.update;
+        m.momentum = g.momentum;
+        m.out = g.out;
+        m.update_stride = g.update_stride;
+        m.out_stride = g.out_stride;
+        m.rows = int(g.rows);
+        m.cols = int(g.cols);
+        m.rate = g.rate;
+        const int rows = m.rows < m.cols ? m.rows : m.cols, cols = m.rows < m.cols ? m.cols : m.rows;
+        while (ranks < 8 && ((cols / ranks > 40 && 2 * ranks * n <= n_sm) || short_smem(rows, cols, ranks) > kShortSmemLimit)) ranks *= 2;
+    }
+    for (int i = 0; i < n; ++i) {
+        const int rows = b.m[i].rows < b.m[i].cols ? b.m[i].rows : b.m[i].cols, cols = b.m[i].rows < b.m[i].cols ? b.m[i].cols : b.m[i].rows;
+        const size_t need = short_smem(rows, cols, ranks);
+        smem = need > smem ? need : smem;
+    }
+    GMC_CUDA_TRY(cudaFuncSetAttribute(short_kernel<T, MUON>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kShortSmemLimit)));
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(unsigned(n * ranks));
+    config.blockDim = dim3(kShortThreads);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attribute;
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = unsigned(ranks);
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    GMC_CUDA_TRY(cudaLaunchKernelEx(&config, short_kernel<T, MUON>, b, ranks, mo, steps, ca, cb, cc, epsilon));
+    return GMC_OK;
+}
+
+template <typename T, bool MUON>
+int run_typed(const gmc_matrix* matrices, int n, int steps, float ca, float cb, float cc, float epsilon, const Momentum& mo,
+              void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+    int which[kMaxMatrices], count = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+        for (int i = 0; i <= n; ++i) {
+            if (i < n && is_short(matrices[i]) == (pass == 0)) which[count++] = i;
+            if (count == kMaxMatrices || (i == n && count > 0)) {
+                if (pass == 0) {
+                    if (int s = run_short<T, MUON>(matrices, which, count, steps, ca, cb, cc, epsilon, mo, stream)) return s;
+                } else {
+                    Batch b;
+                    size_t bytes = 0;
+                    fill(matrices, which, count, &b, &bytes, static_cast<uint8_t*>(workspace));
+                    if (bytes > workspace_bytes) return GMC_ERR_WORKSPACE;
+                    if (int s = run_batch<T, MUON>(b, steps, ca, cb, cc, epsilon, mo, stream)) return s;
+                }
+                count = 0;
+            }
+        }
+    }
+    return GMC_OK;
+}
+
+size_t workspace_bytes_of(const gmc_matrix* matrices, int n) {
+    int which[kMaxMatrices], count = 0;
+    size_t most = 0;
+    for (int i = 0; i <= n; ++i) {
+        if (i < n && !is_short(matrices[i])) which[count++] = i;
+        if (count == kMaxMatrices || (i == n && count > 0)) {
+            Batch b;
+            size_t bytes = 0;
+            fill(matrices, which, count, &b, &bytes, nullptr);
+            most = bytes > most ? bytes : most;
+            count = 0;
+        }
+    }
+    return most;
+}
+
 template <bool MUON>
 int run(const gmc_matrix* matrices, int n, int dtype, int steps, float ca, float cb, float cc, float epsilon, const Momentum& mo,
         void* workspace, size_t workspace_bytes, void* stream) {
@@ -499,23 +791,14 @@ int run(const gmc_matrix* matrices, int n, int dtype, int steps, float ca, float
     if (int s = check_polynomial(steps, ca, cb, cc)) return s;
     for (int i = 0; i < n; ++i)
         if (!matrices[i].update || !matrices[i].out || (MUON && !matrices[i].momentum)) return GMC_ERR_NULL_POINTER;
-    if (n == 0) return GMC_OK;
-    if (!workspace) return GMC_ERR_NULL_POINTER;
     if (reinterpret_cast<uintptr_t>(workspace) & 1023u) return GMC_ERR_UNSUPPORTED;
-    for (int first = 0; first < n; first += kMaxMatrices) {
-        const int here = n - first < kMaxMatrices ? n - first : kMaxMatrices;
-        Batch b;
-        size_t bytes = 0;
-        if (int s = fill(matrices + first, here, &b, &bytes, static_cast<uint8_t*>(workspace))) return s;
-        if (bytes > workspace_bytes) return GMC_ERR_WORKSPACE;
-        cudaStream_t cs = as_stream(stream);
-        int s;
-        if (dtype == GMC_FLOAT32) s = run_batch<float, MUON>(b, steps, ca, cb, cc, epsilon, mo, cs);
-        else if (dtype == GMC_BFLOAT16) s = run_batch<__nv_bfloat16, MUON>(b, steps, ca, cb, cc, epsilon, mo, cs);
-        else s = run_batch<__half, MUON>(b, steps, ca, cb, cc, epsilon, mo, cs);
-        if (s) return s;
-    }
-    return GMC_OK;
+    const size_t need = workspace_bytes_of(matrices, n);
+    if (need > 0 && !workspace) return GMC_ERR_NULL_POINTER;
+    if (need > workspace_bytes) return GMC_ERR_WORKSPACE;
+    cudaStream_t cs = as_stream(stream);
+    if (dtype == GMC_FLOAT32) return run_typed<float, MUON>(matrices, n, steps, ca, cb, cc, epsilon, mo, workspace, workspace_bytes, cs);
+    if (dtype == GMC_BFLOAT16) return run_typed<__nv_bfloat16, MUON>(matrices, n, steps, ca, cb, cc, epsilon, mo, workspace, workspace_bytes, cs);
+    return run_typed<__half, MUON>(matrices, n, steps, ca, cb, cc, epsilon, mo, workspace, workspace_bytes, cs);
 }
 
 }  // namespace
@@ -526,15 +809,7 @@ GMC_DEFINE_TU_CHECK_READER(newton_schulz)
 extern "C" size_t gmc_orthogonalise_workspace_bytes(const gmc_matrix* matrices, int n_matrices) {
     using namespace gmc;
     if (check_matrices(matrices, n_matrices)) return 0;
-    size_t most = 0;
-    for (int first = 0; first < n_matrices; first += kMaxMatrices) {
-        const int here = n_matrices - first < kMaxMatrices ? n_matrices - first : kMaxMatrices;
-        Batch b;
-        size_t bytes = 0;
-        if (fill(matrices + first, here, &b, &bytes, nullptr)) return 0;
-        most = bytes > most ? bytes : most;
-    }
-    return most;
+    return workspace_bytes_of(matrices, n_matrices);
 }
 
 extern "C" int gmc_orthogonalise(const gmc_matrix* matrices, int n_matrices, int dtype, int steps, float a, float b, float c,

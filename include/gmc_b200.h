@@ -373,8 +373,9 @@ int gmc_log_probabilities_backward(const void* logits, int dtype, const long lon
  * within a call, and no matrix may appear twice. Products are accurate to fp32 rounding whatever `dtype`.
  * 1 <= steps <= 32; coefficients whose iterates leave |X| < 1.4, |b A + c A A| < 3.9 for singular values in [0, 1] are
  * refused (GMC_ERR_UNSUPPORTED); 1e-30 <= epsilon <= 1e30; 0 <= momentum < 1.
- * workspace: gmc_orthogonalise_workspace_bytes (0 = sizes out of range; depends on the shapes only), aligned to 1024 bytes,
- * content undefined before and after; concurrent calls need one each. Nothing is allocated, kept or synchronised.
+ * workspace: gmc_orthogonalise_workspace_bytes (depends on the shapes only; 0 = none needed, or sizes out of range), aligned
+ * to 1024 bytes, content undefined before and after; concurrent calls need one each. Nothing is allocated, kept or
+ * synchronised.
  * ---------------------------------------------------------------------------------------------- */
 typedef struct gmc_matrix {
     const void* update;

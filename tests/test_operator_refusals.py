@@ -51,14 +51,14 @@ def test_orthogonalise_argument_checks():
     from gmc import _native
     address = 1024
 
-    def run(rows=4, cols=5, us=5, os_=5, update=16, out=16, momentum=16, dtype=0, steps=5, abc=(3.4445, -4.775, 2.0315), eps=1e-7,
+    def run(rows=130, cols=140, us=140, os_=140, update=16, out=16, momentum=16, dtype=0, steps=5, abc=(3.4445, -4.775, 2.0315), eps=1e-7,
             n=1, work=address, size=1 << 30, muon=False, beta=0.9):
         m = _native.matrix_struct.pack(update, momentum, out, rows, cols, us, os_, 0.1)
         if muon:
             return _native.lib.gmc_muon_update(m, n, dtype, steps, *abc, eps, beta, 1, 1.0, work, size, NULL)
         return _native.lib.gmc_orthogonalise(m, n, dtype, steps, *abc, eps, work, size, NULL)
 
-    assert run(rows=0) == 1 and run(cols=0) == 1 and run(rows=32769) == 1 and run(us=4) == 1 and run(os_=4) == 1 and run(n=-1) == 1
+    assert run(rows=0) == 1 and run(cols=0) == 1 and run(rows=32769) == 1 and run(us=139) == 1 and run(os_=139) == 1 and run(n=-1) == 1
     assert run(dtype=3) == 4 and run(steps=0) == 4 and run(steps=33) == 4 and run(eps=0.0) == 4 and run(eps=float("nan")) == 4
     assert run(abc=(10.0, 0.0, 0.0)) == 4 and run(abc=(float("nan"), 0.0, 0.0)) == 4 and run(abc=(1.0, -4.0, 0.0)) == 4
     assert run(update=0) == 3 and run(out=0) == 3 and run(work=0) == 3 and run(work=address + 16) == 4
@@ -66,6 +66,7 @@ def test_orthogonalise_argument_checks():
     assert run(muon=True, momentum=0) == 3 and run(muon=True, beta=1.0) == 4 and run(muon=True, beta=-0.1) == 4
     m = _native.matrix_struct.pack(16, 0, 16, 300, 500, 500, 500, 0.0)
     assert _native.lib.gmc_orthogonalise_workspace_bytes(m, 1) > 0
+    assert _native.lib.gmc_orthogonalise_workspace_bytes(_native.matrix_struct.pack(16, 0, 16, 30, 50, 50, 50, 0.0), 1) == 0
     assert _native.lib.gmc_orthogonalise_workspace_bytes(_native.matrix_struct.pack(16, 0, 16, 0, 5, 5, 5, 0.0), 1) == 0
 
 

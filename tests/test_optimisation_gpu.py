@@ -2,7 +2,9 @@
 
 Error bound. The operands carry 22 bits where a 32-bit evaluation carries 24, and the polynomial amplifies either by the same
 factors: the error (2-norm over the matrix) may be 2^2 times that of the plain 32-bit evaluation of the same formula on the
-same input, plus 2^-20 of the result's norm for inputs on which the plain one is exact by luck, plus half a step of the
+same input. The plain one can be exact by luck (equal elements round alike), so there is a floor, from the last step alone:
+its terms a s, b s^3, c s^5 of a singular value s <= 1.21 add up to 4.2 + 8.5 + 5.3 = 18 in absolute value, each passes through
+four roundings (norm of X, A, A A, B X), 72 x 2^-24, and the result is at least 0.68: 106 x 2^-24 of it, below 2^-17. Last, half a step of the
 output's type on every value."""
 import copy
 import math
@@ -33,7 +35,7 @@ def _check(got, u, steps=5, coefficients=COEFFICIENTS, epsilon=1e-7):
     assert got.shape == u.shape and got.dtype == u.dtype
     norm = lambda t: torch.linalg.matrix_norm(t)  # noqa: E731
     half = torch.finfo(u.dtype).eps / 2 if u.dtype != torch.float32 else 0.0
-    bound = 4 * norm(plain - ref) + (2.0 ** -20 + half) * norm(ref) + torch.finfo(u.dtype).tiny * math.sqrt(u.shape[-1] * u.shape[-2])
+    bound = 4 * norm(plain - ref) + (2.0 ** -17 + half) * norm(ref) + torch.finfo(u.dtype).tiny * math.sqrt(u.shape[-1] * u.shape[-2])
     off = norm(got.double() - ref)
     assert (off <= bound).all(), f"{(off / norm(ref)).max().item():.3e} against {(bound / norm(ref)).min().item():.3e}"
 
@@ -91,7 +93,7 @@ def test_inputs_at_the_edges(m, n):
 def test_nan_and_infinity_stay_in_their_matrix(m, n):
     from gmc.optimisation import orthogonalise
     u = _update(4, m, n)
-    clean = orthogonalise(u)
+    clean = orthogonalise(u)            # the same call but for the values
     u[1, m - 1, n - 1] = math.nan
     u[2, 0, 0] = math.inf
     got = orthogonalise(u)
@@ -118,21 +120,16 @@ def test_singular_values_end_near_one(m, n):
 
 def test_batches_lists_and_strides():
     from gmc.optimisation import orthogonalise
+    # how many CTAs share a matrix's sums depends on what else is in the call: every result is held to the bound by itself
     u = _update(3, 2, 70, 90)
-    got = orthogonalise(u)
-    _check(got, u)
-    for i in range(3):
-        for j in range(2):
-            assert torch.equal(got[i, j], orthogonalise(u[i, j]))
-    many = _update(101, 10, 12)
-    assert torch.equal(orthogonalise(many)[77], orthogonalise(many[77]))
-    many = _update(50, 130, 70)
-    got = orthogonalise(many)
-    assert torch.equal(got[49], orthogonalise(many[49])) and torch.equal(got[0], orthogonalise(many[0]))
-    shapes = [(30, 40), (300, 140), (1, 9), (130, 700), (64, 64)]
+    _check(orthogonalise(u), u)
+    for shape in ((101, 10, 12), (50, 130, 70), (2, 1, 300, 200)):
+        many = _update(*shape)
+        _check(orthogonalise(many), many)
+    shapes = [(30, 40), (300, 140), (1, 9), (130, 700), (64, 64), (64, 3000), (700, 90)]
     mixed = [_update(m, n, seed=i) for i, (m, n) in enumerate(shapes)]
     for o, t in zip(orthogonalise(mixed), mixed):
-        assert torch.equal(o, orthogonalise(t))
+        _check(o, t)
     for size in (40, 200):
         wide = _update(size, 3 * size + 5)
         for view in (wide[:, 3:3 + size], wide[::2, 1:size], wide[:, :size].t(), wide[:1].expand(size, -1)):
