@@ -389,199 +389,307 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
 }
 
 // ---- matrices with a short side: the whole chain in one launch, fp32 -------------------------------------------------
-// One cluster per matrix. Each CTA keeps X for its share of the columns in shared memory over all steps; per step the CTAs
-// add up their shares of X X^T over distributed shared memory (CTA q sums rows q, q + ranks, .. and hands them to all), form
-// b A + c A A (each for itself) and multiply their own columns with it in place. Nothing goes through global memory between
+// One cluster per matrix. Each CTA keeps X for its share of the columns in shared memory over all steps; per step every CTA
+// adds up all shares of X X^T over distributed shared memory, forms P = a I + b A + c A A for itself and multiplies its own
+// columns with it in place. Nothing goes through global memory between
 // the update's elements and the result, there is one launch instead of three per step, and the products are fp32.
 constexpr int kShortThreads = 512;
+constexpr int kShortWarps = kShortThreads / 32;
 constexpr int kShortRows = 64;
-constexpr int kShortPartials = 8448;             // floats: groups x tiles x 16 partial sums of X X^T
 struct ShortBatch {
     Matrix m[kMaxMatrices];
 };
-__host__ __device__ inline int short_padded_rows(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
-__host__ __device__ inline int short_columns(int cols, int ranks) { return ((cols + ranks - 1) / ranks + 3) & ~3; }
-__host__ __device__ inline int short_pitch(int columns) { return ((columns + 27) / 32) * 32 + 4; }       // = 4 mod 32 banks, >= columns
-__host__ __device__ inline size_t short_smem(int rows, int cols, int ranks) {
-    const size_t mp = short_padded_rows(rows);
-    return (mp * short_pitch(short_columns(cols, ranks)) + 2 * mp * (mp + 4) + kShortPartials) * sizeof(float);
+// Sizes for X padded to MP rows: 4 x 4 tiles on and below the diagonal of X X^T, and groups of threads that share its sums.
+__host__ __device__ constexpr int short_padded_rows(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+__host__ __device__ constexpr int short_tiles(int mp) { return (mp / 4) * (mp / 4 + 1) / 2; }
+__host__ __device__ constexpr int short_packed(int mp) { return short_tiles(mp) * 16; }
+__host__ __device__ constexpr int short_groups(int mp) { return mp == 64 ? kShortThreads / short_tiles(64) : 1; }
+__host__ __device__ constexpr int short_columns(int cols, int ranks) { return ((cols + ranks - 1) / ranks + 3) & ~3; }
+__host__ __device__ constexpr int short_pitch(int columns) { return ((columns + 27) / 32) * 32 + 4; }    // = 4 mod 32 banks, >= columns
+__host__ __device__ constexpr size_t short_smem(int rows, int cols, int ranks) {
+    const int mp = short_padded_rows(rows);
+    return size_t(mp * short_pitch(short_columns(cols, ranks)) + 2 * mp * (mp + 4) + (2 + short_groups(mp)) * short_packed(mp)) * sizeof(float);
+}
+
+// Sums 16 values over the warp's lanes; returns the sum of value lane / 2 (both lanes of a pair hold it).
+__device__ __forceinline__ float warp_sum16(const float (&v)[16], int lane) {
+    float a[8], b[4], c[2];
+    const bool h16 = lane & 16, h8 = lane & 8, h4 = lane & 4, h2 = lane & 2;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = (h16 ? v[8 + i] : v[i]) + __shfl_xor_sync(0xffffffffu, h16 ? v[i] : v[8 + i], 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = (h8 ? a[4 + i] : a[i]) + __shfl_xor_sync(0xffffffffu, h8 ? a[i] : a[4 + i], 8);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) c[i] = (h4 ? b[2 + i] : b[i]) + __shfl_xor_sync(0xffffffffu, h4 ? b[i] : b[2 + i], 4);
+    const float d = (h2 ? c[1] : c[0]) + __shfl_xor_sync(0xffffffffu, h2 ? c[0] : c[1], 2);
+    return d + __shfl_xor_sync(0xffffffffu, d, 1);
+}
+
+// acc[4 i + j] += row (pi + i down) . row (pj + j down) over c = first, first + step, .. < length, four columns at a time
+__device__ __forceinline__ void tile_product(float (&acc)[16], const float* pi, const float* pj, int down, int first, int step, int length) {
+    for (int c = first; c < length; c += step) {
+        float4 p[4], q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            p[i] = *reinterpret_cast<const float4*>(pi + i * down + c);
+            q[i] = *reinterpret_cast<const float4*>(pj + i * down + c);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                acc[4 * i + j] += p[i].x * q[j].x;
+                acc[4 * i + j] += p[i].y * q[j].y;
+                acc[4 * i + j] += p[i].z * q[j].z;
+                acc[4 * i + j] += p[i].w * q[j].w;
+            }
+    }
+}
+
+// Tile number -> (row, column) of the tile on or below the diagonal.
+__device__ __forceinline__ void tile_place(int tile, int& ti, int& tj) {
+    ti = 0;
+    while ((ti + 1) * (ti + 2) / 2 <= tile) ++ti;
+    tj = tile - ti * (ti + 1) / 2;
+}
+
+// X X^T packed: element (4 i + j) of tile t at (4 i + j) * tiles + t. Tile (ti, tj) holds rows ti + side i and columns
+// tj + side j, so that neighbouring tiles read neighbouring rows, which the pitch puts into different banks.
+// MP = 64: a thread per tile and group of columns, the groups' sums added through shared memory; smaller: a warp per tile,
+// its lanes share the columns. done(e, value) is called once for every packed element.
+template <int MP, typename Done>
+__device__ __forceinline__ void symmetric_product(const float* from, int pitch, int length, float* partial, Done&& done) {
+    constexpr int side = MP / 4, tiles = short_tiles(MP), packed = short_packed(MP), groups = short_groups(MP);
+    const int tid = threadIdx.x;
+    if constexpr (groups > 1) {
+        const int tile = tid % tiles, group = tid / tiles;
+        if (group < groups) {
+            int ti, tj;
+            tile_place(tile, ti, tj);
+            float acc[16] = {};
+            tile_product(acc, from + ti * pitch, from + tj * pitch, side * pitch, group * 4, groups * 4, length);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) partial[group * packed + i * tiles + tile] = acc[i];
+        }
+        __syncthreads();
+        constexpr int each = (packed + kShortThreads - 1) / kShortThreads;
+        float v[each];
+#pragma unroll
+        for (int i = 0; i < each; ++i) {
+            const int e = tid + i * kShortThreads;
+            v[i] = 0.f;
+#pragma unroll
+            for (int g = 0; g < groups; ++g) v[i] += e < packed ? partial[g * packed + e] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < each; ++i)
+            if (tid + i * kShortThreads < packed) done(tid + i * kShortThreads, v[i]);
+    } else {
+        const int lane = tid & 31;
+        for (int tile = tid >> 5; tile < tiles; tile += kShortWarps) {
+            int ti, tj;
+            tile_place(tile, ti, tj);
+            float acc[16] = {};
+            tile_product(acc, from + ti * pitch, from + tj * pitch, side * pitch, lane * 4, 128, length);
+            const float v = warp_sum16(acc, lane);
+            if ((lane & 1) == 0) done((lane >> 1) * tiles + tile, v);
+        }
+    }
+}
+// Packed element -> its places (row, column) and (column, row) in a matrix of the given pitch.
+template <int MP>
+__device__ __forceinline__ void packed_places(int e, int pitch, int& at, int& mirror) {
+    constexpr int side = MP / 4, tiles = short_tiles(MP);
+    int ti, tj;
+    tile_place(e % tiles, ti, tj);
+    const int i = e / tiles, r = ti + side * (i >> 2), c = tj + side * (i & 3);
+    at = r * pitch + c;
+    mirror = c * pitch + r;
+}
+
+// X <- P X in place, RT x 4 elements per thread: a warp holds all rows of its columns, so what it overwrites it alone reads.
+template <int MP, int RT>
+__device__ __forceinline__ void multiply_in_place(float* x, int pitch, int columns, const float* p) {
+    constexpr int gp = MP + 4, row_tiles = MP / RT, col_tiles = 32 / row_tiles;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int row = (lane % row_tiles) * 4, my_col = (lane / row_tiles) * 4;
+    for (int c0 = warp * col_tiles * 4; c0 < columns; c0 += kShortWarps * col_tiles * 4) {
+        const int c = c0 + my_col;
+        const bool in = c < columns;
+        float acc[RT][4] = {};
+        if (in) {
+            const float* xc = x + c;
+            const float* pr = p + row;
+#pragma unroll 8
+            for (int k = 0; k < MP; ++k) {
+                const float4 v = *reinterpret_cast<const float4*>(xc + k * pitch);
+#pragma unroll
+                for (int h = 0; h < RT / 4; ++h) {
+                    const float4 q4 = *reinterpret_cast<const float4*>(pr + k * gp + h * row_tiles * 4);
+                    const float q[4] = {q4.x, q4.y, q4.z, q4.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        acc[h * 4 + i][0] += q[i] * v.x, acc[h * 4 + i][1] += q[i] * v.y;
+                        acc[h * 4 + i][2] += q[i] * v.z, acc[h * 4 + i][3] += q[i] * v.w;
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        if (in)
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+                *reinterpret_cast<float4*>(x + (row + (i / 4) * row_tiles * 4 + (i & 3)) * pitch + c) =
+                    make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+    }
+}
+
+template <typename T, bool MUON, int MP>
+__device__ __forceinline__ void short_matrix(const Matrix& m, int ranks, int rank, const Momentum& mo, int steps, float ca, float cb, float cc,
+                                             float epsilon, float* smem, double* warp_sum, double* cta_sum) {
+    constexpr int gp = MP + 4, packed = short_packed(MP);
+    cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const bool tall = m.rows > m.cols;
+    const int wide_rows = tall ? m.cols : m.rows, wide_cols = tall ? m.rows : m.cols;
+    const int columns = short_columns(wide_cols, ranks), pitch = short_pitch(columns);
+    const int col0 = rank * columns, here = max(0, min(columns, wide_cols - col0));
+    float* x = smem;
+    float* gram = x + MP * pitch;                // A
+    float* poly = gram + MP * gp;                // P = a I + b A + c A A
+    float* share = poly + MP * gp;               // the CTA's share of A, packed; two buffers in turn
+    float* partial = share + 2 * packed;
+
+    for (int i = tid * 4; i < MP * pitch; i += kShortThreads * 4) *reinterpret_cast<float4*>(x + i) = make_float4(0.f, 0.f, 0.f, 0.f);
+    __syncthreads();
+    // neighbouring threads along the rows of the update: `inner` elements of `outer` rows
+    const int inner = tall ? wide_rows : here, outer = inner > 0 ? (tall ? here : wide_rows) : 0;
+    const int step_outer = inner > 0 ? kShortThreads / inner : 0, step_inner = inner > 0 ? kShortThreads % inner : 0;
+    const long long first = tall ? 0 : col0, first_row = tall ? col0 : 0;
+    const int start_outer = inner > 0 ? tid / inner : 0, start_inner = inner > 0 ? tid % inner : 0;
+    auto next = [&](int& o, int& i) {
+        o += step_outer;
+        i += step_inner;
+        if (i >= inner) i -= inner, ++o;
+    };
+    constexpr int kBatch = 8;                                         // loads in flight per thread
+    double s = 0.;
+    for (int o0 = start_outer, i0 = start_inner; o0 < outer;) {
+        float u[kBatch], old[kBatch];
+        int o = o0, i = i0;
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const bool in = o < outer;
+            u[j] = in ? load_float<T>(m.update, (first_row + o) * m.update_stride + first + i) : 0.f;
+            if constexpr (MUON) old[j] = in ? m.momentum[(first_row + o) * m.cols + first + i] : 0.f;
+            next(o, i);
+        }
+        o = o0, i = i0;
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            if (o < outer) {
+                if constexpr (MUON) {
+                    const float now = mo.beta * old[j] + mo.one_minus_beta * u[j];
+                    m.momentum[(first_row + o) * m.cols + first + i] = now;
+                    u[j] = mo.nesterov ? mo.one_minus_beta * u[j] + mo.beta * now : now;
+                }
+                x[tall ? i * pitch + o : o * pitch + i] = u[j];
+                s += double(u[j]) * double(u[j]);
+            }
+            next(o, i);
+        }
+        o0 = o, i0 = i;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) warp_sum[warp] = s;
+    __syncthreads();
+    s = lane < kShortWarps ? warp_sum[lane] : 0.;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    s = __shfl_sync(0xffffffffu, s, 0);
+    if (ranks > 1) {
+        if (tid == 0) *cta_sum = s;
+        cluster.sync();
+        s = lane < ranks ? *cluster.map_shared_rank(cta_sum, lane) : 0.;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        s = __shfl_sync(0xffffffffu, s, 0);
+    }
+    const float factor = float(1. / (sqrt(s) + double(epsilon)));
+    for (int i = tid * 4; i < MP * pitch; i += kShortThreads * 4) {
+        float4 v = *reinterpret_cast<float4*>(x + i);
+        v.x *= factor, v.y *= factor, v.z *= factor, v.w *= factor;
+        *reinterpret_cast<float4*>(x + i) = v;
+    }
+    // where this thread's elements of the packed sums go (the same in every step)
+    constexpr int each = (packed + kShortThreads - 1) / kShortThreads;
+    int at[each], mirror[each];
+#pragma unroll
+    for (int i = 0; i < each; ++i) packed_places<MP>(min(tid + i * kShortThreads, packed - 1), gp, at[i], mirror[i]);
+    __syncthreads();
+
+    for (int step = 0; step < steps; ++step) {
+        // A: every CTA adds up all shares in their order. A share's buffer is written again two steps, so one barrier, later.
+        float* mine = share + (step & 1) * packed;
+        symmetric_product<MP>(x, pitch, columns, partial, [&](int e, float v) { mine[e] = v; });
+        if (ranks > 1) cluster.sync();
+        else __syncthreads();
+        float v[each];
+#pragma unroll
+        for (int i = 0; i < each; ++i) v[i] = 0.f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            if (q < ranks) {
+                const float* theirs = ranks > 1 ? cluster.map_shared_rank(mine, q) : mine;
+#pragma unroll
+                for (int i = 0; i < each; ++i) v[i] += theirs[min(tid + i * kShortThreads, packed - 1)];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < each; ++i)
+            if (tid + i * kShortThreads < packed) gram[at[i]] = gram[mirror[i]] = v[i];
+        __syncthreads();
+        symmetric_product<MP>(gram, gp, MP, partial, [&](int e, float v) {
+            int a, b;
+            if constexpr (short_groups(MP) > 1) {
+                const int i = (e - tid) / kShortThreads;
+                a = b = 0;
+#pragma unroll
+                for (int j = 0; j < each; ++j)
+                    if (i == j) a = at[j], b = mirror[j];
+            } else {
+                packed_places<MP>(e, gp, a, b);
+            }
+            poly[a] = poly[b] = cb * gram[a] + cc * v + (a == b ? ca : 0.f);
+        });
+        __syncthreads();
+        // the taller tile reads less per product, the lower one has more warps at work while there are few columns
+        if (columns * MP >= 4 * 4 * kShortThreads) multiply_in_place<MP, 8>(x, pitch, columns, poly);
+        else multiply_in_place<MP, 4>(x, pitch, columns, poly);
+        __syncthreads();
+    }
+    T* out = static_cast<T*>(m.out);
+#pragma unroll 4
+    for (int o = start_outer, i = start_inner; o < outer; next(o, i)) {
+        T* to = out + (first_row + o) * m.out_stride + first + i;
+        const float v = x[tall ? i * pitch + o : o * pitch + i];
+        *to = T(MUON ? float(*to) * mo.decay - m.rate * v : v);
+    }
+    if (ranks > 1) cluster.sync();                                    // no CTA leaves while its shared memory is read
 }
 
 template <typename T, bool MUON>
 __global__ void __launch_bounds__(kShortThreads, 1) short_kernel(const __grid_constant__ ShortBatch b, int ranks, Momentum mo, int steps, float ca,
                                                                  float cb, float cc, float epsilon) {
     extern __shared__ __align__(16) float smem[];
-    __shared__ double warp_sum[kShortThreads / 32], cta_sum;
-    cg::cluster_group cluster = cg::this_cluster();
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    __shared__ double warp_sum[kShortWarps], cta_sum;
     const Matrix& m = b.m[blockIdx.x / unsigned(ranks)];
-    const int rank = int(blockIdx.x % unsigned(ranks));
-    const bool tall = m.rows > m.cols;
-    const int wide_rows = tall ? m.cols : m.rows, wide_cols = tall ? m.rows : m.cols;
-    const int mp = short_padded_rows(wide_rows), columns = short_columns(wide_cols, ranks), pitch = short_pitch(columns), gp = mp + 4;
-    const int col0 = rank * columns, here = max(0, min(columns, wide_cols - col0));
-    float* x = smem;
-    float* gram = x + mp * pitch;                // A, complete
-    float* poly = gram + mp * gp;                // the CTA's share of A, then b A + c A A
-    float* partial = poly + mp * gp;
-
-    for (int i = tid; i < mp * pitch; i += kShortThreads) x[i] = 0.f;
-    __syncthreads();
-    double s = 0.;
-    for (int i = tid; i < wide_rows * here; i += kShortThreads) {
-        // neighbouring threads read along a row of the update
-        const int r = tall ? i % wide_rows : i / here, c = tall ? i / wide_rows : i % here;
-        const long long rr = tall ? col0 + c : r, cc_ = tall ? r : col0 + c;
-        float u = load_float<T>(m.update, rr * m.update_stride + cc_);
-        if constexpr (MUON) {
-            float* at = m.momentum + rr * m.cols + cc_;
-            const float now = mo.beta * *at + mo.one_minus_beta * u;
-            *at = now;
-            u = mo.nesterov ? mo.one_minus_beta * u + mo.beta * now : now;
-        }
-        x[r * pitch + c] = u;
-        s += double(u) * double(u);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) warp_sum[warp] = s;
-    __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < kShortThreads / 32; ++w) s += warp_sum[w];
-        cta_sum = s;
-    }
-    cluster.sync();
-    s = 0.;
-    for (int q = 0; q < ranks; ++q) s += *cluster.map_shared_rank(&cta_sum, q);
-    const float norm = float(sqrt(s) + double(epsilon));
-    for (int i = tid; i < wide_rows * here; i += kShortThreads) {
-        const int r = i / here, c = i - r * here;
-        x[r * pitch + c] /= norm;
-    }
-    __syncthreads();
-
-    const int tiles_side = mp / 4, tiles = tiles_side * (tiles_side + 1) / 2;
-    // this thread's 4 x 4 tile on or below the diagonal, and its share of a long axis
-    const int groups = min(kShortThreads / tiles, kShortPartials / (tiles * 16));
-    const int tile = tid % tiles, group = tid / tiles;
-    int ti = 0;
-    while ((ti + 1) * (ti + 2) / 2 <= tile) ++ti;
-    const int tj = tile - ti * (ti + 1) / 2;
-
-    // symmetric product rows x rows^T of `length` columns (a multiple of 4) of `from`; sum over the CTA's groups handed to
-    // store(row, column, value) for each element on or below the diagonal tiles
-    auto symmetric = [&](const float* from, int from_pitch, int length, auto&& store) {
-        if (group < groups) {
-            float acc[4][4] = {};
-            for (int c = group * 4; c < length; c += groups * 4) {
-                float4 p[4], q[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    p[i] = *reinterpret_cast<const float4*>(from + (ti * 4 + i) * from_pitch + c);
-                    q[i] = *reinterpret_cast<const float4*>(from + (tj * 4 + i) * from_pitch + c);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] += p[i].x * q[j].x + p[i].y * q[j].y + p[i].z * q[j].z + p[i].w * q[j].w;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<float4*>(partial + ((group * tiles + tile) * 4 + i) * 4) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
-        }
-        __syncthreads();
-        auto element = [&](int e, float v) {
-            int i = 0;
-            const int t = e >> 4;
-            while ((i + 1) * (i + 2) / 2 <= t) ++i;
-            store(i * 4 + ((e >> 2) & 3), (t - i * (i + 1) / 2) * 4 + (e & 3), v);
-        };
-        if (groups <= 16) {
-            for (int e = tid; e < tiles * 16; e += kShortThreads) {
-                float v = 0.f;
-                for (int g = 0; g < groups; ++g) v += partial[g * tiles * 16 + e];
-                element(e, v);
-            }
-        } else {
-            for (int e = warp; e < tiles * 16; e += kShortThreads / 32) {
-                float v = 0.f;
-                for (int g = lane; g < groups; g += 32) v += partial[g * tiles * 16 + e];
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-                if (lane == 0) element(e, v);
-            }
-        }
-    };
-
-    for (int step = 0; step < steps; ++step) {
-        symmetric(x, pitch, columns, [&](int i, int j, float v) {
-            poly[i * gp + j] = v;
-            poly[j * gp + i] = v;
-        });
-        if (ranks > 1) {
-            cluster.sync();
-            // rows rank, rank + ranks, .. : sum over the CTAs in their order, to all of them
-            const int quads = mp / 4;
-            for (int i = tid; i < ((mp - rank + ranks - 1) / ranks) * quads; i += kShortThreads) {
-                const int r = rank + (i / quads) * ranks, c = (i % quads) * 4;
-                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (int q = 0; q < ranks; ++q) {
-                    const float4 w = *reinterpret_cast<const float4*>(cluster.map_shared_rank(poly, q) + r * gp + c);
-                    v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
-                }
-                for (int q = 0; q < ranks; ++q) *reinterpret_cast<float4*>(cluster.map_shared_rank(gram, q) + r * gp + c) = v;
-            }
-            cluster.sync();
-        } else {
-            __syncthreads();
-        }
-        const float* full = ranks > 1 ? gram : poly;
-        float* to = ranks > 1 ? poly : gram;
-        symmetric(full, gp, mp, [&](int i, int j, float v) {
-            v = cb * full[i * gp + j] + cc * v;
-            to[i * gp + j] = v;
-            to[j * gp + i] = v;
-        });
-        __syncthreads();
-        // X <- a X + P X in place: a warp holds all rows of 4 * 32 / tiles_side columns, so what it overwrites it alone reads
-        const int col_tiles = 32 / tiles_side, row = (lane % tiles_side) * 4, my_col = (lane / tiles_side) * 4;
-        for (int c0 = warp * col_tiles * 4; c0 < columns; c0 += (kShortThreads / 32) * col_tiles * 4) {
-            const int c = c0 + my_col;
-            const bool in = c < columns;
-            float acc[4][4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float4 v = in ? *reinterpret_cast<const float4*>(x + (row + i) * pitch + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-                acc[i][0] = ca * v.x, acc[i][1] = ca * v.y, acc[i][2] = ca * v.z, acc[i][3] = ca * v.w;
-            }
-            if (in) {
-#pragma unroll 4
-                for (int k = 0; k < mp; ++k) {
-                    const float4 p = *reinterpret_cast<const float4*>(to + k * gp + row);
-                    const float4 v = *reinterpret_cast<const float4*>(x + k * pitch + c);
-                    const float pr[4] = {p.x, p.y, p.z, p.w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        acc[i][0] += pr[i] * v.x, acc[i][1] += pr[i] * v.y, acc[i][2] += pr[i] * v.z, acc[i][3] += pr[i] * v.w;
-                    }
-                }
-            }
-            __syncwarp();
-            if (in)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<float4*>(x + (row + i) * pitch + c) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
-        }
-        __syncthreads();
-    }
-    T* out = static_cast<T*>(m.out);
-    for (int i = tid; i < wide_rows * here; i += kShortThreads) {
-        const int r = tall ? i % wide_rows : i / here, c = tall ? i / wide_rows : i % here;
-        const long long o = tall ? (col0 + c) * m.out_stride + r : r * m.out_stride + col0 + c;
-        const float v = x[r * pitch + c];
-        out[o] = T(MUON ? float(out[o]) * mo.decay - m.rate * v : v);
-    }
-    cluster.sync();                                                   // no CTA leaves while its shared memory is read or written
+    const int rank = int(blockIdx.x % unsigned(ranks)), rows = min(m.rows, m.cols);
+    if (rows <= 8) short_matrix<T, MUON, 8>(m, ranks, rank, mo, steps, ca, cb, cc, epsilon, smem, warp_sum, &cta_sum);
+    else if (rows <= 16) short_matrix<T, MUON, 16>(m, ranks, rank, mo, steps, ca, cb, cc, epsilon, smem, warp_sum, &cta_sum);
+    else if (rows <= 32) short_matrix<T, MUON, 32>(m, ranks, rank, mo, steps, ca, cb, cc, epsilon, smem, warp_sum, &cta_sum);
+    else short_matrix<T, MUON, 64>(m, ranks, rank, mo, steps, ca, cb, cc, epsilon, smem, warp_sum, &cta_sum);
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------
@@ -693,7 +801,7 @@ int run_batch(const Batch& b, int steps, float ca, float cb, float cc, float eps
 }
 
 // A matrix goes to the one-launch kernel if its short side fits the tile grid and X fits the shared memory of eight CTAs.
-constexpr size_t kShortSmemLimit = 200 * 1024;
+constexpr size_t kShortSmemLimit = 220 * 1024;
 bool is_short(const gmc_matrix& g) {
     const long long rows = g.rows < g.cols ? g.rows : g.cols, cols = g.rows < g.cols ? g.cols : g.rows;
     return rows <= kShortRows && short_smem(int(rows), int(cols), 8) <= kShortSmemLimit;
