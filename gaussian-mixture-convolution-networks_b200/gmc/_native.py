@@ -129,7 +129,8 @@ def ptr(t) -> ctypes.c_void_p:
 
 
 def stream_of(t: torch.Tensor) -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+    # the raw handle: torch.cuda.current_stream() builds a Stream object first, which takes as long as the launch
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(t.device.index))
 
 
 def require_cuda_f32(t: torch.Tensor, name: str) -> None:

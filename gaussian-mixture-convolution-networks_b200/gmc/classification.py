@@ -19,30 +19,34 @@ class LogProbabilities(typing.NamedTuple):
     top_indices: typing.Optional[Tensor]     # [..., n_top] these classes; equal logits by the lower class
 
 
-def _forward(logits: Tensor, targets: typing.Optional[Tensor], n_top: int, temperature: float, ignore_index: int,
+def _forward(logits: Tensor, code: int, targets: typing.Optional[Tensor], n_top: int, temperature: float, ignore_index: int,
              keep_stats: bool):
     n, c = logits.shape
-    floats = dict(dtype=torch.float32, device=logits.device)
-    target = torch.empty(n, **floats) if targets is not None else None
-    entropy = torch.empty(n, **floats)
-    stats = torch.empty((n, 2), **floats) if keep_stats else None
-    top = torch.empty((n, n_top), **floats) if n_top else None
-    top_indices = torch.empty((n, n_top), dtype=torch.int64, device=logits.device) if n_top else None
+    device, f32 = logits.device, torch.float32
+    target = torch.empty(n, dtype=f32, device=device) if targets is not None else None
+    entropy = torch.empty(n, dtype=f32, device=device)
+    stats = torch.empty((n, 2), dtype=f32, device=device) if keep_stats else None
+    top = torch.empty((n, n_top), dtype=f32, device=device) if n_top else None
+    top_indices = torch.empty((n, n_top), dtype=torch.int64, device=device) if n_top else None
     with torch.cuda.device_of(logits):
         _native.check(_native.lib.gmc_log_probabilities_forward(
-            _native.ptr(logits), _native.dtype_code(logits, "logits"), _native.ptr(targets), n, c, logits.stride(0),
-            temperature, ignore_index, n_top, _native.ptr(target), _native.ptr(entropy), _native.ptr(stats), _native.ptr(top),
-            _native.ptr(top_indices), _native.stream_of(logits)), "log-probabilities")
+            logits.data_ptr(), code, _address(targets), n, c, logits.stride(0), temperature, ignore_index, n_top,
+            _address(target), entropy.data_ptr(), _address(stats), _address(top), _address(top_indices),
+            _native.stream_of(logits)), "log-probabilities")
     return target, entropy, top, top_indices, stats
+
+
+def _address(t: typing.Optional[Tensor]) -> typing.Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 class _LogProbabilities(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, targets, n_top, temperature, ignore_index):
+    def forward(ctx, logits, code, targets, n_top, temperature, ignore_index):
         ctx.set_materialize_grads(False)
-        target, entropy, top, top_indices, stats = _forward(logits, targets, n_top, temperature, ignore_index, True)
+        target, entropy, top, top_indices, stats = _forward(logits, code, targets, n_top, temperature, ignore_index, True)
         ctx.save_for_backward(logits, targets, entropy, top_indices, stats)
-        ctx.config = (n_top, temperature, ignore_index)
+        ctx.config = (code, n_top, temperature, ignore_index)
         if top_indices is not None:
             ctx.mark_non_differentiable(top_indices)
         return target, entropy, top, top_indices
@@ -50,20 +54,19 @@ class _LogProbabilities(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_target, grad_entropy, grad_top, _):
-        logits, targets, entropy, top_indices, stats = ctx.saved_tensors
-        n_top, temperature, ignore_index = ctx.config
         if grad_target is None and grad_entropy is None and grad_top is None:
-            return (None,) * 5
+            return None, None, None, None, None, None
+        logits, targets, entropy, top_indices, stats = ctx.saved_tensors
+        code, n_top, temperature, ignore_index = ctx.config
         grads = [None if g is None else g.contiguous() for g in (grad_target, grad_entropy, grad_top)]
         n, c = logits.shape
         grad_logits = torch.empty((n, c), dtype=logits.dtype, device=logits.device)
         with torch.cuda.device_of(logits):
             _native.check(_native.lib.gmc_log_probabilities_backward(
-                _native.ptr(logits), _native.dtype_code(logits, "logits"), _native.ptr(targets), _native.ptr(top_indices),
-                _native.ptr(stats), _native.ptr(entropy), _native.ptr(grads[0]), _native.ptr(grads[1]), _native.ptr(grads[2]),
-                _native.ptr(grad_logits), n, c, logits.stride(0), temperature, ignore_index, n_top,
-                _native.stream_of(logits)), "gradient of log-probabilities")
-        return grad_logits, None, None, None, None
+                logits.data_ptr(), code, _address(targets), _address(top_indices), stats.data_ptr(), entropy.data_ptr(),
+                _address(grads[0]), _address(grads[1]), _address(grads[2]), grad_logits.data_ptr(), n, c, logits.stride(0),
+                temperature, ignore_index, n_top, _native.stream_of(logits)), "gradient of log-probabilities")
+        return grad_logits, None, None, None, None, None
 
 
 def log_probabilities(logits: Tensor, targets: typing.Optional[Tensor] = None, n_top: int = 0, temperature: float = 1.0,
@@ -79,7 +82,7 @@ def log_probabilities(logits: Tensor, targets: typing.Optional[Tensor] = None, n
     memory are copied; rows may be any distance apart."""
     if not isinstance(logits, Tensor) or logits.dim() < 1 or logits.shape[-1] < 1:
         raise _native.GmcError("logits must be a tensor [..., n_classes] with at least one class")
-    _native.dtype_code(logits, "logits")
+    code = _native.dtype_code(logits, "logits")
     c = logits.shape[-1]
     if not 0 <= n_top <= min(MAX_TOP, c):
         raise _native.GmcError(f"n_top must be between 0 and min({MAX_TOP}, n_classes = {c}), got {n_top}")
@@ -90,14 +93,15 @@ def log_probabilities(logits: Tensor, targets: typing.Optional[Tensor] = None, n
         if targets.device != logits.device or targets.dtype != torch.int64 or targets.shape != lead:
             raise _native.GmcError(f"targets must be int64 {tuple(lead)} on {logits.device}, "
                                    f"got {targets.dtype} {tuple(targets.shape)} on {targets.device}")
-        targets = targets.reshape(-1).contiguous()
+        targets = targets.contiguous() if targets.dim() == 1 else targets.reshape(-1).contiguous()
     rows = logits if logits.dim() == 2 else logits.reshape(-1, c)
     if rows.stride(1) != 1 and c > 1:
         rows = rows.contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
-        target, entropy, top, top_indices = _LogProbabilities.apply(rows, targets, int(n_top), float(temperature), int(ignore_index))
+    n_top, temperature, ignore_index = int(n_top), float(temperature), int(ignore_index)
+    if logits.requires_grad and torch.is_grad_enabled():
+        target, entropy, top, top_indices = _LogProbabilities.apply(rows, code, targets, n_top, temperature, ignore_index)
     else:
-        target, entropy, top, top_indices, _ = _forward(rows, targets, int(n_top), float(temperature), int(ignore_index), False)
+        target, entropy, top, top_indices, _ = _forward(rows, code, targets, n_top, temperature, ignore_index, False)
     if logits.dim() != 2:
         target = None if target is None else target.view(lead)
         entropy = entropy.view(lead)
