@@ -1,6 +1,9 @@
 // Orthogonalisation of updates by Newton-Schulz products, and the Muon update around it.
 //
-//   X = U / (|U| + eps) (transposed if it is taller than wide);  steps times: A = X X^T, B = b A + c A A, X <- a X + B X
+//   X = U / (|U| + eps) (transposed if it is taller than wide);  steps times: A = X X^T, X <- (a I + b A + c A A) X
+//
+// The square is completed: a I + b A + c A A = c S S + d I with S = A + b / (2 c) I, d = a - b^2 / (4 c), so that a product's
+// tile needs nothing but its own sums and a number on the diagonal.
 //
 // Precision. The polynomial multiplies what is small by up to a^steps (485 for the usual coefficients), and rounding errors
 // with it, so operands of 11 or 8 bits would leave errors of 1e-1 where U is close to rank one. Every operand is therefore
@@ -8,13 +11,16 @@
 // [0, 1] keeps below the largest fp16 number), and a product takes three tensor-core products, hi hi + hi lo + lo hi, into
 // one fp32 accumulator; the left-out lo lo is 2^-22 of it. The cost is three times the operations of one product.
 //
-// Layout. Planes lie in global memory as blocks of 128 rows x 64 columns in the exact byte order the tensor core reads from
-// shared memory (128-byte swizzle), padded with zeros: loading an operand tile is one contiguous bulk copy, whatever the
-// matrix's shape, and X serves both as rows (X X^T, K = columns) and across (B X, K = rows) without a transposed copy.
-// A and A A are symmetric: only tiles on and below the diagonal are computed, their mirror images are stored with them.
+// Layout. Both planes lie in global memory as blocks of 128 rows x 64 columns in the exact byte order the tensor core reads
+// from shared memory (128-byte swizzle, eight rows of hi and of lo in turn), padded with zeros: loading an operand tile is
+// one or two contiguous bulk copies, whatever the matrix's shape (a copy costs its issuing thread 130 cycles or more, whatever
+// its size), and X serves both as rows (X X^T, K = columns) and across (P X, K = rows) without a transposed copy.
+// A and A A are symmetric: only tiles on and below the diagonal are computed and stored, what lies above is read across.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <atomic>
 
 #include "tcgen05.cuh"
 
@@ -23,12 +29,15 @@ namespace {
 
 namespace cg = cooperative_groups;
 
+constexpr int kPairs = 74;                       // CTA pairs of the GPU: 148 multiprocessors
 constexpr int kMaxMatrices = 48;                 // descriptors of one launch (kernel parameter)
-constexpr int kBlockBytes = 128 * 64 * 2;        // one block of one plane
-constexpr int kStageBytes = 4 * kBlockBytes;     // hi and lo of both operands, 64 wide in K
+constexpr int kBlockBytes = 2 * 128 * 64 * 2;    // one block, both planes
+constexpr int kHalfBlock = kBlockBytes / 2;      // 64 rows of it
+constexpr int kStageBytes = 2 * kBlockBytes;     // both operands, 64 wide in K
 constexpr int kStages = 3;
-constexpr int kProductSmem = kStages * kStageBytes + 1024;
-constexpr float kScaleX = 32768.f, kScaleA = 32768.f, kScaleB = 16384.f;
+constexpr int kStagingBytes = 2 * 16 * 128;      // 16 rows of a block, both planes, on their way out
+constexpr int kChainSmem = kStages * kStageBytes + 8 * kStagingBytes + 1024;
+constexpr float kScaleX = 32768.f;               // |X| stays below 1.8, the largest fp16 number is 65504
 constexpr int kNormElements = 4096;              // elements of a matrix per CTA of the norm
 
 // The matrices of a launch. Wide form: m <= n after the transposition.
@@ -40,15 +49,19 @@ struct Matrix {
     int rows, cols;
     int row_tiles, col_blocks;  // of the wide form: 128 rows, 64 columns (even number)
     float rate;                 // factor of the orthogonalised update that is subtracted from the parameters
-    int norm_first, gram_first, step_first, block_first;      // first CTA of the matrix in each launch
-    long long x_block, gram_block;                             // first block in the workspace's arrays
+    int norm_first, block_first;                       // first CTA of the matrix in the launches before and after the chain
+    int pair_first, pairs;                             // CTA pairs of the matrix in the chain
+    int gram_wide, poly_wide, step_wide, splits;       // tiles 256 instead of 128 columns wide; shares of the columns in X X^T
+    long long x_block, gram_block, partial_first;      // first block, first partial sum in the workspace's arrays
 };
 struct Batch {
     Matrix m[kMaxMatrices];
     int n;
     __half *x[2], *gram, *poly;
-    double* partial;            // one per CTA of the norm
-    int norm_ctas, gram_ctas, step_ctas, blocks;
+    double* squares;            // one per CTA of the norm
+    float* partial;             // tiles of X X^T over shares of the columns
+    unsigned* arrived;          // one counter per matrix, then the failure flag
+    int norm_ctas, pairs, blocks;
 };
 struct Momentum {
     float beta, one_minus_beta;
@@ -71,6 +84,7 @@ __device__ __forceinline__ int find_matrix(const Batch& b, int cta) {
 // momentum the running average is updated on the way.
 template <typename T, bool MUON>
 __global__ void __launch_bounds__(256) norm_kernel(const __grid_constant__ Batch b, Momentum mo) {
+    if (blockIdx.x == 0 && threadIdx.x <= unsigned(b.n)) b.arrived[threadIdx.x] = 0;        // for the chain
     const int which = find_matrix<&Matrix::norm_first>(b, blockIdx.x);
     const Matrix& m = b.m[which];
     const long long total = (long long)m.rows * m.cols;
@@ -98,7 +112,7 @@ __global__ void __launch_bounds__(256) norm_kernel(const __grid_constant__ Batch
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < 8; ++w) s += warp_sum[w];
-        b.partial[blockIdx.x] = s;
+        b.squares[blockIdx.x] = s;
     }
 }
 
@@ -120,7 +134,7 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ Batc
     const int norm_end = which + 1 < b.n ? b.m[which + 1].norm_first : b.norm_ctas;
     __shared__ double warp_sum[8];
     double s = 0.;
-    for (int i = m.norm_first + threadIdx.x; i < norm_end; i += 256) s += b.partial[i];
+    for (int i = m.norm_first + threadIdx.x; i < norm_end; i += 256) s += b.squares[i];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if ((threadIdx.x & 31) == 0) warp_sum[threadIdx.x >> 5] = s;
@@ -131,9 +145,8 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ Batc
     const bool tall = m.rows > m.cols;
     const int wide_rows = tall ? m.cols : m.rows, wide_cols = tall ? m.rows : m.cols;
     const int row_tile = block / m.col_blocks, col_block = block - row_tile * m.col_blocks;
-    const long long planes = (long long)m.row_tiles * m.col_blocks;
     uint8_t* hi_block = reinterpret_cast<uint8_t*>(b.x[0]) + (m.x_block + block) * kBlockBytes;
-    uint8_t* lo_block = hi_block + planes * kBlockBytes;
+    uint8_t* lo_block = hi_block + kPlaneOffset;
     for (int i = threadIdx.x; i < 128 * 8; i += 256) {
         const int row = tall ? i & 127 : i >> 3, chunk = tall ? i >> 7 : i & 7;      // neighbouring threads read along a row
         const int r = row_tile * 128 + row;
@@ -168,10 +181,10 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Bat
     const bool tall = m.rows > m.cols;
     const int wide_rows = tall ? m.cols : m.rows, wide_cols = tall ? m.rows : m.cols;
     const int row_tile = block / m.col_blocks, col_block = block - row_tile * m.col_blocks;
-    const long long planes = (long long)m.row_tiles * m.col_blocks;
     const uint8_t* hi_block = reinterpret_cast<const uint8_t*>(b.x[which_x]) + (m.x_block + block) * kBlockBytes;
-    const uint8_t* lo_block = hi_block + planes * kBlockBytes;
+    const uint8_t* lo_block = hi_block + kPlaneOffset;
     T* out = static_cast<T*>(m.out);
+    const bool failed = b.arrived[b.n] != 0;
     for (int i = threadIdx.x; i < 128 * 8; i += 256) {
         const int row = tall ? i & 127 : i >> 3, chunk = tall ? i >> 7 : i & 7;
         const int r = row_tile * 128 + row;
@@ -185,206 +198,423 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Bat
             const int c = col_block * 64 + chunk * 8 + e;
             if (c >= wide_cols) break;
             const long long o = tall ? c * m.out_stride + r : r * m.out_stride + c;
-            const float x = (__half2float(hi.h[e]) + __half2float(lo.h[e])) * (1.f / kScaleX);
+            float x = (__half2float(hi.h[e]) + __half2float(lo.h[e])) * (1.f / kScaleX);
+            if (failed) x = __int_as_float(0x7fffffff);
             out[o] = T(MUON ? float(out[o]) * mo.decay - m.rate * x : x);
         }
     }
 }
 
-enum Product { GRAM, POLY, STEP };
-
-// One 128 x kTileN tile of a product per CTA. Warps 0-7 write the tile (warp w: rows 32 (w % 4) .. + 31, half w / 4 of the
-// columns), warp 8 loads (bulk copies into a ring of stages), warp 9 issues the MMAs.
+// All products of a call in one persistent launch. A matrix has some pairs of CTAs; a pair computes tiles of 256 rows (128
+// per CTA) by 256 or 128 columns with two-CTA MMAs, which read half the operand bytes per CTA that one CTA alone would (with
+// one CTA and 128 x 128 tiles the shared memory's 128 bytes per cycle, filled and read at once, held the tensor core at 40 %).
+// Between the products of a step the matrix's CTAs wait for one another at a counter in global memory; the launch is
+// cooperative, so all of them are resident.
+//
+// Roles: warps 0-7 write tiles (warp w: rows 32 (w % 4) .. + 31 of the CTA's 128, half w / 4 of the columns), warps 8 and 9
+// load one operand each (bulk copies into a ring of stages), warp 10 of the pair's first CTA issues the MMAs, that of the
+// second one passes on that its operands have arrived.
 //
 // The tensor core adds into its fp32 accumulator without rounding to nearest, which over a long inner axis drifts (7e-6 of
 // the result at 2000 columns). hi hi is therefore accumulated over kChunk stages only and then added to registers, while
 // the MMAs of the next chunk's mixed products run; hi lo and lo hi, 2^-11 as large, have an accumulator of their own.
-constexpr int kTileN = 128;
+enum Product { GRAM, POLY, STEP };
 constexpr int kWriters = 256;
-constexpr int kProductThreads = kWriters + 64;
-constexpr int kChunk = 2;                         // stages, 64 wide in K each
-template <Product P>
-__global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __grid_constant__ Batch b, int from_x, float c0, float c1) {
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t full[kStages], empty[kStages], ready, drained, done;
-    __shared__ uint32_t tmem_address;
-    __shared__ int failed;
-    const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
-    uint8_t* stages = smem_raw + pad;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+constexpr int kChainThreads = kWriters + 96;
+constexpr int kChunk = 4;                         // stages, 64 wide in K each
+constexpr int kMixedColumns = 256;                // TMEM columns: 256 for hi hi, 256 for the mixed products
 
-    constexpr bool symmetric = P != STEP;
-    const int which = find_matrix<symmetric ? &Matrix::gram_first : &Matrix::step_first>(b, blockIdx.x);
-    const Matrix& m = b.m[which];
-    int tile = int(blockIdx.x) - (symmetric ? m.gram_first : m.step_first);
-    int ti, tj;                                                       // tile row, tile column
-    if (symmetric) {
+// A matrix in the workspace: blocks of 128 x 64, both planes.
+struct Planes {
+    uint8_t* base;
+    int row_blocks, col_blocks;
+    __device__ __forceinline__ uint8_t* block(int r, int c) const { return base + ((long long)r * col_blocks + c) * kBlockBytes; }
+};
+
+// One operand of a stage: `groups` x 64 rows from row group `row` on, 64 wide in K at `kb`. Along K the rows are those of the
+// matrix; across K they are its columns (K = its rows).
+__device__ __forceinline__ void load_operand(uint8_t* to, const Planes& p, int row, int groups, int kb, bool across, uint64_t* bar) {
+    if (!across) {
+        const int r = min(row >> 1, p.row_blocks - 1);                                  // rows behind the last tile are not stored
+        bulk_copy_g2s(to, p.block(r, kb) + (groups == 1 ? (row & 1) * kHalfBlock : 0), groups * kHalfBlock, bar);
+    } else {
+        for (int g = 0; g < groups; ++g)
+            bulk_copy_g2s(to + g * kHalfBlock, p.block(kb >> 1, min(row + g, p.col_blocks - 1)) + (kb & 1) * kHalfBlock, kHalfBlock, bar);
+    }
+}
+
+// Tiles of a symmetric product: rows of 256, columns of 256 or 128, the column's 256 not above the row's.
+__host__ __device__ __forceinline__ int symmetric_tiles(int row_tiles, int wide) {
+    const int rows = (row_tiles + 1) / 2;
+    return wide ? rows * (rows + 1) / 2 : rows * (rows + 1) - (row_tiles & 1);
+}
+__device__ __forceinline__ void symmetric_tile(int tile, int wide, int& ti, int& tj) {
+    ti = 0;
+    if (wide) {
         ti = int((sqrtf(8.f * float(tile) + 1.f) - 1.f) * 0.5f);
         while (ti * (ti + 1) / 2 > tile) --ti;
         while ((ti + 1) * (ti + 2) / 2 <= tile) ++ti;
         tj = tile - ti * (ti + 1) / 2;
     } else {
-        const int col_tiles = m.col_blocks >> 1;
-        ti = tile / col_tiles;
-        tj = tile - ti * col_tiles;
+        ti = int((sqrtf(4.f * float(tile) + 1.f) - 1.f) * 0.5f);
+        while (ti * (ti + 1) > tile) --ti;
+        while ((ti + 1) * (ti + 2) <= tile) ++ti;
+        tj = tile - ti * (ti + 1);
     }
-    const int gram_blocks = 2 * m.row_tiles;                          // column blocks of A and B
-    const long long x_plane = (long long)m.row_tiles * m.col_blocks * kBlockBytes;
-    const long long gram_plane = (long long)m.row_tiles * gram_blocks * kBlockBytes;
-    const uint8_t* x = reinterpret_cast<const uint8_t*>(b.x[from_x]) + m.x_block * kBlockBytes;
-    uint8_t* x_out = reinterpret_cast<uint8_t*>(b.x[from_x ^ 1]) + m.x_block * kBlockBytes;
-    uint8_t* gram = reinterpret_cast<uint8_t*>(b.gram) + m.gram_block * kBlockBytes;
-    uint8_t* poly = reinterpret_cast<uint8_t*>(b.poly) + m.gram_block * kBlockBytes;
-    const int k_blocks = P == GRAM ? m.col_blocks : gram_blocks;      // even
-    const int chunks = k_blocks / kChunk;
+}
 
-    if (tid == 0) {
-        for (int s = 0; s < kStages; ++s) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
-        }
-        mbar_init(&ready, 1);
-        mbar_init(&drained, kWriters / 32);
-        mbar_init(&done, 1);
-        failed = 0;
-        fence_mbar_init();
+// What a CTA needs to walk through the products of its matrix; the same in every role.
+struct Walk {
+    Planes x0, x1, gram, poly;
+    int pair, pairs, splits;
+    int gram_wide, poly_wide, step_wide;
+    __device__ __forceinline__ const Planes& x(int i) const { return i ? x1 : x0; }
+    __device__ __forceinline__ int wide(Product p) const { return p == GRAM ? gram_wide : p == POLY ? poly_wide : step_wide; }
+    __device__ __forceinline__ int tiles(Product p) const {
+        return p == STEP ? ((gram.row_blocks + 1) / 2) * ((x0.col_blocks + (step_wide ? 3 : 1)) / (step_wide ? 4 : 2))
+                         : symmetric_tiles(gram.row_blocks, wide(p));
     }
-    if (warp == kWriters / 32 + 1) tmem_alloc(&tmem_address, 2 * kTileN);
-    tmem_fence_before();
-    __syncthreads();
-    tmem_fence_after();
-    const uint32_t main_sum = tmem_address, mixed_sum = tmem_address + kTileN;
+    // unit -> tile row (256), tile column (256 or 128), first and last 64 in K
+    __device__ __forceinline__ void unit(Product p, int u, int& ti, int& tj, int& k0, int& k1) const {
+        const int n = tiles(p), share = u / n, tile = u - share * n, all = p == GRAM ? x0.col_blocks : gram.col_blocks;
+        if (p == STEP) {
+            const int columns = (x0.col_blocks + (step_wide ? 3 : 1)) / (step_wide ? 4 : 2);
+            ti = tile / columns;
+            tj = tile - ti * columns;
+        } else {
+            symmetric_tile(tile, wide(p), ti, tj);
+        }
+        const int parts = p == GRAM ? splits : 1;
+        k0 = int((long long)all * share / parts);
+        k1 = int((long long)all * (share + 1) / parts);
+    }
+    __device__ __forceinline__ int units(Product p) const { return tiles(p) * (p == GRAM ? splits : 1); }
+};
 
-    if (tid == kWriters) {
-        bool ok = true;
-        int issued = 0;
-        for (int kb = 0; kb < k_blocks; ++kb) {
-            const int s = kb % kStages;
-            if (kb >= kStages && !(ok = mbar_wait_bounded(&empty[s], ((kb / kStages) - 1) & 1))) break;
-            uint8_t* stage = stages + s * kStageBytes;
-            mbar_arrive_expect_tx(&full[s], kStageBytes);
-            const uint8_t* a;
-            long long plane;
-            if (P == GRAM) a = x + ((long long)ti * m.col_blocks + kb) * kBlockBytes, plane = x_plane;
-            else a = (P == POLY ? gram : poly) + ((long long)ti * gram_blocks + kb) * kBlockBytes, plane = gram_plane;
-            bulk_copy_g2s(stage, a, kBlockBytes, &full[s]);
-            bulk_copy_g2s(stage + kBlockBytes, a + plane, kBlockBytes, &full[s]);
-            if (P == STEP) {
-                // 64 rows of two neighbouring column blocks of X, each half a block
-                const uint8_t* xb = x + ((long long)(kb >> 1) * m.col_blocks + 2 * tj) * kBlockBytes + (kb & 1) * (kBlockBytes / 2);
-                for (int q = 0; q < 4; ++q)
-                    bulk_copy_g2s(stage + 2 * kBlockBytes + q * (kBlockBytes / 2), xb + (q >> 1) * x_plane + (long long)(q & 1) * kBlockBytes,
-                                  kBlockBytes / 2, &full[s]);
-            } else {
-                const uint8_t* r = P == GRAM ? x + ((long long)tj * m.col_blocks + kb) * kBlockBytes
-                                             : gram + ((long long)tj * gram_blocks + kb) * kBlockBytes;
-                bulk_copy_g2s(stage + 2 * kBlockBytes, r, kBlockBytes, &full[s]);
-                bulk_copy_g2s(stage + 3 * kBlockBytes, r + plane, kBlockBytes, &full[s]);
-            }
-            issued = kb + 1;
-        }
-        if (!ok) {
-            *(volatile int*)&failed = 1;
-            for (int kb = max(0, issued - kStages); kb < issued; ++kb) mbar_wait_bounded(&full[kb % kStages], (kb / kStages) & 1);
-        }
-    } else if (tid == kWriters + 32) {
-        constexpr uint32_t instruction = f16_instruction(128, kTileN, P == STEP);
-        bool ok = true;
-        for (int kb = 0; kb < k_blocks; ++kb) {
-            const int s = kb % kStages, chunk = kb / kChunk;
-            if (!(ok = mbar_wait_bounded(&full[s], (kb / kStages) & 1))) break;
-            tmem_fence_after();
-            const uint32_t stage = smem_u32(stages + s * kStageBytes);
-            auto a_of = [&](int plane, int k) { return k_major_descriptor(stage + plane * kBlockBytes + k * 32); };
-            auto b_of = [&](int plane, int k) {
-                return P == STEP ? mn_major_descriptor(stage + (2 + plane) * kBlockBytes + k * 2048, kBlockBytes / 2)
-                                 : k_major_descriptor(stage + (2 + plane) * kBlockBytes + k * 32);
-            };
+__device__ __forceinline__ bool wait_counter(const unsigned* counter, unsigned value) {
+    for (int i = 0; i < (1 << 22); ++i) {
+        unsigned now;
+        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(counter) : "memory");
+        if (now >= value) return true;
+    }
+    report_check(CHECK_MBARRIER_TIMEOUT);
+    return false;
+}
+__device__ __forceinline__ void fence_proxy_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
+__device__ __forceinline__ void writers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWriters) : "memory"); }
+
+// A warp's 32 rows of one block (rows 32 `quarter`, 64 columns): v c1, plus c0 on the matrix's diagonal, as planes. Sixteen
+// rows at a time are laid out in shared memory as the block has them and leave as one contiguous bulk copy.
+__device__ __forceinline__ void emit(const Planes& to, int row_block, int quarter, int col_block, const float* v, float c0, float c1,
+                                     uint8_t* staging, int lane) {
+    if (row_block >= to.row_blocks || col_block >= to.col_blocks) return;
+    const int diagonal = row_block * 128 + quarter * 32 + lane - col_block * 64;
+    uint8_t* out = to.block(row_block, col_block) + quarter * 2 * kStagingBytes;
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();
+        if ((lane >> 4) == half) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {                             // 16 of the 64 in K
-                mma_f16(mixed_sum, a_of(0, k), b_of(1, k), instruction, kb > 0 || k > 0);
-                mma_f16(mixed_sum, a_of(1, k), b_of(0, k), instruction, true);
-            }
-            if (kb % kChunk == 0 && chunk > 0) {
-                if (!(ok = mbar_wait_bounded(&drained, (chunk - 1) & 1))) break;
-                tmem_fence_after();
-            }
+            for (int g = 0; g < 8; ++g) {                             // 8 columns = one 16-byte chunk
+                Chunk hi, lo;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) mma_f16(main_sum, a_of(0, k), b_of(0, k), instruction, kb % kChunk > 0 || k > 0);
-            mma_commit(&empty[s]);
-            if (kb % kChunk == kChunk - 1) mma_commit(&ready);
+                for (int e = 0; e < 8; ++e) split(v[g * 8 + e] * c1 + (g * 8 + e == diagonal ? c0 : 0.f), hi.h[e], lo.h[e]);
+                uint8_t* at = staging + swizzled_offset(lane & 15, g);
+                *reinterpret_cast<uint4*>(at) = hi.raw;
+                *reinterpret_cast<uint4*>(at + kPlaneOffset) = lo.raw;
+            }
         }
-        if (!ok) *(volatile int*)&failed = 1;
-        mma_commit(&done);
-        mbar_wait_bounded(&done, 0);                                  // nothing of this CTA in flight when its TMEM is freed
-    } else if (warp < kWriters / 32) {
-        constexpr int C = kTileN / 2;                                 // columns of a warp
-        const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-        const int col0 = (warp >> 2) * C;
-        float sum[C];
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(out + half * kStagingBytes), "r"(smem_u32(staging)),
+                         "n"(kStagingBytes)
+                         : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+    }
+}
+
+struct ChainBarriers {
+    uint64_t full[kStages], peer_full[kStages], empty[kStages], ready, drained, done;
+};
+
+// Writers: the tiles of one product. `chunk` counts the chunks since the launch.
+template <Product P>
+__device__ __forceinline__ bool write_product(const Walk& w, ChainBarriers& bar, uint32_t tmem, int cta, unsigned& chunk, const Planes& to, float c0,
+                                              float c1, float* partial, uint8_t* staging) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+    const int wide = w.wide(P), half = wide ? 128 : 64, col0 = (warp >> 2) * half;
+    for (int u = w.pair; u < w.units(P); u += w.pairs) {
+        int ti, tj, k0, k1;
+        w.unit(P, u, ti, tj, k0, k1);
+        float sum[128];
 #pragma unroll
-        for (int i = 0; i < C; ++i) sum[i] = 0.f;
-        bool complete = true;
-        for (int chunk = 0; chunk < chunks && complete; ++chunk) {
-            complete = mbar_wait_bounded(&ready, chunk & 1);
+        for (int i = 0; i < 128; ++i) sum[i] = 0.f;
+        for (int kb = k0; kb < k1; kb += kChunk, ++chunk) {
+            if (!mbar_wait_bounded(&bar.ready, chunk & 1)) return false;
             tmem_fence_after();
 #pragma unroll
-            for (int q = 0; q < C; q += 32) {
-                float v[32];
-                tmem_load32(main_sum + lanes + col0 + q, v);
+            for (int q = 0; q < 4; ++q) {
+                if (q < 2 || wide) {
+                    float v[32];
+                    tmem_load32(tmem + lanes + col0 + q * 32, v);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) sum[q + i] += v[i];
+                    for (int i = 0; i < 32; ++i) sum[q * 32 + i] += v[i];
+                }
             }
-            tmem_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&drained);
-        }
-        complete = complete && *(volatile int*)&failed == 0;
-        const int row = (warp & 3) * 32 + lane;
-        const long long plane = P == STEP ? x_plane : gram_plane;
+            if (kb + kChunk >= k1) {
 #pragma unroll
-        for (int q = 0; q < C; q += 32) {                             // 32 columns at a time
-            float v[32];
-            tmem_load32(mixed_sum + lanes + col0 + q, v);
-            const int col = col0 + q;
-            const long long to_block = (P == STEP ? (long long)ti * m.col_blocks + (kTileN / 64) * tj
-                                                  : (long long)ti * gram_blocks + (kTileN / 64) * tj) + (col >> 6);
-            uint8_t* to = (P == GRAM ? gram : P == POLY ? poly : x_out) + to_block * kBlockBytes;
-            const uint8_t* from = (P == POLY ? gram : x) + to_block * kBlockBytes;
+                for (int q = 0; q < 4; ++q) {
+                    if (q < 2 || wide) {
+                        float v[32];
+                        tmem_load32(tmem + kMixedColumns + lanes + col0 + q * 32, v);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {                             // 8 columns = one 16-byte chunk
-                const uint32_t at = swizzled_offset(row, ((col & 63) >> 3) + g);
-                Chunk hi, lo, from_hi, from_lo;
-                if (P != GRAM) {
-                    from_hi.raw = *reinterpret_cast<const uint4*>(from + at);
-                    from_lo.raw = *reinterpret_cast<const uint4*>(from + plane + at);
-                }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float r = (sum[q + g * 8 + e] + v[g * 8 + e]) * c1;
-                    if (P != GRAM) r += c0 * (__half2float(from_hi.h[e]) + __half2float(from_lo.h[e]));
-                    if (!complete) r = __int_as_float(0x7fffffff);
-                    split(r, hi.h[e], lo.h[e]);
-                }
-                *reinterpret_cast<uint4*>(to + at) = hi.raw;
-                *reinterpret_cast<uint4*>(to + plane + at) = lo.raw;
-                if (symmetric && ti != tj) {
-                    uint8_t* mirror = (P == GRAM ? gram : poly) + ((long long)tj * gram_blocks + 2 * ti + (row >> 6)) * kBlockBytes;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const uint32_t to_at = swizzled_offset(col + g * 8 + e, (row & 63) >> 3) + (row & 7) * 2;
-                        *reinterpret_cast<__half*>(mirror + to_at) = hi.h[e];
-                        *reinterpret_cast<__half*>(mirror + plane + to_at) = lo.h[e];
+                        for (int i = 0; i < 32; ++i) sum[q * 32 + i] += v[i];
                     }
                 }
             }
+            tmem_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_at(&bar.drained, 0);
         }
+        if (P == GRAM && w.splits > 1) {
+            // [unit][CTA][column][row]
+            float* out = partial + (((long long)u * 2 + cta) * (2 * half) + col0) * 128 + (warp & 3) * 32 + lane;
+#pragma unroll
+            for (int i = 0; i < 128; ++i)
+                if (i < 64 || wide) out[i * 128] = sum[i];
+        } else {
+            const int block = (tj * 2 * half + col0) >> 6;
+            emit(to, 2 * ti + cta, warp & 3, block, sum, c0, c1, staging, lane);
+            if (wide) emit(to, 2 * ti + cta, warp & 3, block + 1, sum + 64, c0, c1, staging, lane);
+        }
+    }
+    return true;
+}
+
+// Writers: adds up the shares of X X^T, 32 rows x 64 columns per warp at a time, in the shares' order.
+__device__ __forceinline__ void reduce_gram(const Walk& w, int cta, const float* partial, const Planes& to, float c0, float c1, uint8_t* staging) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int columns = w.gram_wide ? 256 : 128, strips = columns / 64, tiles = w.tiles(GRAM);
+    for (int i = (w.pair * 2 + cta) * (kWriters / 32) + warp; i < tiles * 2 * strips * 4; i += w.pairs * 2 * (kWriters / 32)) {
+        const int quarter = i & 3, strip = (i >> 2) % strips, half = (i >> 2) / strips, of = half & 1, tile = half >> 1;
+        int ti, tj;
+        symmetric_tile(tile, w.gram_wide, ti, tj);
+        float v[64];
+#pragma unroll
+        for (int c = 0; c < 64; ++c) v[c] = 0.f;
+        for (int s = 0; s < w.splits; ++s) {
+            const float* from = partial + ((((long long)s * tiles + tile) * 2 + of) * columns + strip * 64) * 128 + quarter * 32 + lane;
+#pragma unroll
+            for (int c = 0; c < 64; ++c) v[c] += from[c * 128];
+        }
+        emit(to, 2 * ti + of, quarter, (tj * columns >> 6) + strip, v, c0, c1, staging, lane);
+    }
+}
+
+// The numbers of a step: a product's sums times `factor`, plus `diagonal`. Without c (two coefficients) X X^T gives the
+// polynomial at once and there is no second product.
+struct Polynomial {
+    float gram_factor, gram_diagonal, poly_factor, poly_diagonal, step_factor;
+    int linear;
+};
+
+__global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_constant__ Batch b, int steps, Polynomial poly) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ ChainBarriers bar;
+    __shared__ uint32_t tmem_address;
+    const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
+    uint8_t* stages = smem_raw + pad;                                 // then the warps' staging
+    const int tid = threadIdx.x, warp = tid >> 5;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int cta = int(cluster.block_rank()), pair = int(blockIdx.x >> 1);
+    const int which = find_matrix<&Matrix::pair_first>(b, pair);
+    const Matrix& m = b.m[which];
+
+    __shared__ Walk w;                                                // not in registers: the writers' are full of sums
+    if (tid == 0) {
+        w.x0 = {reinterpret_cast<uint8_t*>(b.x[0]) + m.x_block * kBlockBytes, m.row_tiles, m.col_blocks};
+        w.x1 = {reinterpret_cast<uint8_t*>(b.x[1]) + m.x_block * kBlockBytes, m.row_tiles, m.col_blocks};
+        w.gram = {reinterpret_cast<uint8_t*>(b.gram) + m.gram_block * kBlockBytes, m.row_tiles, 2 * m.row_tiles};
+        w.poly = {reinterpret_cast<uint8_t*>(b.poly) + m.gram_block * kBlockBytes, m.row_tiles, 2 * m.row_tiles};
+        w.pair = pair - m.pair_first;
+        w.pairs = m.pairs;
+        w.splits = m.splits;
+        w.gram_wide = m.gram_wide;
+        w.poly_wide = m.poly_wide;
+        w.step_wide = m.step_wide;
+    }
+    unsigned* counter = b.arrived + which;
+    unsigned* failed = b.arrived + b.n;
+    float* partial = b.partial + m.partial_first;
+    const unsigned ctas = 2 * m.pairs;
+    const int products = 2 + (m.splits > 1) + !poly.linear;           // arrivals of a step
+
+    if (tid == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&bar.full[s], 2);
+            mbar_init(&bar.peer_full[s], 1);
+            mbar_init(&bar.empty[s], 1);
+        }
+        mbar_init(&bar.ready, 1);
+        mbar_init(&bar.drained, 2 * (kWriters / 32));
+        mbar_init(&bar.done, 1);
+        fence_mbar_init();
+    }
+    if (warp == kWriters / 32 + 2) tmem_alloc(&tmem_address, 512);
+    tmem_fence_before();
+    cluster.sync();
+    tmem_fence_after();
+
+    // For each product in turn: f(product, X's buffer, arrivals on the counter that its inputs need). Stops when f fails.
+    auto each_product = [&](auto&& f) {
+        for (int step = 0; step < steps; ++step) {
+            const unsigned before = unsigned(step) * products;
+            if (!f(GRAM, step & 1, before)) return false;
+            if (!poly.linear && !f(POLY, step & 1, before + products - 2)) return false;
+            if (!f(STEP, step & 1, before + products - 1)) return false;
+        }
+        return true;
+    };
+
+    if (tid == kWriters || tid == kWriters + 32) {
+        const bool first = tid == kWriters;                           // the rows' operand, or the columns'
+        unsigned k = 0, s = 0, phase = 1;                             // stages filled since the launch
+        const bool ok = each_product([&](Product p, int from_x, unsigned before) {
+            const int groups = first || w.wide(p) ? 2 : 1;
+            const Planes from = first ? (p == GRAM ? w.x(from_x) : p == POLY ? w.gram : w.poly) : (p == POLY ? w.gram : w.x(from_x));
+            if (!wait_counter(counter, before * ctas)) return false;
+            fence_proxy_async_all();
+            for (int u = w.pair; u < w.units(p); u += w.pairs) {
+                int ti, tj, k0, k1;
+                w.unit(p, u, ti, tj, k0, k1);
+                const int row = first ? ti * 4 + cta * 2 : (tj * 2 + cta) * groups;
+                // of a symmetric matrix the 256 x 256 blocks above the diagonal are read across from below it
+                const int below = p == GRAM ? k1 : !first && p == STEP ? -1 : ((first ? ti : tj * groups / 2) + 1) * 4;
+                for (int kb = k0; kb < k1; ++kb, ++k) {
+                    if (k >= kStages && !mbar_wait_bounded(&bar.empty[s], phase)) return false;
+                    mbar_arrive_expect_tx(&bar.full[s], groups * kHalfBlock);
+                    load_operand(stages + s * kStageBytes + (first ? 0 : kBlockBytes), from, row, groups, kb, kb >= below, &bar.full[s]);
+                    if (++s == kStages) s = 0, phase ^= 1;
+                }
+            }
+            return true;
+        });
+        if (!ok) {
+            // a stage that only the other operand's thread fills does not complete: wait for what was asked for here, with a limit
+            *(volatile unsigned*)failed = 1;
+            for (unsigned i = k > kStages ? k - kStages : 0; i < k; ++i) mbar_wait_bounded(&bar.full[i % kStages], (i / kStages) & 1);
+        }
+    } else if (tid == kWriters + 64 && cta == 1) {
+        unsigned s = 0, phase = 0;
+        const bool ok = each_product([&](Product p, int, unsigned) {
+            for (int u = w.pair; u < w.units(p); u += w.pairs) {
+                int ti, tj, k0, k1;
+                w.unit(p, u, ti, tj, k0, k1);
+                for (int kb = k0; kb < k1; ++kb) {
+                    if (!mbar_wait_bounded(&bar.full[s], phase)) return false;
+                    mbar_arrive_at(&bar.peer_full[s], 0);
+                    if (++s == kStages) s = 0, phase ^= 1;
+                }
+            }
+            return true;
+        });
+        if (!ok) *(volatile unsigned*)failed = 1;
+        mbar_wait_bounded(&bar.done, 0);                              // no MMA reads this CTA when its memory is given up
+    } else if (tid == kWriters + 64) {
+        const uint32_t main_sum = tmem_address, mixed_sum = tmem_address + kMixedColumns;
+        unsigned s = 0, phase = 0, chunk = 0;
+        const bool ok = each_product([&](Product p, int, unsigned) {
+            const int groups_b = w.wide(p) ? 2 : 1;
+            for (int u = w.pair; u < w.units(p); u += w.pairs) {
+                int ti, tj, k0, k1;
+                w.unit(p, u, ti, tj, k0, k1);
+                const int first_b = tj * groups_b / 2;
+                const int below_a = p == GRAM ? k1 : (ti + 1) * 4, below_b = p == GRAM ? k1 : p == STEP ? -1 : (first_b + 1) * 4;
+                for (int kb = k0; kb < k1; ++kb) {
+                    const int of_chunk = (kb - k0) % kChunk;
+                    if (!mbar_wait_bounded(&bar.full[s], phase) || !mbar_wait_cluster(&bar.peer_full[s], phase)) return false;
+                    // a new tile's mixed sums overwrite the last one's: they are read
+                    if (kb == k0 && chunk > 0 && !mbar_wait_cluster(&bar.drained, (chunk - 1) & 1)) return false;
+                    tmem_fence_after();
+                    const uint32_t a = smem_u32(stages + s * kStageBytes), bb = a + kBlockBytes;
+                    const bool across_a = kb >= below_a, across_b = kb >= below_b;
+                    const uint32_t instruction = f16_instruction(256, groups_b * 128, across_a, across_b);
+                    uint64_t a_hi = across_a ? mn_major_descriptor(a, kHalfBlock) : k_major_descriptor(a);
+                    uint64_t b_hi = across_b ? mn_major_descriptor(bb, kHalfBlock) : k_major_descriptor(bb);
+                    const uint64_t step_a = (across_a ? mnMajorStep : kMajorStep) >> 4, step_b = (across_b ? mnMajorStep : kMajorStep) >> 4;
+                    constexpr uint64_t lo = kPlaneOffset >> 4;
+                    // the mixed products first: the writers take the last chunk's sums away meanwhile
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {                     // 16 of the 64 in K
+                        mma_f16(mixed_sum, a_hi + i * step_a, b_hi + i * step_b + lo, instruction, kb > k0 || i > 0);
+                        mma_f16(mixed_sum, a_hi + i * step_a + lo, b_hi + i * step_b, instruction, true);
+                    }
+                    if (of_chunk == 0 && kb > k0) {
+                        if (!mbar_wait_cluster(&bar.drained, (chunk - 1) & 1)) return false;
+                        tmem_fence_after();
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mma_f16(main_sum, a_hi + i * step_a, b_hi + i * step_b, instruction, of_chunk > 0 || i > 0);
+                    mma_commit(&bar.empty[s]);
+                    if (of_chunk == kChunk - 1 || kb == k1 - 1) {
+                        mma_commit(&bar.ready);
+                        ++chunk;
+                    }
+                    if (++s == kStages) s = 0, phase ^= 1;
+                }
+            }
+            return true;
+        });
+        if (!ok) *(volatile unsigned*)failed = 1;
+        mma_commit(&bar.done);
+        mbar_wait_bounded(&bar.done, 0);                              // nothing in flight when the TMEM is freed
+    } else if (warp < kWriters / 32) {
+        unsigned chunk = 0;
+        uint8_t* staging = stages + kStages * kStageBytes + warp * kStagingBytes;
+        auto arrive = [&]() {                                         // this CTA's part of a product is written
+            if ((tid & 31) == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+            __threadfence();
+            fence_proxy_async_all();
+            writers_sync();
+            if (tid == 0) atomicAdd(counter, 1u);
+        };
+        auto wait = [&](unsigned arrivals) {                          // the warp goes on when its first lane has seen the counter
+            int ok = 1;
+            if ((tid & 31) == 0) ok = wait_counter(counter, arrivals * ctas);
+            return __shfl_sync(0xffffffffu, ok, 0) != 0;
+        };
+        const uint32_t tmem = tmem_address;
+        const bool ok = each_product([&](Product p, int from_x, unsigned before) {
+            // a pair without tiles in a product must not arrive for the next one early: the counter has no names
+            if (!wait(before)) return false;
+            if (p == GRAM) {
+                const Planes& to = poly.linear ? w.poly : w.gram;
+                if (!write_product<GRAM>(w, bar, tmem, cta, chunk, to, poly.gram_diagonal, poly.gram_factor, partial, staging)) return false;
+                if (w.splits > 1) {
+                    arrive();
+                    if (!wait(before + 1)) return false;
+                    reduce_gram(w, cta, partial, to, poly.gram_diagonal, poly.gram_factor, staging);
+                }
+            } else if (p == POLY) {
+                if (!write_product<POLY>(w, bar, tmem, cta, chunk, w.poly, poly.poly_diagonal, poly.poly_factor, partial, staging)) return false;
+            } else {
+                if (!write_product<STEP>(w, bar, tmem, cta, chunk, w.x(from_x ^ 1), 0.f, poly.step_factor, partial, staging)) return false;
+            }
+            arrive();
+            return true;
+        });
+        if (!ok) *(volatile unsigned*)failed = 1;
         tmem_fence_before();
     }
-    __syncthreads();
-    if (warp == kWriters / 32 + 1) {
+    __syncwarp();
+    cluster.sync();                                                   // the pair's memory and barriers are used until here
+    if (warp == kWriters / 32 + 2) {
         tmem_fence_after();
-        tmem_free(tmem_address, 2 * kTileN);
+        tmem_free(tmem_address, 512);
     }
 }
 
@@ -695,11 +925,50 @@ __global__ void __launch_bounds__(kShortThreads, 1) short_kernel(const __grid_co
 // ---- host side -------------------------------------------------------------------------------------------------------
 int ceil_div(long long a, long long b) { return int((a + b - 1) / b); }
 
-void fill(const gmc_matrix* matrices, const int* which, int n, Batch* batch, size_t* bytes, uint8_t* workspace) {
+// Cycles of a product with a number of pairs, for the choice of tiles and pairs: per 64 in K a pair's MMAs take 1536 cycles at
+// 256 columns and, bound by shared memory, 950 at 128; a tile costs about 2500 and 1800 more to start and to write.
+long long product_cycles(long long tiles, int wide, long long k_blocks, int pairs) {
+    return (tiles + pairs - 1) / pairs * (wide ? 1536 * k_blocks + 2500 : 950 * k_blocks + 1800);
+}
+long long step_tiles(const Matrix& m, int wide) { return (long long)((m.row_tiles + 1) / 2) * ((m.col_blocks + (wide ? 3 : 1)) / (wide ? 4 : 2)); }
+
+// Chooses tile widths and shares of the columns for a matrix with some pairs; returns the step's cycles.
+long long plan(Matrix& m, int pairs) {
+    const long long barrier = 3000;
+    long long total = 2 * barrier, best = -1;
+    m.pairs = pairs;
+    for (int wide = 0; wide < 2; ++wide) {
+        const long long tiles = symmetric_tiles(m.row_tiles, wide);
+        for (int splits = 1; splits <= 32; splits *= 2) {
+            if (splits > 1 && (tiles * splits > pairs || m.col_blocks < 4 * splits)) break;
+            const long long reduce = splits > 1 ? barrier + 1500 + 400 * splits * ((tiles * (wide ? 64 : 32) + pairs * 16 - 1) / (pairs * 16)) : 0;
+            const long long t = product_cycles(tiles * splits, wide, m.col_blocks / splits, pairs) + reduce;
+            if (best < 0 || t < best) best = t, m.gram_wide = wide, m.splits = splits;
+        }
+    }
+    total += best;
+    const long long p0 = product_cycles(symmetric_tiles(m.row_tiles, 0), 0, 2 * m.row_tiles, pairs);
+    const long long p1 = product_cycles(symmetric_tiles(m.row_tiles, 1), 1, 2 * m.row_tiles, pairs);
+    m.poly_wide = p1 <= p0;
+    const long long s0 = product_cycles(step_tiles(m, 0), 0, 2 * m.row_tiles, pairs), s1 = product_cycles(step_tiles(m, 1), 1, 2 * m.row_tiles, pairs);
+    m.step_wide = s1 <= s0;
+    return total + (p1 <= p0 ? p1 : p0) + (s1 <= s0 ? s1 : s0) + barrier;
+}
+
+// Pairs beyond this have nothing to do.
+long long most_units(const Matrix& m) {
+    const long long gram = (long long)symmetric_tiles(m.row_tiles, 0) * (m.col_blocks / 4 > 1 ? m.col_blocks / 4 : 1);
+    const long long step = step_tiles(m, 0);
+    return gram > step ? gram : step;
+}
+
+// Lays out the workspace and hands out `pairs` CTA pairs: one each, the others to whoever takes longest.
+void fill(const gmc_matrix* matrices, const int* which, int n, int pairs, Batch* batch, size_t* bytes, uint8_t* workspace) {
     Batch& b = *batch;
     b.n = n;
-    long long x_blocks = 0, gram_blocks = 0;
-    b.norm_ctas = b.gram_ctas = b.step_ctas = b.blocks = 0;
+    long long x_blocks = 0, gram_blocks = 0, partials = 0;
+    b.norm_ctas = b.blocks = 0;
+    long long cycles[kMaxMatrices];
     for (int i = 0; i < n; ++i) {
         const gmc_matrix& g = matrices[which[i]];
         Matrix& m = b.m[i];
@@ -715,18 +984,32 @@ void fill(const gmc_matrix* matrices, const int* which, int n, Batch* batch, siz
         m.row_tiles = ceil_div(wide_rows, 128);
         m.col_blocks = 2 * ceil_div(wide_cols, 128);
         m.norm_first = b.norm_ctas;
-        m.gram_first = b.gram_ctas;
-        m.step_first = b.step_ctas;
         m.block_first = b.blocks;
         m.x_block = x_blocks;
         m.gram_block = gram_blocks;
         const long long blocks = (long long)m.row_tiles * m.col_blocks;
         b.norm_ctas += ceil_div(g.rows * g.cols, kNormElements);
-        b.gram_ctas += m.row_tiles * (m.row_tiles + 1) / 2;
-        b.step_ctas += int(blocks / 2);
         b.blocks += int(blocks);
-        x_blocks += 2 * blocks;
-        gram_blocks += 2LL * m.row_tiles * 2 * m.row_tiles;
+        x_blocks += blocks;
+        gram_blocks += 2LL * m.row_tiles * m.row_tiles;
+        cycles[i] = plan(m, 1);
+    }
+    for (int left = pairs - n; left > 0; --left) {
+        int most = -1;
+        for (int i = 0; i < n; ++i)
+            if (b.m[i].pairs < most_units(b.m[i]) && (most < 0 || cycles[i] > cycles[most])) most = i;
+        if (most < 0) break;
+        cycles[most] = plan(b.m[most], b.m[most].pairs + 1);
+    }
+    b.pairs = 0;
+    bool splittable = false;
+    for (int i = 0; i < n; ++i) {
+        Matrix& m = b.m[i];
+        m.pair_first = b.pairs;
+        b.pairs += m.pairs;
+        m.partial_first = partials;
+        if (m.splits > 1) partials += (long long)symmetric_tiles(m.row_tiles, m.gram_wide) * m.splits * 256 * (m.gram_wide ? 256 : 128);
+        splittable = splittable || m.row_tiles <= 16;
     }
     size_t at = 0;
     auto take = [&](size_t size) {
@@ -738,8 +1021,39 @@ void fill(const gmc_matrix* matrices, const int* which, int n, Batch* batch, siz
     b.x[1] = reinterpret_cast<__half*>(take(size_t(x_blocks) * kBlockBytes));
     b.gram = reinterpret_cast<__half*>(take(size_t(gram_blocks) * kBlockBytes));
     b.poly = reinterpret_cast<__half*>(take(size_t(gram_blocks) * kBlockBytes));
-    b.partial = reinterpret_cast<double*>(take(size_t(b.norm_ctas) * sizeof(double)));
+    b.squares = reinterpret_cast<double*>(take(size_t(b.norm_ctas) * sizeof(double)));
+    // a matrix has no more tiles times shares than pairs, and none of 17 row tiles or more (9 x 10 / 2 tiles) has shares: the
+    // size holds for any number of pairs up to kPairs
+    b.partial = reinterpret_cast<float*>(take(splittable ? size_t(kPairs) * 256 * 256 * sizeof(float) : 0));
+    b.arrived = reinterpret_cast<unsigned*>(take(size_t(n + 1) * sizeof(unsigned)));
     *bytes = at;
+}
+
+// Pairs of CTAs of the chain that the current device holds at once: a property of the device, asked for once per device.
+int chain_pairs(int* pairs) {
+    static std::atomic<int> known[64];
+    int device = 0;
+    GMC_CUDA_TRY(cudaGetDevice(&device));
+    if (device < 64 && known[device].load() > 0) {
+        *pairs = known[device].load();
+        return GMC_OK;
+    }
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(2 * kPairs);
+    config.blockDim = dim3(kChainThreads);
+    config.dynamicSmemBytes = kChainSmem;
+    cudaLaunchAttribute attribute;
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = 2;
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    GMC_CUDA_TRY(cudaFuncSetAttribute(chain_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kChainSmem));
+    GMC_CUDA_TRY(cudaOccupancyMaxActiveClusters(pairs, chain_kernel, &config));
+    if (*pairs > kPairs) *pairs = kPairs;
+    if (*pairs < kMaxMatrices) return GMC_ERR_UNSUPPORTED;
+    if (device < 64) known[device].store(*pairs);
+    return GMC_OK;
 }
 
 constexpr long long kMaxSide = 32768;
@@ -754,48 +1068,64 @@ int check_matrices(const gmc_matrix* matrices, int n) {
     return GMC_OK;
 }
 
-// Bounds of the iterates on [0, 1]: the planes' scales leave room for |X| < 1.4 and |b A + c A A| < 3.9. The extrema of
-// x (a + b x^2 + c x^4) and b l + c l^2 lie at the end of the interval or where the derivative is zero.
-int check_polynomial(int steps, float a, float b, float c) {
+// Bounds of the iterates and of the polynomial for singular values in [0, 1], and from them the planes' scales: powers of two
+// that keep every value below the largest fp16 number. The extrema of x (a + b x^2 + c x^4) and of a + b l + c l^2 lie at
+// the ends of the interval or where the derivative is zero.
+int make_polynomial(int steps, float a, float b, float c, Polynomial* out) {
     if (steps < 1 || steps > 32) return GMC_ERR_UNSUPPORTED;
     const double da = a, db = b, dc = c;
+    if (!(fabs(da) < 100. && fabs(db) < 100. && fabs(dc) < 100.)) return GMC_ERR_UNSUPPORTED;
+    const double shift = dc != 0. ? db / (2. * dc) : 0.;
+    if (fabs(shift) > 16.) return GMC_ERR_UNSUPPORTED;
     const double root = sqrt(fmax(0., 9. * db * db - 20. * da * dc));
-    double top = 1.;
+    double top = 1., poly = fabs(da);
     for (int s = 0; s < steps; ++s) {
         const double end = top * top;
-        const double at[4] = {end, (-3. * db + root) / (10. * dc), (-3. * db - root) / (10. * dc), -db / (2. * dc)};
-        double next = 0., poly = 0.;
+        double at[4] = {end, end, end, end};
+        if (dc != 0.) at[1] = (-3. * db + root) / (10. * dc), at[2] = (-3. * db - root) / (10. * dc), at[3] = -shift;
+        else if (db != 0.) at[1] = -da / (3. * db);
+        double next = 0.;
         for (double l : at) {
-            if (dc == 0. && l != end) l = db != 0. ? -da / (3. * db) : end;
             if (!(l > 0. && l <= end)) continue;
-            next = fmax(next, fabs(sqrt(l) * (da + l * (db + dc * l))));
-            poly = fmax(poly, fabs(l * (db + dc * l)));
+            const double f = da + l * (db + dc * l);
+            next = fmax(next, fabs(sqrt(l) * f));
+            poly = fmax(poly, fabs(f));
         }
-        if (!(poly < 3.9) || !(next < 1.4)) return GMC_ERR_UNSUPPORTED;
+        if (!(next < 1.8)) return GMC_ERR_UNSUPPORTED;
         top = next;
     }
-    return da == da && db == db && dc == dc ? GMC_OK : GMC_ERR_UNSUPPORTED;
+    auto scale_for = [](double most) { return exp2(floor(log2(60000. / most))); };
+    const double sx = kScaleX, ss = scale_for(fabs(shift) + 1.8 * 1.8), sp = scale_for(poly);
+    out->linear = dc == 0.;
+    out->gram_factor = float(dc != 0. ? ss / (sx * sx) : db * sp / (sx * sx));
+    out->gram_diagonal = float(dc != 0. ? shift * ss : da * sp);
+    out->poly_factor = float(dc * sp / (ss * ss));
+    out->poly_diagonal = float((da - dc * shift * shift) * sp);
+    out->step_factor = float(1. / sp);
+    return GMC_OK;
 }
 
 template <typename T, bool MUON>
-int run_batch(const Batch& b, int steps, float ca, float cb, float cc, float epsilon, const Momentum& mo, cudaStream_t stream) {
+int run_batch(const Batch& b, int steps, const Polynomial& poly, float epsilon, const Momentum& mo, cudaStream_t stream) {
     norm_kernel<T, MUON><<<b.norm_ctas, 256, 0, stream>>>(b, mo);
     GMC_LAUNCH_CHECK();
     split_kernel<T, MUON><<<b.blocks, 256, 0, stream>>>(b, mo, epsilon);
     GMC_LAUNCH_CHECK();
-    GMC_CUDA_TRY(cudaFuncSetAttribute(product_kernel<GRAM>, cudaFuncAttributeMaxDynamicSharedMemorySize, kProductSmem));
-    GMC_CUDA_TRY(cudaFuncSetAttribute(product_kernel<POLY>, cudaFuncAttributeMaxDynamicSharedMemorySize, kProductSmem));
-    GMC_CUDA_TRY(cudaFuncSetAttribute(product_kernel<STEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kProductSmem));
-    int x = 0;
-    for (int s = 0; s < steps; ++s, x ^= 1) {
-        product_kernel<GRAM><<<b.gram_ctas, kProductThreads, kProductSmem, stream>>>(b, x, 0.f, kScaleA / (kScaleX * kScaleX));
-        GMC_LAUNCH_CHECK();
-        product_kernel<POLY><<<b.gram_ctas, kProductThreads, kProductSmem, stream>>>(b, x, cb * (kScaleB / kScaleA), cc * (kScaleB / (kScaleA * kScaleA)));
-        GMC_LAUNCH_CHECK();
-        product_kernel<STEP><<<b.step_ctas, kProductThreads, kProductSmem, stream>>>(b, x, ca, 1.f / kScaleB);
-        GMC_LAUNCH_CHECK();
-    }
-    finish_kernel<T, MUON><<<b.blocks, 256, 0, stream>>>(b, mo, x);
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(unsigned(2 * b.pairs));
+    config.blockDim = dim3(kChainThreads);
+    config.dynamicSmemBytes = kChainSmem;
+    config.stream = stream;
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeClusterDimension;
+    attributes[0].val.clusterDim.x = 2;
+    attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
+    attributes[1].id = cudaLaunchAttributeCooperative;
+    attributes[1].val.cooperative = 1;
+    config.attrs = attributes;
+    config.numAttrs = 2;
+    GMC_CUDA_TRY(cudaLaunchKernelEx(&config, chain_kernel, b, steps, poly));
+    finish_kernel<T, MUON><<<b.blocks, 256, 0, stream>>>(b, mo, steps & 1);
     GMC_LAUNCH_CHECK();
     return GMC_OK;
 }
@@ -851,7 +1181,7 @@ int run_short(const gmc_matrix* matrices, const int* which, int n, int steps, fl
 }
 
 template <typename T, bool MUON>
-int run_typed(const gmc_matrix* matrices, int n, int steps, float ca, float cb, float cc, float epsilon, const Momentum& mo,
+int run_typed(const gmc_matrix* matrices, int n, int steps, float ca, float cb, float cc, const Polynomial& poly, float epsilon, const Momentum& mo,
               void* workspace, size_t workspace_bytes, cudaStream_t stream) {
     int which[kMaxMatrices], count = 0;
     for (int pass = 0; pass < 2; ++pass) {
@@ -863,9 +1193,11 @@ int run_typed(const gmc_matrix* matrices, int n, int steps, float ca, float cb, 
                 } else {
                     Batch b;
                     size_t bytes = 0;
-                    fill(matrices, which, count, &b, &bytes, static_cast<uint8_t*>(workspace));
+                    int pairs = 0;
+                    if (int s = chain_pairs(&pairs)) return s;
+                    fill(matrices, which, count, pairs, &b, &bytes, static_cast<uint8_t*>(workspace));
                     if (bytes > workspace_bytes) return GMC_ERR_WORKSPACE;
-                    if (int s = run_batch<T, MUON>(b, steps, ca, cb, cc, epsilon, mo, stream)) return s;
+                    if (int s = run_batch<T, MUON>(b, steps, poly, epsilon, mo, stream)) return s;
                 }
                 count = 0;
             }
@@ -882,7 +1214,7 @@ size_t workspace_bytes_of(const gmc_matrix* matrices, int n) {
         if (count == kMaxMatrices || (i == n && count > 0)) {
             Batch b;
             size_t bytes = 0;
-            fill(matrices, which, count, &b, &bytes, nullptr);
+            fill(matrices, which, count, kPairs, &b, &bytes, nullptr);
             most = bytes > most ? bytes : most;
             count = 0;
         }
@@ -896,7 +1228,8 @@ int run(const gmc_matrix* matrices, int n, int dtype, int steps, float ca, float
     if (int s = check_matrices(matrices, n)) return s;
     if (dtype < GMC_FLOAT32 || dtype > GMC_FLOAT16) return GMC_ERR_UNSUPPORTED;
     if (!(epsilon >= 1e-30f && epsilon <= 1e30f)) return GMC_ERR_UNSUPPORTED;
-    if (int s = check_polynomial(steps, ca, cb, cc)) return s;
+    Polynomial poly;
+    if (int s = make_polynomial(steps, ca, cb, cc, &poly)) return s;
     for (int i = 0; i < n; ++i)
         if (!matrices[i].update || !matrices[i].out || (MUON && !matrices[i].momentum)) return GMC_ERR_NULL_POINTER;
     if (reinterpret_cast<uintptr_t>(workspace) & 1023u) return GMC_ERR_UNSUPPORTED;
@@ -904,9 +1237,9 @@ int run(const gmc_matrix* matrices, int n, int dtype, int steps, float ca, float
     if (need > 0 && !workspace) return GMC_ERR_NULL_POINTER;
     if (need > workspace_bytes) return GMC_ERR_WORKSPACE;
     cudaStream_t cs = as_stream(stream);
-    if (dtype == GMC_FLOAT32) return run_typed<float, MUON>(matrices, n, steps, ca, cb, cc, epsilon, mo, workspace, workspace_bytes, cs);
-    if (dtype == GMC_BFLOAT16) return run_typed<__nv_bfloat16, MUON>(matrices, n, steps, ca, cb, cc, epsilon, mo, workspace, workspace_bytes, cs);
-    return run_typed<__half, MUON>(matrices, n, steps, ca, cb, cc, epsilon, mo, workspace, workspace_bytes, cs);
+    if (dtype == GMC_FLOAT32) return run_typed<float, MUON>(matrices, n, steps, ca, cb, cc, poly, epsilon, mo, workspace, workspace_bytes, cs);
+    if (dtype == GMC_BFLOAT16) return run_typed<__nv_bfloat16, MUON>(matrices, n, steps, ca, cb, cc, poly, epsilon, mo, workspace, workspace_bytes, cs);
+    return run_typed<__half, MUON>(matrices, n, steps, ca, cb, cc, poly, epsilon, mo, workspace, workspace_bytes, cs);
 }
 
 }  // namespace

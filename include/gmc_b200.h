@@ -371,8 +371,8 @@ int gmc_log_probabilities_backward(const void* logits, int dtype, const long lon
  * momentum is contiguous fp32. Matrices may differ in shape; 1 <= rows, cols <= 32768. A zero matrix gives zero; NaN or
  * infinity in a matrix makes that matrix NaN. out may be update (the same address and stride), no other overlap is allowed
  * within a call, and no matrix may appear twice. Products are accurate to fp32 rounding whatever `dtype`.
- * 1 <= steps <= 32; coefficients whose iterates leave |X| < 1.4, |b A + c A A| < 3.9 for singular values in [0, 1] are
- * refused (GMC_ERR_UNSUPPORTED); 1e-30 <= epsilon <= 1e30; 0 <= momentum < 1.
+ * 1 <= steps <= 32; coefficients whose iterates reach 1.8 for a singular value in [0, 1], that are 100 or more, or with
+ * |b| > 32 |c| > 0 are refused (GMC_ERR_UNSUPPORTED); 1e-30 <= epsilon <= 1e30; 0 <= momentum < 1.
  * workspace: gmc_orthogonalise_workspace_bytes (depends on the shapes only; 0 = none needed, or sizes out of range), aligned
  * to 1024 bytes, content undefined before and after; concurrent calls need one each. Nothing is allocated, kept or
  * synchronised.
