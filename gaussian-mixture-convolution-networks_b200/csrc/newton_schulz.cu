@@ -307,12 +307,24 @@ __device__ __forceinline__ bool wait_counter(const unsigned* counter, unsigned v
 __device__ __forceinline__ void fence_proxy_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
 __device__ __forceinline__ void writers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWriters) : "memory"); }
 
-__device__ __forceinline__ void split8(const float* v, float c1, float c0, const Chunk* in_hi, const Chunk* in_lo, Chunk& hi, Chunk& lo) {
+// Eight columns: v c1, plus c0 (in_hi + in_lo), as planes.
+template <bool ADD>
+__device__ __forceinline__ void split8(const float* v, float c1, float c0, const uint4& in_hi, const uint4& in_lo, uint4& hi, uint4& lo) {
+    const __half2* ih = reinterpret_cast<const __half2*>(&in_hi);
+    const __half2* il = reinterpret_cast<const __half2*>(&in_lo);
+    __half2* oh = reinterpret_cast<__half2*>(&hi);
+    __half2* ol = reinterpret_cast<__half2*>(&lo);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        float r = v[e] * c1;
-        if (in_hi) r += c0 * (__half2float(in_hi->h[e]) + __half2float(in_lo->h[e]));
-        split(r, hi.h[e], lo.h[e]);
+    for (int e = 0; e < 4; ++e) {
+        float x = v[2 * e] * c1, y = v[2 * e + 1] * c1;
+        if (ADD) {
+            const float2 h = __half22float2(ih[e]), l = __half22float2(il[e]);
+            x += c0 * (h.x + l.x);
+            y += c0 * (h.y + l.y);
+        }
+        oh[e] = __floats2half2_rn(x, y);
+        const float2 back = __half22float2(oh[e]);
+        ol[e] = __floats2half2_rn(x - back.x, y - back.y);
     }
 }
 
@@ -320,46 +332,53 @@ struct ChainBarriers {
     uint64_t full[kStages], peer_full[kStages], empty[kStages], ready, drained, mixed_ready, mixed_drained, done;
 };
 
+// One lane polls for its warp.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, unsigned parity) {
+    int ok = 1;
+    if ((threadIdx.x & 31) == 0) ok = mbar_wait_bounded(bar, parity);
+    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+
 // Writers: the tiles of one product. `chunk`, `tile`, `k` count the chunks, tiles and stages since the launch.
 struct WriterCounts {
     unsigned chunk, tile, k;
 };
-template <Product P>
-__device__ __forceinline__ bool write_product(const Walk& w, ChainBarriers& bar, uint8_t* stages, uint32_t tmem, int cta, WriterCounts& n,
-                                              const Planes& to, float c0, float c1, int stages_per_chunk, float* partial) {
+__device__ __forceinline__ bool write_product(Product p, const Walk& w, ChainBarriers& bar, uint8_t* stages, uint32_t tmem, int cta,
+                                              WriterCounts& n, const Planes& to, float c0, float c1, int stages_per_chunk, float* partial) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-    const int wide = w.wide(P), half = wide ? 128 : 64, col0 = (warp >> 2) * half;
-    for (int u = w.pair; u < w.units(P); u += w.pairs, ++n.tile) {
+    const int wide = w.wide(p), half = wide ? 128 : 64, col0 = (warp >> 2) * half;
+    const int units = w.units(p);
+    for (int u = w.pair; u < units; u += w.pairs, ++n.tile) {
         int ti, tj, k0, k1;
-        w.unit(P, u, ti, tj, k0, k1);
+        w.unit(p, u, ti, tj, k0, k1);
         const int diagonal = (2 * ti + cta) * 128 + (warp & 3) * 32 + lane - tj * 2 * half - col0;       // this row's
         float sum[128];
 #pragma unroll
         for (int i = 0; i < 128; ++i) sum[i] = 0.f;
         for (int kb = k0; kb < k1; kb += stages_per_chunk, ++n.chunk) {
-            if (!mbar_wait_bounded(&bar.ready, n.chunk & 1)) return false;
+            if (!warp_wait(&bar.ready, n.chunk & 1)) return false;
             tmem_fence_after();
             // The mean of what the chunk's n = 4 additions per stage have lost. X X^T: measured 2.0 n 2^-25 where all terms have
             // one sign (the diagonal), 0.7 n 2^-25 where signs are random; 1.3 leaves a third of either. A A and B X: one term,
             // with the diagonal's element, is much larger than the others, and the half of the additions that follow it lose
             // half a step each, 0.72 n 2^-25 over all mantissas.
             const float loss = 0x1p-25f * 4.f * float(min(stages_per_chunk, k1 - kb));
-            const float made_good = 1.f + 0.7f * loss, diagonal_good = 1.f + (P == GRAM ? 2.f : 2.4f) * loss;
+            const float made_good = 1.f + 0.7f * loss, diagonal_good = 1.f + (p == GRAM ? 2.f : p == POLY ? 2.4f : 0.7f) * loss;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 if (q < 2 || wide) {
                     float v[32];
                     tmem_load32(tmem + lanes + col0 + q * 32, v);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) sum[q * 32 + i] += v[i] * (P != STEP && q * 32 + i == diagonal ? diagonal_good : made_good);
+                    for (int i = 0; i < 32; ++i) sum[q * 32 + i] += v[i] * (q * 32 + i == diagonal ? diagonal_good : made_good);
                 }
             }
             tmem_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_at(&bar.drained, 0);
         }
-        if (!mbar_wait_bounded(&bar.mixed_ready, n.tile & 1)) return false;
+        if (!warp_wait(&bar.mixed_ready, n.tile & 1)) return false;
         tmem_fence_after();
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -374,7 +393,7 @@ __device__ __forceinline__ bool write_product(const Walk& w, ChainBarriers& bar,
         __syncwarp();
         if (lane == 0) mbar_arrive_at(&bar.mixed_drained, 0);
         n.k += k1 - k0;
-        if (P == GRAM && w.splits > 1) {
+        if (p == GRAM && w.splits > 1) {
             // [unit][CTA][column][row]
             float* out = partial + (((long long)u * 2 + cta) * (2 * half) + col0) * 128 + (warp & 3) * 32 + lane;
 #pragma unroll
@@ -385,25 +404,30 @@ __device__ __forceinline__ bool write_product(const Walk& w, ChainBarriers& bar,
         // the stages behind the tile's: two blocks each. Wide: warps 0-3 have the first one's, warps 4-7 the second one's.
         const unsigned k = n.k + (wide ? warp >> 2 : 0), s = k % kStages;
         n.k += wide ? 2 : 1;
-        if (!mbar_wait_bounded(&bar.full[s], (k / kStages) & 1)) return false;
+        if (!warp_wait(&bar.full[s], (k / kStages) & 1)) return false;
         const int row_block = 2 * ti + cta;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             if (j == 0 || wide) {
                 uint8_t* rows = stages + s * kStageBytes + (wide ? j : warp >> 2) * kBlockBytes + (warp & 3) * kWarpRows;
+                // in place; the next chunk is read before this one is written, which the compiler could not know to be safe
+                uint4 next_hi = {}, next_lo = {};
+                if (p != GRAM) {
+                    next_hi = *reinterpret_cast<const uint4*>(rows + swizzled_offset(lane, 0));
+                    next_lo = *reinterpret_cast<const uint4*>(rows + swizzled_offset(lane, 0) + kPlaneOffset);
+                }
 #pragma unroll
                 for (int g = 0; g < 8; ++g) {
                     uint8_t* at = rows + swizzled_offset(lane, g);
-                    Chunk hi, lo, in_hi, in_lo;
-                    if (P != GRAM) {
-                        in_hi.raw = *reinterpret_cast<const uint4*>(at);
-                        in_lo.raw = *reinterpret_cast<const uint4*>(at + kPlaneOffset);
-                        split8(sum + j * 64 + g * 8, c1, c0, &in_hi, &in_lo, hi, lo);
-                    } else {
-                        split8(sum + j * 64 + g * 8, c1, 0.f, nullptr, nullptr, hi, lo);
+                    const uint4 in_hi = next_hi, in_lo = next_lo;
+                    if (g < 7 && p != GRAM) {
+                        next_hi = *reinterpret_cast<const uint4*>(rows + swizzled_offset(lane, g + 1));
+                        next_lo = *reinterpret_cast<const uint4*>(rows + swizzled_offset(lane, g + 1) + kPlaneOffset);
                     }
-                    *reinterpret_cast<uint4*>(at) = hi.raw;
-                    *reinterpret_cast<uint4*>(at + kPlaneOffset) = lo.raw;
+                    uint4 hi, lo;
+                    split8<true>(sum + j * 64 + g * 8, c1, c0, in_hi, in_lo, hi, lo);
+                    *reinterpret_cast<uint4*>(at) = hi;
+                    *reinterpret_cast<uint4*>(at + kPlaneOffset) = lo;
                 }
                 fence_proxy_async();
                 __syncwarp();
@@ -451,11 +475,11 @@ __device__ __forceinline__ void reduce_gram(const Walk& w, int cta, const float*
         uint8_t* out = to.block(row_block, col >> 6) + quarter * kWarpRows;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            Chunk hi, lo;
-            split8(v + g * 8, c1, 0.f, nullptr, nullptr, hi, lo);
+            uint4 none = {}, hi, lo;
+            split8<false>(v + g * 8, c1, 0.f, none, none, hi, lo);
             uint8_t* at = out + swizzled_offset(lane, ((col & 63) >> 3) + g);
-            *reinterpret_cast<uint4*>(at) = hi.raw;
-            *reinterpret_cast<uint4*>(at + kPlaneOffset) = lo.raw;
+            *reinterpret_cast<uint4*>(at) = hi;
+            *reinterpret_cast<uint4*>(at + kPlaneOffset) = lo;
         }
     }
 }
@@ -519,10 +543,11 @@ __global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_co
     // For each product in turn: f(product, X's buffer, arrivals on the counter that its inputs need). Stops when f fails.
     auto each_product = [&](auto&& f) {
         for (int step = 0; step < steps; ++step) {
-            const unsigned before = unsigned(step) * products;
-            if (!f(GRAM, step & 1, before)) return false;
-            if (!poly.linear && !f(POLY, step & 1, before + products - 2)) return false;
-            if (!f(STEP, step & 1, before + products - 1)) return false;
+#pragma unroll 1                                                      // one copy of the code: three do not fit the instruction cache
+            for (int p = GRAM; p <= STEP; ++p) {
+                if (p == POLY && poly.linear) continue;
+                if (!f(Product(p), step & 1, unsigned(step) * products + (p == GRAM ? 0 : p == POLY ? products - 2 : products - 1))) return false;
+            }
         }
         return true;
     };
@@ -533,11 +558,14 @@ __global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_co
         const bool ok = each_product([&](Product p, int from_x, unsigned before) {
             const int groups = first || w.wide(p) ? 2 : 1;
             const Planes from = first ? (p == GRAM ? w.x(from_x) : p == POLY ? w.gram : w.poly) : (p == POLY ? w.gram : w.x(from_x));
-            if (!wait_counter(counter, before * ctas)) return false;
-            fence_proxy_async_all();
-            for (int u = w.pair; u < w.units(p); u += w.pairs) {
+            const int units = w.units(p);
+            for (int u = w.pair; u < units; u += w.pairs) {
                 int ti, tj, k0, k1;
                 w.unit(p, u, ti, tj, k0, k1);
+                if (u == w.pair) {
+                    if (!wait_counter(counter, before * ctas)) return false;
+                    fence_proxy_async_all();
+                }
                 const int row = first ? ti * 4 + cta * 2 : (tj * 2 + cta) * groups;
                 // of a symmetric matrix the 256 x 256 blocks above the diagonal are read across from below it
                 const int below = p == GRAM ? k1 : !first && p == STEP ? -1 : ((first ? ti : tj * groups / 2) + 1) * 4;
@@ -589,15 +617,16 @@ __global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_co
     } else if ((tid == kWriters + 64 || tid == kWriters + 96) && cta == 0) {
         const bool mixed = tid == kWriters + 64;
         const uint32_t sums = mixed ? tmem_address + kMixedColumns : tmem_address;
+        const int chunk_stages = m.chunk;
         unsigned s = 0, phase = 0, peer_phase = 0, chunk = 0, tile = 0;                // peer_phase: one bit per stage
         const bool ok = each_product([&](Product p, int, unsigned) {
             const int groups_b = w.wide(p) ? 2 : 1;
             for (int u = w.pair; u < w.units(p); u += w.pairs, ++tile) {
                 int ti, tj, k0, k1;
                 w.unit(p, u, ti, tj, k0, k1);
+                int of_chunk = 0;
                 const int below_a = p == GRAM ? k1 : (ti + 1) * 4, below_b = p == GRAM ? k1 : p == STEP ? -1 : (tj * groups_b / 2 + 1) * 4;
                 for (int kb = k0; kb < k1; ++kb) {
-                    const int of_chunk = (kb - k0) % m.chunk;
                     const uint32_t a = smem_u32(stages + s * kStageBytes), bb = a + kBlockBytes;
                     const bool across_a = kb >= below_a, across_b = kb >= below_b;
                     const uint32_t instruction = f16_instruction(256, groups_b * 128, across_a, across_b);
@@ -627,10 +656,11 @@ __global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_co
                     mma_commit(&bar.empty[s]);
                     if (mixed) {
                         if (kb == k1 - 1) mma_commit(&bar.mixed_ready);
-                    } else if (of_chunk == m.chunk - 1 || kb == k1 - 1) {
+                    } else if (of_chunk == chunk_stages - 1 || kb == k1 - 1) {
                         mma_commit(&bar.ready);
                         ++chunk;
                     }
+                    if (++of_chunk == chunk_stages) of_chunk = 0;
                     if (++s == kStages) s = 0, phase ^= 1;
                 }
                 for (int e = 0; e < w.extra(p); ++e)
@@ -643,12 +673,14 @@ __global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_co
         mbar_wait_bounded(&bar.done, 0);                              // nothing in flight when the TMEM is freed
     } else if (warp < kWriters / 32) {
         WriterCounts n = {0, 0, 0};
-        auto arrive = [&]() {                                         // this CTA's part of a product is written
+        // This CTA's part of a product is written: by bulk copies, for which the lanes that issued them wait, or by all threads
+        // with plain stores. Others read it by bulk copies.
+        auto arrive = [&](bool plain) {
             if ((tid & 31) == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-            __threadfence();
-            fence_proxy_async_all();
+            if (plain) __threadfence();
+            if (plain || (tid & 31) == 0) fence_proxy_async_all();
             writers_sync();
-            if (tid == 0) atomicAdd(counter, 1u);
+            if (tid == 0) asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(counter) : "memory");
         };
         auto wait = [&](unsigned arrivals) {                          // the warp goes on when its first lane has seen the counter
             int ok = 1;
@@ -659,20 +691,16 @@ __global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_co
         const bool ok = each_product([&](Product p, int from_x, unsigned before) {
             // a pair without tiles in a product must not arrive for the next one early: the counter has no names
             if (!wait(before)) return false;
-            if (p == GRAM) {
-                const Planes& to = poly.linear ? w.poly : w.gram;
-                if (!write_product<GRAM>(w, bar, stages, tmem, cta, n, to, 0.f, poly.gram_factor, m.chunk, partial)) return false;
-                if (w.splits > 1) {
-                    arrive();
-                    if (!wait(before + 1)) return false;
-                    reduce_gram(w, cta, partial, to, poly.gram_factor);
-                }
-            } else if (p == POLY) {
-                if (!write_product<POLY>(w, bar, stages, tmem, cta, n, w.poly, poly.poly_from, poly.poly_factor, m.chunk, partial)) return false;
-            } else {
-                if (!write_product<STEP>(w, bar, stages, tmem, cta, n, w.x(from_x ^ 1), poly.step_from, poly.step_factor, m.chunk, partial)) return false;
+            const Planes& to = p == STEP ? w.x(from_x ^ 1) : p == POLY || poly.linear ? w.poly : w.gram;
+            const float c0 = p == STEP ? poly.step_from : p == POLY ? poly.poly_from : 0.f;
+            const float c1 = p == STEP ? poly.step_factor : p == POLY ? poly.poly_factor : poly.gram_factor;
+            if (!write_product(p, w, bar, stages, tmem, cta, n, to, c0, c1, m.chunk, partial)) return false;
+            if (p == GRAM && w.splits > 1) {
+                arrive(true);
+                if (!wait(before + 1)) return false;
+                reduce_gram(w, cta, partial, to, c1);
             }
-            arrive();
+            arrive(p == GRAM && w.splits > 1);
             return true;
         });
         if (!ok) *(volatile unsigned*)failed = 1;
@@ -993,23 +1021,24 @@ __global__ void __launch_bounds__(kShortThreads, 1) short_kernel(const __grid_co
 // ---- host side -------------------------------------------------------------------------------------------------------
 int ceil_div(long long a, long long b) { return int((a + b - 1) / b); }
 
-// Cycles of a product with a number of pairs, for the choice of tiles and pairs: per 64 in K a pair's MMAs take 1536 cycles at
-// 256 columns and, bound by shared memory, 950 at 128; a tile costs about 2500 and 1800 more to start and to write.
+// Cycles of a product with a number of pairs, for the choice of tiles and pairs: measured per 64 in K 1520 cycles at 256
+// columns (the MMAs' own time is 1536) and 1440 at 128 (the barriers' latencies, behind the operands' traffic in shared
+// memory); a tile costs about 8000 and 6000 more to start and to write.
 long long product_cycles(long long tiles, int wide, long long k_blocks, int pairs) {
-    return (tiles + pairs - 1) / pairs * (wide ? 1536 * k_blocks + 2500 : 950 * k_blocks + 1800);
+    return (tiles + pairs - 1) / pairs * (wide ? 1520 * k_blocks + 8000 : 1440 * k_blocks + 6000);
 }
 long long step_tiles(const Matrix& m, int wide) { return (long long)((m.row_tiles + 1) / 2) * ((m.col_blocks + (wide ? 3 : 1)) / (wide ? 4 : 2)); }
 
 // Chooses tile widths and shares of the columns for a matrix with some pairs; returns the step's cycles.
 long long plan(Matrix& m, int pairs) {
-    const long long barrier = 3000;
+    const long long barrier = 8000;
     long long total = 2 * barrier, best = -1;
     m.pairs = pairs;
     for (int wide = 0; wide < 2; ++wide) {
         const long long tiles = symmetric_tiles(m.row_tiles, wide);
         for (int splits = 1; splits <= 32; splits *= 2) {
             if (splits > 1 && (tiles * splits > pairs || m.col_blocks < 4 * splits)) break;
-            const long long reduce = splits > 1 ? barrier + 1500 + 400 * splits * ((tiles * (wide ? 64 : 32) + pairs * 16 - 1) / (pairs * 16)) : 0;
+            const long long reduce = splits > 1 ? 22000 + 400 * splits * ((tiles * (wide ? 64 : 32) + pairs * 16 - 1) / (pairs * 16)) : 0;
             const long long t = product_cycles(tiles * splits, wide, m.col_blocks / splits, pairs) + reduce;
             if (best < 0 || t < best) best = t, m.gram_wide = wide, m.splits = splits;
         }
@@ -1052,9 +1081,9 @@ void fill(const gmc_matrix* matrices, const int* which, int n, int pairs, bool f
         m.row_tiles = ceil_div(wide_rows, 128);
         m.col_blocks = 2 * ceil_div(wide_cols, 128);
         // fp32 results: against the plain fp32 evaluation's error, 256 x 4000 has 1.2 times with two stages and 2.3 with four,
-        // from 700 x 2000 on four have 0.9 and less and save 10 % of the time (2048 x 2048); 16-bit results: the whole axis,
-        // 5e-5 of the result at 2048 against half a step of 2^-9 or 2^-12
-        m.chunk = !fp32 ? 1 << 20 : wide_rows <= 512 ? 2 : 4;
+        // 700 x 2000 0.9 with four and 1.6 with eight, 2048 x 2048 0.7 with eight and the time is 810, 720 and 680 us; 16-bit
+        // results: the whole axis, 5e-5 of the result at 2048 against half a step of 2^-9 or 2^-12
+        m.chunk = !fp32 ? 1 << 20 : wide_rows <= 512 ? 2 : wide_rows <= 1024 ? 4 : 8;
         m.norm_first = b.norm_ctas;
         m.block_first = b.blocks;
         m.x_block = x_blocks;
