@@ -17,6 +17,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -721,7 +722,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_co
 // the update's elements and the result, there is one launch instead of three per step, and the products are fp32.
 constexpr int kShortThreads = 512;
 constexpr int kShortWarps = kShortThreads / 32;
-constexpr int kShortRows = 64;
+constexpr int kShortRows = 16;
 struct ShortBatch {
     Matrix m[kMaxMatrices];
 };
@@ -1018,6 +1019,306 @@ __global__ void __launch_bounds__(kShortThreads, 1) short_kernel(const __grid_co
     else short_matrix<T, MUON, 64>(m, ranks, rank, mo, steps, ca, cb, cc, epsilon, smem, warp_sum, &cta_sum);
 }
 
+// ---- matrices with a side of 17 to 128: the whole chain in one launch, on the tensor cores ---------------------------
+// One cluster per matrix; each CTA keeps X for its share of the columns in shared memory, as the chain's planes (blocks of MP
+// rows x 64 columns). Per step: X X^T of the CTA's columns; the shares are added up over distributed shared memory, CTA q
+// summing rows q MP / ranks .. and handing them to all as planes; B = b A + c A A in A's place, each CTA for itself;
+// X <- a X + B X in place. All accumulators are in tensor memory; additions per accumulator are few (128 in K), so that the
+// losses of the module comment stay small. What bounds it is the chain of latencies, about eight barriers a step.
+constexpr int kMidThreads = 512;
+constexpr int kMidWarps = kMidThreads / 32;
+__host__ __device__ constexpr int mid_rows(int rows) { return rows <= 64 ? 64 : 128; }
+__host__ __device__ constexpr int mid_max_blocks(int mp) { return mp == 64 ? 8 : 3; }                    // of 64 columns per CTA
+__host__ __device__ constexpr int mid_block_bytes(int mp) { return mp * 64 * 4; }
+__host__ __device__ constexpr int mid_blocks(int cols, int ranks) { return ((cols + ranks - 1) / ranks + 63) / 64; }
+__host__ __device__ constexpr int mid_smem(int mp, int blocks) { return blocks * mid_block_bytes(mp) + 2 * mp * mp * 4 + 1024; }
+
+template <typename T, bool MUON, int MP>
+__device__ __forceinline__ void mid_matrix(const Matrix& m, int ranks, int rank, const Momentum& mo, int steps, const Polynomial& poly, float epsilon,
+                                           uint8_t* smem, uint32_t tmem, uint64_t* bar, double* warp_sum, double* cta_sum) {
+    constexpr int kBlock = mid_block_bytes(MP), kMaxUnits = MP * mid_max_blocks(MP) * 8 / kMidThreads;
+    constexpr int kPerSum = MP == 64 ? 2 : 1;                         // blocks of X X^T per accumulator
+    constexpr uint32_t kMixedGram = 512 - MP;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const bool tall = m.rows > m.cols;
+    const int wide_rows = tall ? m.cols : m.rows, wide_cols = tall ? m.rows : m.cols;
+    const int blocks = mid_blocks(wide_cols, ranks), col0 = rank * blocks * 64;
+    uint8_t* x = smem;
+    uint8_t* gram = x + blocks * kBlock;                              // A's planes, then B's
+    float* share = reinterpret_cast<float*>(gram + MP * MP * 4);      // the CTA's part of A; float4 c of row r at c ^ (r & 7)
+    bool ok = true;
+    unsigned phase = 0;
+    auto wait_mma = [&]() {
+        ok = warp_wait(bar, phase) && ok;
+        phase ^= 1;
+        tmem_fence_after();
+    };
+
+    // the update: units of eight columns of a row, neighbouring threads along the rows of the update
+    float u[kMaxUnits][8];
+    double s = 0.;
+    const int units = MP * blocks * 8;
+#pragma unroll
+    for (int i = 0; i < kMaxUnits; ++i) {
+        const int unit = tid + i * kMidThreads, row = tall ? unit & (MP - 1) : unit / (blocks * 8), chunk = tall ? unit / MP : unit % (blocks * 8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int c = col0 + chunk * 8 + e;
+            u[i][e] = 0.f;
+            if (unit < units && row < wide_rows && c < wide_cols) {
+                const long long rr = tall ? c : row, cc = tall ? row : c;
+                float v = load_float<T>(m.update, rr * m.update_stride + cc);
+                if constexpr (MUON) {
+                    float* at = m.momentum + rr * m.cols + cc;
+                    const float now = mo.beta * *at + mo.one_minus_beta * v;
+                    *at = now;
+                    v = mo.nesterov ? mo.one_minus_beta * v + mo.beta * now : now;
+                }
+                u[i][e] = v;
+                s += double(v) * double(v);
+            }
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) warp_sum[warp] = s;
+    __syncthreads();
+    s = lane < kMidWarps ? warp_sum[lane] : 0.;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    s = __shfl_sync(0xffffffffu, s, 0);
+    if (ranks > 1) {
+        if (tid == 0) *cta_sum = s;
+        cluster.sync();
+        s = lane < ranks ? *cluster.map_shared_rank(cta_sum, lane) : 0.;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        s = __shfl_sync(0xffffffffu, s, 0);
+    }
+    const float factor = float(double(kScaleX) / (sqrt(s) + double(epsilon)));
+    const uint4 none = {};
+#pragma unroll
+    for (int i = 0; i < kMaxUnits; ++i) {
+        const int unit = tid + i * kMidThreads, row = tall ? unit & (MP - 1) : unit / (blocks * 8), chunk = tall ? unit / MP : unit % (blocks * 8);
+        if (unit < units) {
+            uint4 hi, lo;
+            split8<false>(u[i], factor, 0.f, none, none, hi, lo);
+            uint8_t* at = x + (chunk >> 3) * kBlock + swizzled_offset(row, chunk & 7);
+            *reinterpret_cast<uint4*>(at) = hi;
+            *reinterpret_cast<uint4*>(at + kPlaneOffset) = lo;
+        }
+    }
+    fence_proxy_async();
+    __syncthreads();
+
+    const int quarter = warp & 3, part = warp >> 2, row = quarter * 32 + lane;         // rows of the warp, share of the columns
+    const bool rows_here = quarter * 32 < MP;
+    const uint32_t lanes = uint32_t(quarter * 32) << 16;
+    constexpr uint64_t lo_plane = kPlaneOffset >> 4;
+    const uint32_t x_at = smem_u32(x), gram_at = smem_u32(gram);
+    const int last = min(blocks * 64, wide_cols - col0);              // columns of this CTA that hold something
+    for (int step = 0; step < steps; ++step) {
+        const int sums = (blocks + kPerSum - 1) / kPerSum;
+        if (tid == 0) {
+            tmem_fence_after();
+            constexpr uint32_t instruction = f16_instruction(128, MP, false, false);
+            for (int k = 0; k * 16 < last || k == 0; ++k) {
+                const uint64_t a = k_major_descriptor(x_at + (k >> 2) * kBlock + (k & 3) * kMajorStep);
+                mma_f16_single(tmem + kMixedGram, a, a + lo_plane, instruction, k > 0);
+                mma_f16_single(tmem + kMixedGram, a + lo_plane, a, instruction, true);
+                mma_f16_single(tmem + (k / (4 * kPerSum)) * MP, a, a, instruction, k % (4 * kPerSum) > 0);
+            }
+            mma_commit_single(bar);
+        }
+        wait_mma();
+        if (rows_here) {
+#pragma unroll 1
+            for (int q = part * 32; q < MP; q += (kMidWarps / 4) * 32) {
+                float v[32], add[32];
+                tmem_load32(tmem + lanes + kMixedGram + q, v);
+                for (int i = 0; i < sums; ++i) {
+                    if (i * kPerSum * 64 >= last && i > 0) break;     // no columns, no sums
+                    tmem_load32(tmem + lanes + i * MP + q, add);
+                    const float loss = 0x1p-25f * 4.f * float(min(kPerSum, blocks - i * kPerSum));
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) v[e] += add[e] * (q + e == row ? 1.f + 2.f * loss : 1.f + 0.7f * loss);
+                }
+                float4* to = reinterpret_cast<float4*>(share) + row * (MP / 4);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    to[(q / 4 + e) ^ (row & 7)] = make_float4(v[4 * e] * poly.gram_factor, v[4 * e + 1] * poly.gram_factor, v[4 * e + 2] * poly.gram_factor,
+                                                              v[4 * e + 3] * poly.gram_factor);
+            }
+        }
+        tmem_fence_before();
+        if (ranks > 1) cluster.sync();
+        else __syncthreads();
+        {
+            const int each = MP / ranks;                              // rows that this CTA sums
+            for (int i = tid; i < each * (MP / 8); i += kMidThreads) {
+                const int r = rank * each + i / (MP / 8), chunk = i % (MP / 8);
+                float v[8] = {};
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    if (q < ranks) {
+                        const float4* from = reinterpret_cast<const float4*>(ranks > 1 ? cluster.map_shared_rank(share, q) : share) + r * (MP / 4);
+                        const float4 a = from[(2 * chunk) ^ (r & 7)], b = from[(2 * chunk + 1) ^ (r & 7)];
+                        v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
+                    }
+                }
+                uint4 hi, lo;
+                split8<false>(v, 1.f, 0.f, none, none, hi, lo);
+                const uint32_t at = (chunk >> 3) * kBlock + swizzled_offset(r, chunk & 7);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    if (q < ranks) {
+                        uint8_t* to = (ranks > 1 ? cluster.map_shared_rank(gram, q) : gram) + at;
+                        *reinterpret_cast<uint4*>(to) = hi;
+                        *reinterpret_cast<uint4*>(to + kPlaneOffset) = lo;
+                    }
+                }
+            }
+        }
+        fence_proxy_async_all();
+        if (ranks > 1) cluster.sync();
+        else __syncthreads();
+        if (!poly.linear) {
+            if (tid == 0) {
+                fence_proxy_async_all();
+                tmem_fence_after();
+                constexpr uint32_t instruction = f16_instruction(128, MP, false, false);
+#pragma unroll
+                for (int k = 0; k < MP / 16; ++k) {
+                    const uint64_t a = k_major_descriptor(gram_at + (k >> 2) * kBlock + (k & 3) * kMajorStep);
+                    mma_f16_single(tmem + MP, a, a + lo_plane, instruction, k > 0);
+                    mma_f16_single(tmem + MP, a + lo_plane, a, instruction, true);
+                    mma_f16_single(tmem, a, a, instruction, k > 0);
+                }
+                mma_commit_single(bar);
+            }
+            wait_mma();
+            if (rows_here) {
+                constexpr float loss = 0x1p-25f * float(MP / 16);
+#pragma unroll 1
+                for (int q = part * 32; q < MP; q += (kMidWarps / 4) * 32) {
+                    float v[32], add[32];
+                    tmem_load32(tmem + lanes + MP + q, v);
+                    tmem_load32(tmem + lanes + q, add);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) v[e] += add[e] * (q + e == row ? 1.f + 2.4f * loss : 1.f + 0.7f * loss);
+                    uint8_t* block = gram + (q >> 6) * kBlock;
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        uint8_t* at = block + swizzled_offset(row, ((q & 63) >> 3) + g);
+                        const uint4 in_hi = *reinterpret_cast<const uint4*>(at), in_lo = *reinterpret_cast<const uint4*>(at + kPlaneOffset);
+                        uint4 hi, lo;
+                        split8<true>(v + g * 8, poly.poly_factor, poly.poly_from, in_hi, in_lo, hi, lo);
+                        *reinterpret_cast<uint4*>(at) = hi;
+                        *reinterpret_cast<uint4*>(at + kPlaneOffset) = lo;
+                    }
+                }
+            }
+            fence_proxy_async();
+            tmem_fence_before();
+            __syncthreads();
+        }
+        // 256 columns at a time: 256 of tensor memory for each of the two sums
+        for (int c0 = 0; c0 < last; c0 += 256) {
+            const int n = min(256, (last - c0 + 15) & ~15);
+            if (tid == 0) {
+                fence_proxy_async_all();
+                tmem_fence_after();
+                const uint32_t instruction = f16_instruction(128, n, false, true);
+#pragma unroll
+                for (int k = 0; k < MP / 16; ++k) {
+                    const uint64_t a = k_major_descriptor(gram_at + (k >> 2) * kBlock + (k & 3) * kMajorStep);
+                    const uint64_t b = mn_major_descriptor(x_at + (c0 >> 6) * kBlock + k * mnMajorStep, kBlock);
+                    mma_f16_single(tmem + 256, a, b + lo_plane, instruction, k > 0);
+                    mma_f16_single(tmem + 256, a + lo_plane, b, instruction, true);
+                    mma_f16_single(tmem, a, b, instruction, k > 0);
+                }
+                mma_commit_single(bar);
+            }
+            wait_mma();
+            if (rows_here) {
+                constexpr float made_good = 1.f + 0.7f * 0x1p-25f * float(MP / 16);
+#pragma unroll 1
+                for (int q = part * 32; q < n; q += (kMidWarps / 4) * 32) {
+                    float v[32], add[32];
+                    tmem_load32(tmem + lanes + 256 + q, v);
+                    tmem_load32(tmem + lanes + q, add);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) v[e] += add[e] * made_good;
+                    uint8_t* block = x + ((c0 + q) >> 6) * kBlock;
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        // beyond n the sums are not this product's; nothing is stored there but zeros
+                        if (q + g * 8 < n) {
+                            uint8_t* at = block + swizzled_offset(row, ((q & 63) >> 3) + g);
+                            const uint4 in_hi = *reinterpret_cast<const uint4*>(at), in_lo = *reinterpret_cast<const uint4*>(at + kPlaneOffset);
+                            uint4 hi, lo;
+                            split8<true>(v + g * 8, poly.step_factor, poly.step_from, in_hi, in_lo, hi, lo);
+                            *reinterpret_cast<uint4*>(at) = hi;
+                            *reinterpret_cast<uint4*>(at + kPlaneOffset) = lo;
+                        }
+                    }
+                }
+            }
+            fence_proxy_async();
+            tmem_fence_before();
+            __syncthreads();
+        }
+    }
+    if (!ok) report_check(CHECK_MBARRIER_TIMEOUT);
+    T* out = static_cast<T*>(m.out);
+#pragma unroll 1
+    for (int unit = tid; unit < units; unit += kMidThreads) {
+        const int r = tall ? unit & (MP - 1) : unit / (blocks * 8), chunk = tall ? unit / MP : unit % (blocks * 8);
+        if (r >= wide_rows) continue;
+        const uint8_t* at = x + (chunk >> 3) * kBlock + swizzled_offset(r, chunk & 7);
+        Chunk hi, lo;
+        hi.raw = *reinterpret_cast<const uint4*>(at);
+        lo.raw = *reinterpret_cast<const uint4*>(at + kPlaneOffset);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int c = col0 + chunk * 8 + e;
+            if (c < wide_cols) {
+                const long long o = tall ? c * m.out_stride + r : r * m.out_stride + c;
+                float v = (__half2float(hi.h[e]) + __half2float(lo.h[e])) * (1.f / kScaleX);
+                if (!ok) v = __int_as_float(0x7fffffff);
+                out[o] = T(MUON ? float(out[o]) * mo.decay - m.rate * v : v);
+            }
+        }
+    }
+    if (ranks > 1) cluster.sync();                                    // no CTA leaves while its shared memory is read or written
+}
+
+template <typename T, bool MUON>
+__global__ void __launch_bounds__(kMidThreads, 1) mid_kernel(const __grid_constant__ ShortBatch b, int ranks, Momentum mo, int steps, Polynomial poly,
+                                                             float epsilon) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ double warp_sum[kMidWarps], cta_sum;
+    __shared__ uint64_t bar;
+    __shared__ uint32_t tmem_address;
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const Matrix& m = b.m[blockIdx.x / unsigned(ranks)];
+    const int rank = int(blockIdx.x % unsigned(ranks));
+    if (threadIdx.x == 0) {
+        mbar_init(&bar, 1);
+        fence_mbar_init();
+    }
+    if (threadIdx.x < 32) tmem_alloc_single(&tmem_address, 512);
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = tmem_address;
+    if (min(m.rows, m.cols) <= 64) mid_matrix<T, MUON, 64>(m, ranks, rank, mo, steps, poly, epsilon, smem, tmem, &bar, warp_sum, &cta_sum);
+    else mid_matrix<T, MUON, 128>(m, ranks, rank, mo, steps, poly, epsilon, smem, tmem, &bar, warp_sum, &cta_sum);
+    __syncthreads();
+    if (threadIdx.x < 32) tmem_free_single(tmem, 512);
+}
+
 // ---- host side -------------------------------------------------------------------------------------------------------
 int ceil_div(long long a, long long b) { return int((a + b - 1) / b); }
 
@@ -1059,6 +1360,8 @@ long long most_units(const Matrix& m) {
     return gram > step ? gram : step;
 }
 
+void describe(const gmc_matrix& g, Matrix& m);
+
 // Lays out the workspace and hands out `pairs` CTA pairs: one each, the others to whoever takes longest.
 void fill(const gmc_matrix* matrices, const int* which, int n, int pairs, bool fp32, Batch* batch, size_t* bytes, uint8_t* workspace) {
     Batch& b = *batch;
@@ -1070,14 +1373,7 @@ void fill(const gmc_matrix* matrices, const int* which, int n, int pairs, bool f
         const gmc_matrix& g = matrices[which[i]];
         Matrix& m = b.m[i];
         const long long wide_rows = g.rows < g.cols ? g.rows : g.cols, wide_cols = g.rows < g.cols ? g.cols : g.rows;
-        m.update = g.update;
-        m.momentum = g.momentum;
-        m.out = g.out;
-        m.update_stride = g.update_stride;
-        m.out_stride = g.out_stride;
-        m.rows = int(g.rows);
-        m.cols = int(g.cols);
-        m.rate = g.rate;
+        describe(g, m);
         m.row_tiles = ceil_div(wide_rows, 128);
         m.col_blocks = 2 * ceil_div(wide_cols, 128);
         // fp32 results: against the plain fp32 evaluation's error, 256 x 4000 has 1.2 times with two stages and 2.3 with four,
@@ -1230,11 +1526,62 @@ int run_batch(const Batch& b, int steps, const Polynomial& poly, float epsilon, 
     return GMC_OK;
 }
 
-// A matrix goes to the one-launch kernel if its short side fits the tile grid and X fits the shared memory of eight CTAs.
+// Which kernel a matrix goes to, by its shape.
 constexpr size_t kShortSmemLimit = 220 * 1024;
-bool is_short(const gmc_matrix& g) {
+constexpr int kMidSmemLimit = 227 * 1024 - 512;
+enum Kind { SHORT, MID, CHAIN, KINDS };
+Kind kind_of(const gmc_matrix& g) {
     const long long rows = g.rows < g.cols ? g.rows : g.cols, cols = g.rows < g.cols ? g.cols : g.rows;
-    return rows <= kShortRows && short_smem(int(rows), int(cols), 8) <= kShortSmemLimit;
+    if (rows <= kShortRows && short_smem(int(rows), int(cols), 8) <= kShortSmemLimit) return SHORT;
+    if (rows <= 128 && mid_blocks(int(cols), 8) <= mid_max_blocks(mid_rows(int(rows)))) return MID;
+    return CHAIN;
+}
+void describe(const gmc_matrix& g, Matrix& m) {
+    m.update = g.update;
+    m.momentum = g.momentum;
+    m.out = g.out;
+    m.update_stride = g.update_stride;
+    m.out_stride = g.out_stride;
+    m.rows = int(g.rows);
+    m.cols = int(g.cols);
+    m.rate = g.rate;
+}
+
+// One launch of clusters of `ranks` CTAs, one per matrix.
+template <typename Kernel, typename... Args>
+int launch_clusters(Kernel kernel, int n, int ranks, int threads, size_t smem, size_t smem_limit, cudaStream_t stream, const Args&... args) {
+    GMC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem_limit)));
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(unsigned(n * ranks));
+    config.blockDim = dim3(unsigned(threads));
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attribute;
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = unsigned(ranks);
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    GMC_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, args...));
+    return GMC_OK;
+}
+
+template <typename T, bool MUON>
+int run_mid(const gmc_matrix* matrices, const int* which, int n, int steps, const Polynomial& poly, float epsilon, const Momentum& mo,
+            cudaStream_t stream) {
+    ShortBatch b;
+    int ranks = 1, smem = 0;
+    for (int i = 0; i < n; ++i) {
+        describe(matrices[which[i]], b.m[i]);
+        const int rows = std::min(b.m[i].rows, b.m[i].cols), cols = std::max(b.m[i].rows, b.m[i].cols);
+        // up to 256 columns a CTA: below, the exchange of the shares costs more than the products save
+        while (ranks < 8 && (mid_blocks(cols, ranks) > mid_max_blocks(mid_rows(rows)) || cols > 256 * ranks)) ranks *= 2;
+    }
+    for (int i = 0; i < n; ++i) {
+        const int rows = std::min(b.m[i].rows, b.m[i].cols), cols = std::max(b.m[i].rows, b.m[i].cols);
+        smem = std::max(smem, mid_smem(mid_rows(rows), mid_blocks(cols, ranks)));
+    }
+    return launch_clusters(mid_kernel<T, MUON>, n, ranks, kMidThreads, smem, kMidSmemLimit, stream, b, ranks, mo, steps, poly, epsilon);
 }
 
 template <typename T, bool MUON>
@@ -1246,16 +1593,8 @@ int run_short(const gmc_matrix* matrices, const int* which, int n, int steps, fl
     GMC_CUDA_TRY(cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, device));
     size_t smem = 0;
     for (int i = 0; i < n; ++i) {
-        const gmc_matrix& g = matrices[which[i]];
-        Matrix& m = b.m[i];
-        m.update = g.update;
-        m.momentum = g.momentum;
-        m.out = g.out;
-        m.update_stride = g.update_stride;
-        m.out_stride = g.out_stride;
-        m.rows = int(g.rows);
-        m.cols = int(g.cols);
-        m.rate = g.rate;
+        describe(matrices[which[i]], b.m[i]);
+        const Matrix& m = b.m[i];
         const int rows = m.rows < m.cols ? m.rows : m.cols, cols = m.rows < m.cols ? m.cols : m.rows;
         while (ranks < 8 && ((cols / ranks > 40 && 2 * ranks * n <= n_sm) || short_smem(rows, cols, ranks) > kShortSmemLimit)) ranks *= 2;
     }
@@ -1264,32 +1603,21 @@ int run_short(const gmc_matrix* matrices, const int* which, int n, int steps, fl
         const size_t need = short_smem(rows, cols, ranks);
         smem = need > smem ? need : smem;
     }
-    GMC_CUDA_TRY(cudaFuncSetAttribute(short_kernel<T, MUON>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kShortSmemLimit)));
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(unsigned(n * ranks));
-    config.blockDim = dim3(kShortThreads);
-    config.dynamicSmemBytes = smem;
-    config.stream = stream;
-    cudaLaunchAttribute attribute;
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = unsigned(ranks);
-    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-    config.attrs = &attribute;
-    config.numAttrs = 1;
-    GMC_CUDA_TRY(cudaLaunchKernelEx(&config, short_kernel<T, MUON>, b, ranks, mo, steps, ca, cb, cc, epsilon));
-    return GMC_OK;
+    return launch_clusters(short_kernel<T, MUON>, n, ranks, kShortThreads, smem, kShortSmemLimit, stream, b, ranks, mo, steps, ca, cb, cc, epsilon);
 }
 
 template <typename T, bool MUON>
 int run_typed(const gmc_matrix* matrices, int n, int steps, float ca, float cb, float cc, const Polynomial& poly, float epsilon, const Momentum& mo,
               void* workspace, size_t workspace_bytes, cudaStream_t stream) {
     int which[kMaxMatrices], count = 0;
-    for (int pass = 0; pass < 2; ++pass) {
+    for (int kind = 0; kind < KINDS; ++kind) {
         for (int i = 0; i <= n; ++i) {
-            if (i < n && is_short(matrices[i]) == (pass == 0)) which[count++] = i;
+            if (i < n && kind_of(matrices[i]) == kind) which[count++] = i;
             if (count == kMaxMatrices || (i == n && count > 0)) {
-                if (pass == 0) {
+                if (kind == SHORT) {
                     if (int s = run_short<T, MUON>(matrices, which, count, steps, ca, cb, cc, epsilon, mo, stream)) return s;
+                } else if (kind == MID) {
+                    if (int s = run_mid<T, MUON>(matrices, which, count, steps, poly, epsilon, mo, stream)) return s;
                 } else {
                     Batch b;
                     size_t bytes = 0;
@@ -1310,7 +1638,7 @@ size_t workspace_bytes_of(const gmc_matrix* matrices, int n) {
     int which[kMaxMatrices], count = 0;
     size_t most = 0;
     for (int i = 0; i <= n; ++i) {
-        if (i < n && !is_short(matrices[i])) which[count++] = i;
+        if (i < n && kind_of(matrices[i]) == CHAIN) which[count++] = i;
         if (count == kMaxMatrices || (i == n && count > 0)) {
             Batch b;
             size_t bytes = 0;
