@@ -308,6 +308,39 @@ __device__ __forceinline__ bool wait_counter(const unsigned* counter, unsigned v
 __device__ __forceinline__ void fence_proxy_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
 __device__ __forceinline__ void writers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWriters) : "memory"); }
 
+// Eight neighbouring elements, with vector accesses where `aligned` says that their address allows them.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, bool aligned, float (&v)[8]) {
+    if (aligned) {
+        constexpr int N = 16 / int(sizeof(T));
+        union { uint4 raw[8 / N]; T e[8]; } u;
+#pragma unroll
+        for (int i = 0; i < 8 / N; ++i) u.raw[i] = reinterpret_cast<const uint4*>(p)[i];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = float(u.e[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = float(p[e]);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, bool aligned, const float (&v)[8]) {
+    if (aligned) {
+        constexpr int N = 16 / int(sizeof(T));
+        union { uint4 raw[8 / N]; T e[8]; } u;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u.e[e] = T(v[e]);
+#pragma unroll
+        for (int i = 0; i < 8 / N; ++i) reinterpret_cast<uint4*>(p)[i] = u.raw[i];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = T(v[e]);
+    }
+}
+__device__ __forceinline__ bool rows_aligned(const void* p, long long stride, int size) {
+    return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t(stride) * size)) & 15u) == 0;
+}
+
 // Eight columns: v c1, plus c0 (in_hi + in_lo), as planes.
 template <bool ADD>
 __device__ __forceinline__ void split8(const float* v, float c1, float c0, const uint4& in_hi, const uint4& in_lo, uint4& hi, uint4& lo) {
@@ -718,12 +751,12 @@ __global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_co
 // ---- matrices with a short side: the whole chain in one launch, fp32 -------------------------------------------------
 // One cluster per matrix. Each CTA keeps X for its share of the columns in shared memory over all steps; per step every CTA
 // adds up all shares of X X^T over distributed shared memory, forms P = a I + b A + c A A for itself and multiplies its own
-// columns with it in place. Nothing goes through global memory between
-// the update's elements and the result, there is one launch instead of three per step, and the products are fp32.
+// columns with it in place. Nothing goes through global memory between the update's elements and the result, and the products
+// are fp32. Up to 16 rows; above, the shared memory's bandwidth binds (64 x 160: 49 us) and the tensor cores are faster.
 constexpr int kShortThreads = 512;
 constexpr int kShortWarps = kShortThreads / 32;
 constexpr int kShortRows = 16;
-struct ShortBatch {
+struct ClusterBatch {
     Matrix m[kMaxMatrices];
 };
 // Sizes for X padded to MP rows: 4 x 4 tiles on and below the diagonal of X X^T, and groups of threads that share its sums.
@@ -1006,19 +1039,6 @@ __device__ __forceinline__ void short_matrix(const Matrix& m, int ranks, int ran
     if (ranks > 1) cluster.sync();                                    // no CTA leaves while its shared memory is read
 }
 
-template <typename T, bool MUON>
-__global__ void __launch_bounds__(kShortThreads, 1) short_kernel(const __grid_constant__ ShortBatch b, int ranks, Momentum mo, int steps, float ca,
-                                                                 float cb, float cc, float epsilon) {
-    extern __shared__ __align__(16) float smem[];
-    __shared__ double warp_sum[kShortWarps], cta_sum;
-    const Matrix& m = b.m[blockIdx.x / unsigned(ranks)];
-    const int rank = int(blockIdx.x % unsigned(ranks)), rows = min(m.rows, m.cols);
-    if (rows <= 8) short_matrix<T, MUON, 8>(m, ranks, rank, mo, steps, ca, cb, cc, epsilon, smem, warp_sum, &cta_sum);
-    else if (rows <= 16) short_matrix<T, MUON, 16>(m, ranks, rank, mo, steps, ca, cb, cc, epsilon, smem, warp_sum, &cta_sum);
-    else if (rows <= 32) short_matrix<T, MUON, 32>(m, ranks, rank, mo, steps, ca, cb, cc, epsilon, smem, warp_sum, &cta_sum);
-    else short_matrix<T, MUON, 64>(m, ranks, rank, mo, steps, ca, cb, cc, epsilon, smem, warp_sum, &cta_sum);
-}
-
 // ---- matrices with a side of 17 to 128: the whole chain in one launch, on the tensor cores ---------------------------
 // One cluster per matrix; each CTA keeps X for its share of the columns in shared memory, as the chain's planes (blocks of MP
 // rows x 64 columns). Per step: X X^T of the CTA's columns; the shares are added up over distributed shared memory, CTA q
@@ -1058,28 +1078,54 @@ __device__ __forceinline__ void mid_matrix(const Matrix& m, int ranks, int rank,
     // the update: units of eight columns of a row, neighbouring threads along the rows of the update
     float u[kMaxUnits][8];
     double s = 0.;
-    const int units = MP * blocks * 8;
+    const int units = MP * blocks * 8, row_units = blocks * 8;
+    const unsigned reciprocal = 0xffffffffu / unsigned(row_units) + 1u;                // exact quotients of numbers below 4096
+    const T* update = static_cast<const T*>(m.update);
+    const bool vectors = !tall && rows_aligned(update, m.update_stride, sizeof(T)), momentum_vectors = !tall && rows_aligned(m.momentum, m.cols, 4);
+    auto place = [&](int unit, int& row, int& col) {                                   // in the wide form
+        row = tall ? unit & (MP - 1) : int(__umulhi(unsigned(unit), reciprocal));
+        col = col0 + (tall ? unit / MP : unit - row * row_units) * 8;
+    };
 #pragma unroll
     for (int i = 0; i < kMaxUnits; ++i) {
-        const int unit = tid + i * kMidThreads, row = tall ? unit & (MP - 1) : unit / (blocks * 8), chunk = tall ? unit / MP : unit % (blocks * 8);
+        int row, col;
+        place(tid + i * kMidThreads, row, col);
+        const bool in = tid + i * kMidThreads < units && row < wide_rows;
+        float old[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int c = col0 + chunk * 8 + e;
-            u[i][e] = 0.f;
-            if (unit < units && row < wide_rows && c < wide_cols) {
-                const long long rr = tall ? c : row, cc = tall ? row : c;
-                float v = load_float<T>(m.update, rr * m.update_stride + cc);
-                if constexpr (MUON) {
-                    float* at = m.momentum + rr * m.cols + cc;
-                    const float now = mo.beta * *at + mo.one_minus_beta * v;
-                    *at = now;
-                    v = mo.nesterov ? mo.one_minus_beta * v + mo.beta * now : now;
+        for (int e = 0; e < 8; ++e) u[i][e] = old[e] = 0.f;
+        if (in && !tall && col + 8 <= wide_cols) {
+            load8(update + row * m.update_stride + col, vectors, u[i]);
+            if constexpr (MUON) load8(m.momentum + (long long)row * m.cols + col, momentum_vectors, old);
+        } else if (in) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (col + e < wide_cols) {
+                    const long long rr = tall ? col + e : row, cc = tall ? row : col + e;
+                    u[i][e] = float(update[rr * m.update_stride + cc]);
+                    if constexpr (MUON) old[e] = m.momentum[rr * m.cols + cc];
                 }
-                u[i][e] = v;
-                s += double(v) * double(v);
+            }
+        }
+        if constexpr (MUON) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                old[e] = mo.beta * old[e] + mo.one_minus_beta * u[i][e];
+                u[i][e] = mo.nesterov ? mo.one_minus_beta * u[i][e] + mo.beta * old[e] : old[e];
+            }
+            if (in && !tall && col + 8 <= wide_cols) {
+                store8(m.momentum + (long long)row * m.cols + col, momentum_vectors, old);
+            } else if (in) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (col + e < wide_cols) m.momentum[tall ? (long long)(col + e) * m.cols + row : (long long)row * m.cols + col + e] = old[e];
             }
         }
     }
+#pragma unroll
+    for (int i = 0; i < kMaxUnits; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += double(u[i][e]) * double(u[i][e]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (lane == 0) warp_sum[warp] = s;
@@ -1100,8 +1146,10 @@ __device__ __forceinline__ void mid_matrix(const Matrix& m, int ranks, int rank,
     const uint4 none = {};
 #pragma unroll
     for (int i = 0; i < kMaxUnits; ++i) {
-        const int unit = tid + i * kMidThreads, row = tall ? unit & (MP - 1) : unit / (blocks * 8), chunk = tall ? unit / MP : unit % (blocks * 8);
-        if (unit < units) {
+        int row, col;
+        place(tid + i * kMidThreads, row, col);
+        if (tid + i * kMidThreads < units) {
+            const int chunk = (col - col0) >> 3;
             uint4 hi, lo;
             split8<false>(u[i], factor, 0.f, none, none, hi, lo);
             uint8_t* at = x + (chunk >> 3) * kBlock + swizzled_offset(row, chunk & 7);
@@ -1118,16 +1166,26 @@ __device__ __forceinline__ void mid_matrix(const Matrix& m, int ranks, int rank,
     constexpr uint64_t lo_plane = kPlaneOffset >> 4;
     const uint32_t x_at = smem_u32(x), gram_at = smem_u32(gram);
     const int last = min(blocks * 64, wide_cols - col0);              // columns of this CTA that hold something
+    // two threads issue: the mixed products and hi hi (80 cycles for each MMA that a thread issues)
+    const bool issues_mixed = tid == 0, issues_main = tid == 32;
     for (int step = 0; step < steps; ++step) {
         const int sums = (blocks + kPerSum - 1) / kPerSum;
-        if (tid == 0) {
+        if (issues_mixed || issues_main) {
             tmem_fence_after();
             constexpr uint32_t instruction = f16_instruction(128, MP, false, false);
+            uint64_t a = k_major_descriptor(x_at);
+            uint32_t sum = tmem;
+            bool more = false;                                        // the accumulator holds something already
             for (int k = 0; k * 16 < last || k == 0; ++k) {
-                const uint64_t a = k_major_descriptor(x_at + (k >> 2) * kBlock + (k & 3) * kMajorStep);
-                mma_f16_single(tmem + kMixedGram, a, a + lo_plane, instruction, k > 0);
-                mma_f16_single(tmem + kMixedGram, a + lo_plane, a, instruction, true);
-                mma_f16_single(tmem + (k / (4 * kPerSum)) * MP, a, a, instruction, k % (4 * kPerSum) > 0);
+                if (issues_mixed) {
+                    mma_f16_single(tmem + kMixedGram, a, a + lo_plane, instruction, k > 0);
+                    mma_f16_single(tmem + kMixedGram, a + lo_plane, a, instruction, true);
+                } else {
+                    mma_f16_single(sum, a, a, instruction, more);
+                }
+                a += (k & 3) == 3 ? (kBlock - 3 * kMajorStep) >> 4 : kMajorStep >> 4;
+                more = (k + 1) % (4 * kPerSum) != 0;
+                if (!more) sum += MP;
             }
             mma_commit_single(bar);
         }
@@ -1136,64 +1194,84 @@ __device__ __forceinline__ void mid_matrix(const Matrix& m, int ranks, int rank,
 #pragma unroll 1
             for (int q = part * 32; q < MP; q += (kMidWarps / 4) * 32) {
                 float v[32], add[32];
-                tmem_load32(tmem + lanes + kMixedGram + q, v);
-                for (int i = 0; i < sums; ++i) {
-                    if (i * kPerSum * 64 >= last && i > 0) break;     // no columns, no sums
-                    tmem_load32(tmem + lanes + i * MP + q, add);
+                tmem_load32(tmem + lanes + kMixedGram + q, v, tmem + lanes + q, add);
+                for (int i = 0;;) {
                     const float loss = 0x1p-25f * 4.f * float(min(kPerSum, blocks - i * kPerSum));
 #pragma unroll
                     for (int e = 0; e < 32; ++e) v[e] += add[e] * (q + e == row ? 1.f + 2.f * loss : 1.f + 0.7f * loss);
+                    if (++i >= sums || i * kPerSum * 64 >= last) break;                // no columns, no sums
+                    tmem_load32(tmem + lanes + i * MP + q, add);
                 }
-                float4* to = reinterpret_cast<float4*>(share) + row * (MP / 4);
+                if (ranks > 1) {
+                    float4* to = reinterpret_cast<float4*>(share) + row * (MP / 4);
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    to[(q / 4 + e) ^ (row & 7)] = make_float4(v[4 * e] * poly.gram_factor, v[4 * e + 1] * poly.gram_factor, v[4 * e + 2] * poly.gram_factor,
-                                                              v[4 * e + 3] * poly.gram_factor);
+                    for (int e = 0; e < 8; ++e)
+                        to[(q / 4 + e) ^ (row & 7)] = make_float4(v[4 * e] * poly.gram_factor, v[4 * e + 1] * poly.gram_factor,
+                                                                  v[4 * e + 2] * poly.gram_factor, v[4 * e + 3] * poly.gram_factor);
+                } else {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        uint4 hi, lo;
+                        split8<false>(v + g * 8, poly.gram_factor, 0.f, none, none, hi, lo);
+                        uint8_t* at = gram + (q >> 6) * kBlock + swizzled_offset(row, ((q & 63) >> 3) + g);
+                        *reinterpret_cast<uint4*>(at) = hi;
+                        *reinterpret_cast<uint4*>(at + kPlaneOffset) = lo;
+                    }
+                }
             }
         }
         tmem_fence_before();
-        if (ranks > 1) cluster.sync();
-        else __syncthreads();
-        {
+        if (ranks > 1) {
+            cluster.sync();
             const int each = MP / ranks;                              // rows that this CTA sums
             for (int i = tid; i < each * (MP / 8); i += kMidThreads) {
                 const int r = rank * each + i / (MP / 8), chunk = i % (MP / 8);
-                float v[8] = {};
+                float4 a[8], b[8];
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
                     if (q < ranks) {
-                        const float4* from = reinterpret_cast<const float4*>(ranks > 1 ? cluster.map_shared_rank(share, q) : share) + r * (MP / 4);
-                        const float4 a = from[(2 * chunk) ^ (r & 7)], b = from[(2 * chunk + 1) ^ (r & 7)];
-                        v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
+                        const float4* from = reinterpret_cast<const float4*>(cluster.map_shared_rank(share, q)) + r * (MP / 4);
+                        a[q] = from[(2 * chunk) ^ (r & 7)];
+                        b[q] = from[(2 * chunk + 1) ^ (r & 7)];
                     }
                 }
+                float v[8] = {};
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (q < ranks)
+                        v[0] += a[q].x, v[1] += a[q].y, v[2] += a[q].z, v[3] += a[q].w, v[4] += b[q].x, v[5] += b[q].y, v[6] += b[q].z, v[7] += b[q].w;
                 uint4 hi, lo;
                 split8<false>(v, 1.f, 0.f, none, none, hi, lo);
                 const uint32_t at = (chunk >> 3) * kBlock + swizzled_offset(r, chunk & 7);
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
                     if (q < ranks) {
-                        uint8_t* to = (ranks > 1 ? cluster.map_shared_rank(gram, q) : gram) + at;
+                        uint8_t* to = cluster.map_shared_rank(gram, q) + at;
                         *reinterpret_cast<uint4*>(to) = hi;
                         *reinterpret_cast<uint4*>(to + kPlaneOffset) = lo;
                     }
                 }
             }
+            fence_proxy_async_all();
+            cluster.sync();
+            if (issues_mixed || issues_main) fence_proxy_async_all();
+        } else {
+            fence_proxy_async();
+            __syncthreads();
         }
-        fence_proxy_async_all();
-        if (ranks > 1) cluster.sync();
-        else __syncthreads();
         if (!poly.linear) {
-            if (tid == 0) {
-                fence_proxy_async_all();
+            if (issues_mixed || issues_main) {
                 tmem_fence_after();
                 constexpr uint32_t instruction = f16_instruction(128, MP, false, false);
 #pragma unroll
                 for (int k = 0; k < MP / 16; ++k) {
                     const uint64_t a = k_major_descriptor(gram_at + (k >> 2) * kBlock + (k & 3) * kMajorStep);
-                    mma_f16_single(tmem + MP, a, a + lo_plane, instruction, k > 0);
-                    mma_f16_single(tmem + MP, a + lo_plane, a, instruction, true);
-                    mma_f16_single(tmem, a, a, instruction, k > 0);
+                    if (issues_mixed) {
+                        mma_f16_single(tmem + MP, a, a + lo_plane, instruction, k > 0);
+                        mma_f16_single(tmem + MP, a + lo_plane, a, instruction, true);
+                    } else {
+                        mma_f16_single(tmem, a, a, instruction, k > 0);
+                    }
                 }
                 mma_commit_single(bar);
             }
@@ -1203,8 +1281,7 @@ __device__ __forceinline__ void mid_matrix(const Matrix& m, int ranks, int rank,
 #pragma unroll 1
                 for (int q = part * 32; q < MP; q += (kMidWarps / 4) * 32) {
                     float v[32], add[32];
-                    tmem_load32(tmem + lanes + MP + q, v);
-                    tmem_load32(tmem + lanes + q, add);
+                    tmem_load32(tmem + lanes + MP + q, v, tmem + lanes + q, add);
 #pragma unroll
                     for (int e = 0; e < 32; ++e) v[e] += add[e] * (q + e == row ? 1.f + 2.4f * loss : 1.f + 0.7f * loss);
                     uint8_t* block = gram + (q >> 6) * kBlock;
@@ -1226,17 +1303,19 @@ __device__ __forceinline__ void mid_matrix(const Matrix& m, int ranks, int rank,
         // 256 columns at a time: 256 of tensor memory for each of the two sums
         for (int c0 = 0; c0 < last; c0 += 256) {
             const int n = min(256, (last - c0 + 15) & ~15);
-            if (tid == 0) {
-                fence_proxy_async_all();
+            if (issues_mixed || issues_main) {
                 tmem_fence_after();
                 const uint32_t instruction = f16_instruction(128, n, false, true);
 #pragma unroll
                 for (int k = 0; k < MP / 16; ++k) {
                     const uint64_t a = k_major_descriptor(gram_at + (k >> 2) * kBlock + (k & 3) * kMajorStep);
                     const uint64_t b = mn_major_descriptor(x_at + (c0 >> 6) * kBlock + k * mnMajorStep, kBlock);
-                    mma_f16_single(tmem + 256, a, b + lo_plane, instruction, k > 0);
-                    mma_f16_single(tmem + 256, a + lo_plane, b, instruction, true);
-                    mma_f16_single(tmem, a, b, instruction, k > 0);
+                    if (issues_mixed) {
+                        mma_f16_single(tmem + 256, a, b + lo_plane, instruction, k > 0);
+                        mma_f16_single(tmem + 256, a + lo_plane, b, instruction, true);
+                    } else {
+                        mma_f16_single(tmem, a, b, instruction, k > 0);
+                    }
                 }
                 mma_commit_single(bar);
             }
@@ -1246,8 +1325,7 @@ __device__ __forceinline__ void mid_matrix(const Matrix& m, int ranks, int rank,
 #pragma unroll 1
                 for (int q = part * 32; q < n; q += (kMidWarps / 4) * 32) {
                     float v[32], add[32];
-                    tmem_load32(tmem + lanes + 256 + q, v);
-                    tmem_load32(tmem + lanes + q, add);
+                    tmem_load32(tmem + lanes + 256 + q, v, tmem + lanes + q, add);
 #pragma unroll
                     for (int e = 0; e < 32; ++e) v[e] += add[e] * made_good;
                     uint8_t* block = x + ((c0 + q) >> 6) * kBlock;
@@ -1272,40 +1350,60 @@ __device__ __forceinline__ void mid_matrix(const Matrix& m, int ranks, int rank,
     }
     if (!ok) report_check(CHECK_MBARRIER_TIMEOUT);
     T* out = static_cast<T*>(m.out);
-#pragma unroll 1
+    const bool out_vectors = !tall && rows_aligned(out, m.out_stride, sizeof(T));
+#pragma unroll 2
     for (int unit = tid; unit < units; unit += kMidThreads) {
-        const int r = tall ? unit & (MP - 1) : unit / (blocks * 8), chunk = tall ? unit / MP : unit % (blocks * 8);
-        if (r >= wide_rows) continue;
+        int r, col;
+        place(unit, r, col);
+        if (r >= wide_rows || col >= wide_cols) continue;
+        const int chunk = (col - col0) >> 3;
         const uint8_t* at = x + (chunk >> 3) * kBlock + swizzled_offset(r, chunk & 7);
         Chunk hi, lo;
         hi.raw = *reinterpret_cast<const uint4*>(at);
         lo.raw = *reinterpret_cast<const uint4*>(at + kPlaneOffset);
+        float v[8], old[8];
+        const bool whole = !tall && col + 8 <= wide_cols;
+        if (MUON && whole) load8(out + r * m.out_stride + col, out_vectors, old);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const int c = col0 + chunk * 8 + e;
-            if (c < wide_cols) {
-                const long long o = tall ? c * m.out_stride + r : r * m.out_stride + c;
-                float v = (__half2float(hi.h[e]) + __half2float(lo.h[e])) * (1.f / kScaleX);
-                if (!ok) v = __int_as_float(0x7fffffff);
-                out[o] = T(MUON ? float(out[o]) * mo.decay - m.rate * v : v);
+            v[e] = (__half2float(hi.h[e]) + __half2float(lo.h[e])) * (1.f / kScaleX);
+            if (!ok) v[e] = __int_as_float(0x7fffffff);
+            if (MUON && whole) v[e] = old[e] * mo.decay - m.rate * v[e];
+        }
+        if (whole) {
+            store8(out + r * m.out_stride + col, out_vectors, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (col + e < wide_cols) {
+                    T* to = out + (tall ? (col + e) * m.out_stride + r : r * m.out_stride + col + e);
+                    *to = T(MUON ? float(*to) * mo.decay - m.rate * v[e] : v[e]);
+                }
             }
         }
     }
     if (ranks > 1) cluster.sync();                                    // no CTA leaves while its shared memory is read or written
 }
 
+// One cluster per matrix, of either kind.
 template <typename T, bool MUON>
-__global__ void __launch_bounds__(kMidThreads, 1) mid_kernel(const __grid_constant__ ShortBatch b, int ranks, Momentum mo, int steps, Polynomial poly,
-                                                             float epsilon) {
+__global__ void __launch_bounds__(kMidThreads, 1) cluster_kernel(const __grid_constant__ ClusterBatch b, int ranks, Momentum mo, int steps, float ca,
+                                                                 float cb, float cc, Polynomial poly, float epsilon) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ double warp_sum[kMidWarps], cta_sum;
     __shared__ uint64_t bar;
     __shared__ uint32_t tmem_address;
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const Matrix& m = b.m[blockIdx.x / unsigned(ranks)];
-    const int rank = int(blockIdx.x % unsigned(ranks));
+    const int rank = int(blockIdx.x % unsigned(ranks)), rows = min(m.rows, m.cols);
+    if (rows <= kShortRows) {
+        float* floats = reinterpret_cast<float*>(smem);
+        if (rows <= 8) short_matrix<T, MUON, 8>(m, ranks, rank, mo, steps, ca, cb, cc, epsilon, floats, warp_sum, &cta_sum);
+        else short_matrix<T, MUON, 16>(m, ranks, rank, mo, steps, ca, cb, cc, epsilon, floats, warp_sum, &cta_sum);
+        return;
+    }
     if (threadIdx.x == 0) {
-        mbar_init(&bar, 1);
+        mbar_init(&bar, 2);                                           // commits of the two issuing threads
         fence_mbar_init();
     }
     if (threadIdx.x < 32) tmem_alloc_single(&tmem_address, 512);
@@ -1313,7 +1411,7 @@ __global__ void __launch_bounds__(kMidThreads, 1) mid_kernel(const __grid_consta
     __syncthreads();
     tmem_fence_after();
     const uint32_t tmem = tmem_address;
-    if (min(m.rows, m.cols) <= 64) mid_matrix<T, MUON, 64>(m, ranks, rank, mo, steps, poly, epsilon, smem, tmem, &bar, warp_sum, &cta_sum);
+    if (rows <= 64) mid_matrix<T, MUON, 64>(m, ranks, rank, mo, steps, poly, epsilon, smem, tmem, &bar, warp_sum, &cta_sum);
     else mid_matrix<T, MUON, 128>(m, ranks, rank, mo, steps, poly, epsilon, smem, tmem, &bar, warp_sum, &cta_sum);
     __syncthreads();
     if (threadIdx.x < 32) tmem_free_single(tmem, 512);
@@ -1526,15 +1624,18 @@ int run_batch(const Batch& b, int steps, const Polynomial& poly, float epsilon, 
     return GMC_OK;
 }
 
-// Which kernel a matrix goes to, by its shape.
-constexpr size_t kShortSmemLimit = 220 * 1024;
-constexpr int kMidSmemLimit = 227 * 1024 - 512;
-enum Kind { SHORT, MID, CHAIN, KINDS };
+// Which kernel a matrix goes to, by its shape; the shared memory that it takes with a number of CTAs.
+constexpr int kClusterSmemLimit = 227 * 1024 - 512;
+int cluster_smem(int rows, int cols, int ranks) {
+    return rows <= kShortRows ? int(short_smem(rows, cols, ranks)) + 1024 : mid_smem(mid_rows(rows), mid_blocks(cols, ranks));
+}
+bool fits(int rows, int cols, int ranks) {
+    return cluster_smem(rows, cols, ranks) <= kClusterSmemLimit && (rows <= kShortRows || mid_blocks(cols, ranks) <= mid_max_blocks(mid_rows(rows)));
+}
+enum Kind { CLUSTER, CHAIN, KINDS };
 Kind kind_of(const gmc_matrix& g) {
-    const long long rows = g.rows < g.cols ? g.rows : g.cols, cols = g.rows < g.cols ? g.cols : g.rows;
-    if (rows <= kShortRows && short_smem(int(rows), int(cols), 8) <= kShortSmemLimit) return SHORT;
-    if (rows <= 128 && mid_blocks(int(cols), 8) <= mid_max_blocks(mid_rows(int(rows)))) return MID;
-    return CHAIN;
+    const int rows = int(g.rows < g.cols ? g.rows : g.cols), cols = int(g.rows < g.cols ? g.cols : g.rows);
+    return rows <= 128 && fits(rows, cols, 8) ? CLUSTER : CHAIN;
 }
 void describe(const gmc_matrix& g, Matrix& m) {
     m.update = g.update;
@@ -1567,43 +1668,36 @@ int launch_clusters(Kernel kernel, int n, int ranks, int threads, size_t smem, s
 }
 
 template <typename T, bool MUON>
-int run_mid(const gmc_matrix* matrices, const int* which, int n, int steps, const Polynomial& poly, float epsilon, const Momentum& mo,
-            cudaStream_t stream) {
-    ShortBatch b;
-    int ranks = 1, smem = 0;
-    for (int i = 0; i < n; ++i) {
-        describe(matrices[which[i]], b.m[i]);
-        const int rows = std::min(b.m[i].rows, b.m[i].cols), cols = std::max(b.m[i].rows, b.m[i].cols);
-        // up to 256 columns a CTA: below, the exchange of the shares costs more than the products save
-        while (ranks < 8 && (mid_blocks(cols, ranks) > mid_max_blocks(mid_rows(rows)) || cols > 256 * ranks)) ranks *= 2;
-    }
-    for (int i = 0; i < n; ++i) {
-        const int rows = std::min(b.m[i].rows, b.m[i].cols), cols = std::max(b.m[i].rows, b.m[i].cols);
-        smem = std::max(smem, mid_smem(mid_rows(rows), mid_blocks(cols, ranks)));
-    }
-    return launch_clusters(mid_kernel<T, MUON>, n, ranks, kMidThreads, smem, kMidSmemLimit, stream, b, ranks, mo, steps, poly, epsilon);
-}
-
-template <typename T, bool MUON>
-int run_short(const gmc_matrix* matrices, const int* which, int n, int steps, float ca, float cb, float cc, float epsilon,
-              const Momentum& mo, cudaStream_t stream) {
-    ShortBatch b;
-    int ranks = 1, device = 0, n_sm = 0;
+int run_clusters(const gmc_matrix* matrices, const int* which, int n, int steps, float ca, float cb, float cc, const Polynomial& poly, float epsilon,
+                 const Momentum& mo, cudaStream_t stream) {
+    ClusterBatch b;
+    int ranks = 1, smem = 0, device = 0, n_sm = 0;
     GMC_CUDA_TRY(cudaGetDevice(&device));
     GMC_CUDA_TRY(cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, device));
-    size_t smem = 0;
     for (int i = 0; i < n; ++i) {
         describe(matrices[which[i]], b.m[i]);
-        const Matrix& m = b.m[i];
-        const int rows = m.rows < m.cols ? m.rows : m.cols, cols = m.rows < m.cols ? m.cols : m.rows;
-        while (ranks < 8 && ((cols / ranks > 40 && 2 * ranks * n <= n_sm) || short_smem(rows, cols, ranks) > kShortSmemLimit)) ranks *= 2;
+        const int rows = std::min(b.m[i].rows, b.m[i].cols), cols = std::max(b.m[i].rows, b.m[i].cols);
+        // more CTAs where X does not fit, and while there are free multiprocessors beyond 256 columns a CTA: below, the exchange
+        // of the shares costs more than the products save (64 x 160: 41 us with one CTA, 49 with four)
+        while (ranks < 8 && (!fits(rows, cols, ranks) || (cols > 256 * ranks && 2 * ranks * n <= n_sm))) ranks *= 2;
     }
-    for (int i = 0; i < n; ++i) {
-        const int rows = b.m[i].rows < b.m[i].cols ? b.m[i].rows : b.m[i].cols, cols = b.m[i].rows < b.m[i].cols ? b.m[i].cols : b.m[i].rows;
-        const size_t need = short_smem(rows, cols, ranks);
-        smem = need > smem ? need : smem;
-    }
-    return launch_clusters(short_kernel<T, MUON>, n, ranks, kShortThreads, smem, kShortSmemLimit, stream, b, ranks, mo, steps, ca, cb, cc, epsilon);
+    for (int i = 0; i < n; ++i)
+        smem = std::max(smem, cluster_smem(std::min(b.m[i].rows, b.m[i].cols), std::max(b.m[i].rows, b.m[i].cols), ranks));
+    auto kernel = cluster_kernel<T, MUON>;
+    GMC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kClusterSmemLimit));
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(unsigned(n * ranks));
+    config.blockDim = dim3(kMidThreads);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attribute;
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = unsigned(ranks);
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    GMC_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, b, ranks, mo, steps, ca, cb, cc, poly, epsilon));
+    return GMC_OK;
 }
 
 template <typename T, bool MUON>
@@ -1614,10 +1708,8 @@ int run_typed(const gmc_matrix* matrices, int n, int steps, float ca, float cb, 
         for (int i = 0; i <= n; ++i) {
             if (i < n && kind_of(matrices[i]) == kind) which[count++] = i;
             if (count == kMaxMatrices || (i == n && count > 0)) {
-                if (kind == SHORT) {
-                    if (int s = run_short<T, MUON>(matrices, which, count, steps, ca, cb, cc, epsilon, mo, stream)) return s;
-                } else if (kind == MID) {
-                    if (int s = run_mid<T, MUON>(matrices, which, count, steps, poly, epsilon, mo, stream)) return s;
+                if (kind == CLUSTER) {
+                    if (int s = run_clusters<T, MUON>(matrices, which, count, steps, ca, cb, cc, poly, epsilon, mo, stream)) return s;
                 } else {
                     Batch b;
                     size_t bytes = 0;
