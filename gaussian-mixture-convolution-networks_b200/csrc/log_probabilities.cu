@@ -107,10 +107,23 @@ struct Outputs {
     long long* top_indices;
 };
 
-// One thread: the row's outputs apart from the alternatives. Returns log s.
+// The target of a row and its logit, read early: the outputs come at the end of a chain of latencies.
+struct Target {
+    long long t;
+    float z;
+};
 template <typename T>
-__device__ __forceinline__ float write_row(const Outputs& out, const Stat& st, const T* z, const long long* targets, long long row,
-                                           int n_classes, long long ignored, float inv_t) {
+__device__ __forceinline__ Target read_target(const T* z, const long long* targets, long long row, int n_classes, long long ignored) {
+    Target g = {ignored, 0.f};
+    if (targets) {
+        g.t = targets[row];
+        if (g.t >= 0 && g.t < n_classes) g.z = to_float<T>(z[g.t]);
+    }
+    return g;
+}
+// One thread: the row's outputs apart from the alternatives. Returns log s.
+__device__ __forceinline__ float write_row(const Outputs& out, const Stat& st, const Target& g, long long row, int n_classes, long long ignored,
+                                           float inv_t) {
     const bool empty = st.m == neg_inf() && st.s == 0.f;
     const float log_s = logf(st.s);
     out.entropy[row] = empty ? 0.f : log_s - inv_t * (st.t / st.s);
@@ -119,15 +132,14 @@ __device__ __forceinline__ float write_row(const Outputs& out, const Stat& st, c
         out.stats[2 * row + 1] = log_s;
     }
     if (out.target) {
-        const long long t = targets[row];
         float v;
-        if (t == ignored) {
+        if (g.t == ignored) {
             v = 0.f;
-        } else if (t < 0 || t >= n_classes) {
+        } else if (g.t < 0 || g.t >= n_classes) {
             report_check(CHECK_CLASS_RANGE);
             v = quiet_nan();
         } else {
-            v = empty ? neg_inf() : (to_float<T>(z[t]) - st.m) * inv_t - log_s;
+            v = empty ? neg_inf() : (g.z - st.m) * inv_t - log_s;
         }
         out.target[row] = v;
     }
@@ -150,6 +162,7 @@ __global__ void __launch_bounds__(kSmallThreads) forward_small_kernel(const T* _
     const T* z = logits + row * row_stride;
     float v[E];
     Stat st = {neg_inf(), 0.f, 0.f};
+    const Target given = lane == 0 ? read_target<T>(z, targets, row, n_classes, ignored) : Target{ignored, 0.f};
 #pragma unroll
     for (int i = 0; i < E; ++i) {
         const int c = lane + 32 * i;
@@ -167,7 +180,7 @@ __global__ void __launch_bounds__(kSmallThreads) forward_small_kernel(const T* _
         st.t += __shfl_xor_sync(0xffffffffu, st.t, o);
     }
     float log_s = 0.f;
-    if (lane == 0) log_s = write_row<T>(out, st, z, targets, row, n_classes, ignored, inv_t);
+    if (lane == 0) log_s = write_row(out, st, given, row, n_classes, ignored, inv_t);
     if (n_top == 0) return;
     log_s = __shfl_sync(0xffffffffu, log_s, 0);
     // the k-th alternative is the largest key below the one before it
@@ -230,34 +243,20 @@ __device__ __forceinline__ void list_offer(Key& list, Key& bound, Key key, int n
         waiting &= ~(1u << src);
     }
 }
-__device__ __forceinline__ Key sort_descending(Key key, int lane) {                 // bitonic, within the warp
-#pragma unroll
-    for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-        for (int stride = size >> 1; stride > 0; stride >>= 1) {
-            const Key other = __shfl_xor_sync(0xffffffffu, key, stride);
-            const bool keep_larger = ((lane & size) == 0) == ((lane & stride) == 0);
-            key = (key > other) == keep_larger ? key : other;
-        }
-    return key;
-}
-// Number of keys above `key` in n_lists descending lists of 32.
-__device__ __forceinline__ int rank_in_lists(const Key (*lists)[32], int n_lists, Key key) {
+// Number of keys above `key` among n keys in shared memory, which are all different.
+__device__ __forceinline__ int rank_among(const Key* keys, int n, Key key) {
     int rank = 0;
 #pragma unroll 4
-    for (int l = 0; l < n_lists; ++l) {
-        int at = 0;
-#pragma unroll
-        for (int step = 16; step > 0; step >>= 1)
-            if (lists[l][at + step - 1] > key) at += step;
-        rank += at + (lists[l][at] > key ? 1 : 0);
-    }
+    for (int i = 0; i < n; ++i) rank += keys[i] > key ? 1 : 0;
     return rank;
 }
 
-// Alternatives without a second look at the row: after the sums every thread holds the largest key of the elements it
-// read. The n_top largest elements lie with the n_top threads whose keys are largest (keys are all different), so only
-// those threads' elements are read again, by their warp, and collected in a sorted list per warp.
+// Alternatives without a second look at most of the row. After the sums every thread knows its largest element; the n_top-th
+// largest of the 32 maxima of groups of eight threads is a value that at least n_top elements reach, and few more than that
+// do (about 30 for 20 of independent values). The threads whose maximum reaches it read their elements again and collect
+// those that do; a collected element's place is the number of larger ones. Where too many are equal (a constant row), the
+// warps go through all their elements and keep sorted lists instead.
+constexpr int kCollected = 512;
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kRowThreads) forward_row_kernel(const T* __restrict__ logits, const long long* __restrict__ targets,
                                                                   int n_classes, long long row_stride, int n_ranks, float inv_t, float k,
@@ -265,16 +264,17 @@ __global__ void __launch_bounds__(kRowThreads) forward_row_kernel(const T* __res
     constexpr int N = Vec<T>::N;
     __shared__ Stat warp_stat[kRowWarps];
     __shared__ Stat cta_stat;
-    __shared__ Key lists[kRowWarps][32];
-    __shared__ Key cta_list[32];
-    __shared__ Key threshold;
+    __shared__ float group_max[32], row_log_s;
+    __shared__ Key collected[kCollected];
+    __shared__ Key cta_list[kMaxTop];
+    __shared__ int count;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = int(blockIdx.x % unsigned(n_ranks));
     const long long row = blockIdx.x / unsigned(n_ranks);
     const Row<T> r(logits + row * row_stride, n_classes, rank, n_ranks);
+    const Target given = tid == 0 && rank == 0 ? read_target<T>(r.z, targets, row, n_classes, ignored) : Target{ignored, 0.f};
 
     Stat st = {neg_inf(), 0.f, 0.f};
-    int best_at = -1;                                                               // where st.m was seen first
     const bool has_head = r.singles && tid < r.head, has_tail = r.singles && tid < r.tail;
     const int tail_first = r.head + r.n_vec * N;
     if (has_head) {
@@ -291,10 +291,7 @@ __global__ void __launch_bounds__(kRowThreads) forward_row_kernel(const T* __res
         for (int u = 0; u < kUnroll; ++u)
 #pragma unroll
             for (int i = 0; i < N; ++i) m = fmaxf(m, v[u].at(i));
-        if (m > st.m) {
-            raise(st, m, k);
-            best_at = at;
-        }
+        if (m > st.m) raise(st, m, k);
         const float base = st.m == neg_inf() ? 0.f : st.m;
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u)
@@ -303,14 +300,19 @@ __global__ void __launch_bounds__(kRowThreads) forward_row_kernel(const T* __res
     }
     if (has_tail) {
         const float z = to_float<T>(r.z[tail_first + tid]);
-        if (z > st.m) {
-            raise(st, z, k);
-            best_at = -2;
-        }
+        if (z > st.m) raise(st, z, k);
         add_element(z, st.m == neg_inf() ? 0.f : st.m, k, st.s, st.t);
     }
 
     const float mine = st.m;
+    if constexpr (TOP) {
+        float m = mine;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if ((lane & 7) == 0) group_max[tid >> 3] = m;
+        if (tid == 0) count = 0;
+        if (tid < kMaxTop) cta_list[tid] = 0;
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         const Stat other = {__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
@@ -318,101 +320,111 @@ __global__ void __launch_bounds__(kRowThreads) forward_row_kernel(const T* __res
         st = merge(st, other, k);
     }
     if (lane == 0) warp_stat[warp] = st;
-
-    if constexpr (TOP) {
-        // the thread's largest key: first element equal to its maximum; without one (-inf, NaN) all its elements count
-        Key key = 0;
-        const bool any = mine != neg_inf();
-        if (has_head && (!any || best_at == -1)) key = make_key(to_float<T>(r.z[tid]), unsigned(tid));
-        if (has_tail && (!any || best_at == -2)) {
-            const Key other = make_key(to_float<T>(r.z[tail_first + tid]), unsigned(tail_first + tid));
-            key = other > key ? other : key;
-        }
-        if (!any || best_at >= 0) {
-            const int from = any ? best_at : r.first + tid;
-            const int to = any ? min(r.end, best_at + kRowThreads * kUnroll) : r.end;
-            for (int at = from; at < to; at += kRowThreads) {
-                const Vec<T> v = r.load(at);
+    __syncthreads();
+    // all warps' sums, by the lanes of the first one
+    if (warp == 0) {
+        st = lane < kRowWarps ? warp_stat[lane] : Stat{neg_inf(), 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const Key other = make_key(v.at(i), unsigned(r.element(at) + i));
-                    key = other > key ? other : key;
-                }
+        for (int o = kRowWarps / 2; o > 0; o >>= 1) {
+            const Stat other = {__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
+                                __shfl_xor_sync(0xffffffffu, st.t, o)};
+            st = merge(st, other, k);
+        }
+        if (lane == 0) {
+            cta_stat = st;
+            if (n_ranks == 1) row_log_s = write_row(out, st, given, row, n_classes, ignored, inv_t);
+        }
+    }
+    if constexpr (TOP) {
+        // every warp finds the n_top-th of the groups' maxima
+        const float m = group_max[lane];
+        int above = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const float other = __shfl_sync(0xffffffffu, m, i);
+            above += other > m || (other == m && i < lane) ? 1 : 0;
+        }
+        const float bar = __shfl_sync(0xffffffffu, m, __ffs(__ballot_sync(0xffffffffu, above == n_top - 1)) - 1);
+        auto collect = [&](float z, int c) {
+            if (z >= bar) {
+                const int place = atomicAdd(&count, 1);
+                if (place < kCollected) collected[place] = make_key(z, unsigned(c));
+            }
+        };
+        if (bar > neg_inf() && mine >= bar) {
+            if (has_head) collect(to_float<T>(r.z[tid]), tid);
+            if (has_tail) collect(to_float<T>(r.z[tail_first + tid]), tail_first + tid);
+            for (int at = r.first + tid; at < r.end; at += kRowThreads * kUnroll) {
+                Vec<T> v[kUnroll];
+#pragma unroll
+                for (int u = 0; u < kUnroll; ++u) v[u] = r.load(at + u * kRowThreads);
+#pragma unroll
+                for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) collect(v[u].at(i), r.element(at + u * kRowThreads) + i);
             }
         }
-        lists[warp][lane] = sort_descending(key, lane);
-        if (tid == 0) threshold = 0;
         __syncthreads();
-        const int place = key ? rank_in_lists(lists, kRowWarps, key) : kRowThreads;
-        if (place == n_top - 1) threshold = key - 1;
-        __syncthreads();
-        Key bound = threshold, list = 0;
-        unsigned chosen = __ballot_sync(0xffffffffu, place < n_top);
-        while (chosen) {
-            const int owner = (warp << 5) + __ffs(chosen) - 1;
-            chosen &= chosen - 1;
+        int n = count;
+        if (n > kCollected || bar == neg_inf()) {
+            __syncthreads();                                                        // count and collected are replaced
+            Key list = 0, bound = 0;
             if (r.singles) {
-                const int e = lane == 0 ? (owner < r.head ? owner : -1) : lane == 1 && owner < r.tail ? tail_first + owner : -1;
-                list_offer(list, bound, e >= 0 ? make_key(to_float<T>(r.z[e]), unsigned(e)) : 0, n_top, lane);
+                list_offer(list, bound, has_head ? make_key(to_float<T>(r.z[tid]), unsigned(tid)) : 0, n_top, lane);
+                list_offer(list, bound, has_tail ? make_key(to_float<T>(r.z[tail_first + tid]), unsigned(tail_first + tid)) : 0, n_top, lane);
             }
-            for (int at0 = r.first + owner; at0 < r.end; at0 += kRowThreads * 32) {
-                const int at = at0 + lane * kRowThreads;
+            for (int at0 = r.first + warp * 32; at0 < r.end; at0 += kRowThreads) {
+                const int at = at0 + lane;
                 const Vec<T> v = r.load(at);
 #pragma unroll
                 for (int i = 0; i < N; ++i)
                     list_offer(list, bound, at < r.end ? make_key(v.at(i), unsigned(r.element(at) + i)) : 0, n_top, lane);
             }
+            collected[tid] = list;
+            __syncthreads();
+            n = kRowThreads;
+        }
+        for (int i = tid; i < n; i += kRowThreads) {
+            const Key key = collected[i];
+            const int place = key ? rank_among(collected, n, key) : kRowThreads;
+            if (place < n_top) cta_list[place] = key;
         }
         __syncthreads();
-        lists[warp][lane] = list;
-        if (tid < 32) cta_list[tid] = 0;
-        __syncthreads();
-        const Key entry = lists[warp][lane];
-        if (entry) {
-            const int p = rank_in_lists(lists, kRowWarps, entry);
-            if (p < n_top) cta_list[p] = entry;
-        }
-    }
-    __syncthreads();
-    if (tid == 0) {
-        Stat all = warp_stat[0];
-        for (int w = 1; w < kRowWarps; ++w) all = merge(all, warp_stat[w], k);
-        cta_stat = all;
     }
     if (n_ranks == 1) {
-        __syncthreads();
-        if (warp == 0) {
-            float log_s = 0.f;
-            if (lane == 0) log_s = write_row<T>(out, cta_stat, r.z, targets, row, n_classes, ignored, inv_t);
-            if constexpr (TOP) {
-                log_s = __shfl_sync(0xffffffffu, log_s, 0);
-                if (lane < n_top)
-                    write_alternative(out, cta_list[lane], row, n_top, lane, cta_stat.m, log_s, cta_stat.m == neg_inf() && cta_stat.s == 0.f, inv_t);
-            }
+        if constexpr (TOP) {
+            if (tid < n_top)
+                write_alternative(out, cta_list[tid], row, n_top, tid, cta_stat.m, row_log_s, cta_stat.m == neg_inf() && cta_stat.s == 0.f, inv_t);
         }
         return;
     }
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
     if (rank == 0) {
+        const int total = n_ranks * n_top;
         if constexpr (TOP) {
-            lists[warp][lane] = warp < n_ranks ? cluster.map_shared_rank(cta_list, warp)[lane] : 0;
-            __syncthreads();
-            const Key entry = lists[warp][lane];
-            const int p = entry ? rank_in_lists(lists, kRowWarps, entry) : kRowThreads;
-            __syncthreads();                                                        // lists read before cta_list is replaced
-            if (p < n_top) cta_list[p] = entry;
-            __syncthreads();
+            for (int i = tid; i < total; i += kRowThreads) collected[i] = cluster.map_shared_rank(cta_list, i / n_top)[i % n_top];
         }
         if (warp == 0) {
-            Stat all = *cluster.map_shared_rank(&cta_stat, 0);
-            for (int c = 1; c < n_ranks; ++c) all = merge(all, *cluster.map_shared_rank(&cta_stat, c), k);
-            float log_s = 0.f;
-            if (lane == 0) log_s = write_row<T>(out, all, r.z, targets, row, n_classes, ignored, inv_t);
-            if constexpr (TOP) {
-                log_s = __shfl_sync(0xffffffffu, log_s, 0);
-                if (lane < n_top)
-                    write_alternative(out, cta_list[lane], row, n_top, lane, all.m, log_s, all.m == neg_inf() && all.s == 0.f, inv_t);
+            st = lane < n_ranks ? *cluster.map_shared_rank(&cta_stat, lane) : Stat{neg_inf(), 0.f, 0.f};
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) {
+                const Stat other = {__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
+                                    __shfl_xor_sync(0xffffffffu, st.t, o)};
+                st = merge(st, other, k);
+            }
+            if (lane == 0) {
+                warp_stat[0] = st;
+                row_log_s = write_row(out, st, given, row, n_classes, ignored, inv_t);
+            }
+        }
+        if constexpr (TOP) {
+            __syncthreads();
+            const Stat all = warp_stat[0];
+            for (int i = tid; i < total; i += kRowThreads) {
+                const Key key = collected[i];
+                const int place = key ? rank_among(collected, total, key) : kRowThreads;
+                if (place < n_top) write_alternative(out, key, row, n_top, place, all.m, row_log_s, all.m == neg_inf() && all.s == 0.f, inv_t);
             }
         }
     }
