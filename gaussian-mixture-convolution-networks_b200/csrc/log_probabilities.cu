@@ -86,17 +86,32 @@ __device__ __forceinline__ void raise(Stat& a, float m, float k) {
     }
     a.m = m;
 }
-__device__ __forceinline__ Stat merge(Stat a, Stat b, float k) {
-    const float m = fmaxf(a.m, b.m);
+// Over the lanes: the maximum first, then one rescaling and two sums (a merge of pairs would rescale in each of five steps).
+__device__ __forceinline__ Stat warp_merge(Stat a, float k) {
+    float m = a.m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     raise(a, m, k);
-    raise(b, m, k);
-    return {m, a.s + b.s, a.t + b.t};
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+        a.t += __shfl_xor_sync(0xffffffffu, a.t, o);
+    }
+    return a;
 }
 __device__ __forceinline__ void add_element(float z, float base, float k, float& s, float& t) {
     const float x = z - base;
     const float e = ex2_approx(x * k);
     s += e;
     t += e * fmaxf(x, kLowest);
+}
+
+// Two elements at once: packed additions and products take one issue slot for both.
+__device__ __forceinline__ void add_pair(float2 z, float2 minus_base, float2 k, float2& s, float2& t) {
+    const float2 x = __fadd2_rn(z, minus_base), y = __fmul2_rn(x, k);
+    const float2 e = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+    s = __fadd2_rn(s, e);
+    t = __ffma2_rn(e, make_float2(fmaxf(x.x, kLowest), fmaxf(x.y, kLowest)), t);
 }
 
 struct Outputs {
@@ -258,7 +273,7 @@ __device__ __forceinline__ int rank_among(const Key* keys, int n, Key key) {
 // warps go through all their elements and keep sorted lists instead.
 constexpr int kCollected = 512;
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kRowThreads) forward_row_kernel(const T* __restrict__ logits, const long long* __restrict__ targets,
+__global__ void __launch_bounds__(kRowThreads, 4) forward_row_kernel(const T* __restrict__ logits, const long long* __restrict__ targets,
                                                                   int n_classes, long long row_stride, int n_ranks, float inv_t, float k,
                                                                   long long ignored, int n_top, Outputs out) {
     constexpr int N = Vec<T>::N;
@@ -282,21 +297,31 @@ __global__ void __launch_bounds__(kRowThreads) forward_row_kernel(const T* __res
         if (z > st.m) st.m = z;
         add_element(z, st.m == neg_inf() ? 0.f : st.m, k, st.s, st.t);
     }
+    Vec<T> next[kUnroll];                                                           // on its way while the last ones are added up
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) next[u] = r.load(r.first + tid + u * kRowThreads);
     for (int at = r.first + tid; at < r.end; at += kRowThreads * kUnroll) {
         Vec<T> v[kUnroll];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) v[u] = r.load(at + u * kRowThreads);
+        for (int u = 0; u < kUnroll; ++u) {
+            v[u] = next[u];
+            next[u] = r.load(at + (kUnroll + u) * kRowThreads);
+        }
         float m = v[0].at(0);
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u)
 #pragma unroll
             for (int i = 0; i < N; ++i) m = fmaxf(m, v[u].at(i));
         if (m > st.m) raise(st, m, k);
-        const float base = st.m == neg_inf() ? 0.f : st.m;
+        const float minus_base = st.m == neg_inf() ? 0.f : -st.m;
+        float2 s2 = make_float2(0.f, 0.f), t2 = s2;
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u)
 #pragma unroll
-            for (int i = 0; i < N; ++i) add_element(v[u].at(i), base, k, st.s, st.t);
+            for (int i = 0; i < N; i += 2)
+                add_pair(make_float2(v[u].at(i), v[u].at(i + 1)), make_float2(minus_base, minus_base), make_float2(k, k), s2, t2);
+        st.s += s2.x + s2.y;
+        st.t += t2.x + t2.y;
     }
     if (has_tail) {
         const float z = to_float<T>(r.z[tail_first + tid]);
@@ -313,23 +338,12 @@ __global__ void __launch_bounds__(kRowThreads) forward_row_kernel(const T* __res
         if (tid == 0) count = 0;
         if (tid < kMaxTop) cta_list[tid] = 0;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const Stat other = {__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
-                            __shfl_xor_sync(0xffffffffu, st.t, o)};
-        st = merge(st, other, k);
-    }
+    st = warp_merge(st, k);
     if (lane == 0) warp_stat[warp] = st;
     __syncthreads();
     // all warps' sums, by the lanes of the first one
     if (warp == 0) {
-        st = lane < kRowWarps ? warp_stat[lane] : Stat{neg_inf(), 0.f, 0.f};
-#pragma unroll
-        for (int o = kRowWarps / 2; o > 0; o >>= 1) {
-            const Stat other = {__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
-                                __shfl_xor_sync(0xffffffffu, st.t, o)};
-            st = merge(st, other, k);
-        }
+        st = warp_merge(lane < kRowWarps ? warp_stat[lane] : Stat{neg_inf(), 0.f, 0.f}, k);
         if (lane == 0) {
             cta_stat = st;
             if (n_ranks == 1) row_log_s = write_row(out, st, given, row, n_classes, ignored, inv_t);
@@ -406,13 +420,7 @@ __global__ void __launch_bounds__(kRowThreads) forward_row_kernel(const T* __res
             for (int i = tid; i < total; i += kRowThreads) collected[i] = cluster.map_shared_rank(cta_list, i / n_top)[i % n_top];
         }
         if (warp == 0) {
-            st = lane < n_ranks ? *cluster.map_shared_rank(&cta_stat, lane) : Stat{neg_inf(), 0.f, 0.f};
-#pragma unroll
-            for (int o = 4; o > 0; o >>= 1) {
-                const Stat other = {__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
-                                    __shfl_xor_sync(0xffffffffu, st.t, o)};
-                st = merge(st, other, k);
-            }
+            st = warp_merge(lane < n_ranks ? *cluster.map_shared_rank(&cta_stat, lane) : Stat{neg_inf(), 0.f, 0.f}, k);
             if (lane == 0) {
                 warp_stat[0] = st;
                 row_log_s = write_row(out, st, given, row, n_classes, ignored, inv_t);
@@ -437,8 +445,8 @@ struct Incoming {
     const float* entropy;
     const float* top;
 };
-struct RowGradient {                // grad_j = p_j (a + b (log p_j + H)), plus the given classes' own terms
-    float m, log_s, h, a, b, g_target, log2_s;
+struct RowGradient {                // grad_j = p_j (a + b x_j), x_j = z_j - m, plus the given classes' own terms
+    float m, a, b, g_target, log2_s;
     long long target;
     bool empty, bad;
 };
@@ -446,25 +454,28 @@ __device__ __forceinline__ RowGradient row_gradient(const Incoming& in, const fl
                                                     long long row, int n_classes, long long ignored, int n_top, float inv_t) {
     RowGradient g;
     g.m = stats[2 * row];
-    g.log_s = stats[2 * row + 1];
-    g.log2_s = g.log_s * kLog2e;
-    g.h = entropy[row];
-    g.empty = g.m == neg_inf() && g.log_s == neg_inf();
+    const float log_s = stats[2 * row + 1], h = entropy[row];
+    g.log2_s = log_s * kLog2e;
+    g.empty = g.m == neg_inf() && log_s == neg_inf();
     g.target = in.target ? targets[row] : ignored;
     g.bad = g.target != ignored && (g.target < 0 || g.target >= n_classes);
     g.g_target = g.target != ignored && !g.bad ? in.target[row] : 0.f;
     float sum = g.g_target;
     if (in.top)
         for (int i = 0; i < n_top; ++i) sum += in.top[row * n_top + i];
-    g.a = -sum * inv_t;
-    g.b = in.entropy ? -in.entropy[row] * inv_t : 0.f;
+    // -p_j / T (sum + g_H (x_j / T - log s + H))
+    const float g_h = in.entropy ? in.entropy[row] : 0.f;
+    g.a = -inv_t * (sum + g_h * (h - log_s));
+    g.b = -inv_t * g_h * inv_t;
     return g;
 }
-__device__ __forceinline__ float gradient_at(const RowGradient& g, float z, float inv_t, float k) {
-    const float x = z - g.m;
-    const float p = ex2_approx(x * k - g.log2_s);
-    return p * (g.a + g.b * (fmaxf(x, kLowest) * inv_t + (g.h - g.log_s)));
+__device__ __forceinline__ float2 gradient_pair(const RowGradient& g, float2 z, float k) {
+    const float2 x = __fadd2_rn(z, make_float2(-g.m, -g.m));
+    const float2 y = __ffma2_rn(x, make_float2(k, k), make_float2(-g.log2_s, -g.log2_s));
+    const float2 p = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+    return __fmul2_rn(p, __ffma2_rn(make_float2(fmaxf(x.x, kLowest), fmaxf(x.y, kLowest)), make_float2(g.b, g.b), make_float2(g.a, g.a)));
 }
+__device__ __forceinline__ float gradient_at(const RowGradient& g, float z, float k) { return gradient_pair(g, make_float2(z, z), k).x; }
 // One thread: the whole gradient at the i-th given class (0 = the target, 1.. = the alternatives) of a row, written once
 // for classes that are given more than once.
 template <typename T>
@@ -478,7 +489,7 @@ __device__ __forceinline__ void given_class(const RowGradient& g, const Incoming
     if (i == 0 && in.top)
         for (int j = 0; j < n_top; ++j)
             if (tops[j] == c) own += in.top[row * n_top + j];
-    grad[c] = from_float<T>(gradient_at(g, to_float<T>(z[c]), inv_t, k) + own * inv_t);
+    grad[c] = from_float<T>(gradient_at(g, to_float<T>(z[c]), k) + own * inv_t);
 }
 
 template <typename T, int E>
@@ -498,7 +509,7 @@ __global__ void __launch_bounds__(kSmallThreads) backward_small_kernel(const T* 
     for (int i = 0; i < E; ++i) {
         const int c = lane + 32 * i;
         if (c < n_classes) {
-            const float v = gradient_at(g, to_float<T>(z[c]), inv_t, k);
+            const float v = gradient_at(g, to_float<T>(z[c]), k);
             dz[c] = from_float<T>(g.bad ? quiet_nan() : g.empty ? 0.f : v);
         }
     }
@@ -518,42 +529,51 @@ __global__ void __launch_bounds__(kRowThreads) backward_row_kernel(const T* __re
                                                                    long long row_stride, float inv_t, float k, long long ignored, int n_top) {
     constexpr int N = Vec<T>::N;
     const int tid = threadIdx.x;
-    const long long row = blockIdx.x / unsigned(n_stretches);
-    const int stretch = int(blockIdx.x % unsigned(n_stretches));
+    // from the last row to the first: the forward pass has left the last ones in the L2 cache
+    const unsigned cta = gridDim.x - 1 - blockIdx.x;
+    const long long row = cta / unsigned(n_stretches);
+    const int stretch = int(cta % unsigned(n_stretches));
     const T* z = logits + row * row_stride;
     T* dz = grad + row * n_classes;
+    const bool vectors = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15u) == 0;
+    Row<T> r(z, n_classes, 0, 1);
+    r.first = min(stretch * kStretch, r.n_vec);
+    r.end = min(r.n_vec, r.first + kStretch);
+    Vec<T> v[kUnroll];
+    if (vectors) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) v[u] = r.load(r.first + tid + u * kRowThreads);
+    }
     const RowGradient g = row_gradient(in, stats, entropy, targets, row, n_classes, ignored, n_top, inv_t);
     const bool constant = g.bad || g.empty;
     const float value = g.bad ? quiet_nan() : 0.f;
     int from, to;                                                                   // elements of this CTA
-    if (((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15u) == 0) {
-        Row<T> r(z, n_classes, 0, 1);
-        r.first = min(stretch * kStretch, r.n_vec);
-        r.end = min(r.n_vec, r.first + kStretch);
+    if (vectors) {
         from = stretch == 0 ? 0 : r.element(r.first);
         to = stretch == n_stretches - 1 ? n_classes : r.element(r.end);
-        Vec<T> v[kUnroll];
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) v[u] = r.load(r.first + tid + u * kRowThreads);
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             const int at = r.first + tid + u * kRowThreads;
             if (at < r.end) {
                 Vec<T> w;
 #pragma unroll
-                for (int i = 0; i < N; ++i) w.e[i] = from_float<T>(constant ? value : gradient_at(g, v[u].at(i), inv_t, k));
-                *reinterpret_cast<uint4*>(dz + r.element(at)) = w.raw;
+                for (int i = 0; i < N; i += 2) {
+                    const float2 d = gradient_pair(g, make_float2(v[u].at(i), v[u].at(i + 1)), k);
+                    w.e[i] = from_float<T>(constant ? value : d.x);
+                    w.e[i + 1] = from_float<T>(constant ? value : d.y);
+                }
+                __stcs(reinterpret_cast<uint4*>(dz + r.element(at)), w.raw);
             }
         }
-        if (stretch == 0 && tid < r.head) dz[tid] = from_float<T>(constant ? value : gradient_at(g, to_float<T>(z[tid]), inv_t, k));
+        if (stretch == 0 && tid < r.head) dz[tid] = from_float<T>(constant ? value : gradient_at(g, to_float<T>(z[tid]), k));
         const int c = r.element(r.n_vec) + tid;
         if (stretch == n_stretches - 1 && tid < r.tail)
-            dz[c] = from_float<T>(constant ? value : gradient_at(g, to_float<T>(z[c]), inv_t, k));
+            dz[c] = from_float<T>(constant ? value : gradient_at(g, to_float<T>(z[c]), k));
     } else {                                                                        // the two rows are aligned differently
         from = min(n_classes, stretch * kStretch * N);
         to = stretch == n_stretches - 1 ? n_classes : min(n_classes, from + kStretch * N);
         for (int c = from + tid; c < to; c += kRowThreads)
-            dz[c] = from_float<T>(constant ? value : gradient_at(g, to_float<T>(z[c]), inv_t, k));
+            dz[c] = from_float<T>(constant ? value : gradient_at(g, to_float<T>(z[c]), k));
     }
     if (constant) return;
     __syncthreads();                                                                // the stretch is written before the given classes
@@ -589,7 +609,8 @@ int forward_typed(const void* logits, const long long* targets, long long n_rows
     }
     int n_sm = 0;
     if (int s = multiprocessors(&n_sm)) return s;
-    // a row over several CTAs while there are fewer CTAs than the GPU holds and each keeps a full stretch of vectors
+    // a row over several CTAs while there are fewer CTAs than the GPU holds and each keeps a full stretch of vectors (1021 rows
+    // of 100003 in fp32: 112 us with one CTA per row, 136 with four, whose alternatives take longer than their columns)
     int n_ranks = 1;
     while (n_ranks < 8 && n_rows * n_ranks < 4LL * n_sm && n_classes / (2 * n_ranks) >= kRowThreads * Vec<T>::N) n_ranks *= 2;
     cudaLaunchConfig_t config = {};
