@@ -365,17 +365,23 @@ __global__ void __launch_bounds__(kRowThreads, 4) forward_row_kernel(const T* __
                 if (place < kCollected) collected[place] = make_key(z, unsigned(c));
             }
         };
-        if (bar > neg_inf() && mine >= bar) {
+        if (bar > neg_inf()) {
             if (has_head) collect(to_float<T>(r.z[tid]), tid);
             if (has_tail) collect(to_float<T>(r.z[tail_first + tid]), tail_first + tid);
-            for (int at = r.first + tid; at < r.end; at += kRowThreads * kUnroll) {
-                Vec<T> v[kUnroll];
+            // a thread's vectors by its whole warp: one after the other they would each wait for the memory
+            unsigned owners = __ballot_sync(0xffffffffu, mine >= bar);
+            while (owners) {
+                const int owner = (warp << 5) + __ffs(owners) - 1;
+                owners &= owners - 1;
+                for (int at0 = r.first + owner; at0 < r.end; at0 += kRowThreads * 32 * 2) {
+                    Vec<T> v[2];
 #pragma unroll
-                for (int u = 0; u < kUnroll; ++u) v[u] = r.load(at + u * kRowThreads);
+                    for (int u = 0; u < 2; ++u) v[u] = r.load(at0 + (u * 32 + lane) * kRowThreads);
 #pragma unroll
-                for (int u = 0; u < kUnroll; ++u)
+                    for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int i = 0; i < N; ++i) collect(v[u].at(i), r.element(at + u * kRowThreads) + i);
+                        for (int i = 0; i < N; ++i) collect(v[u].at(i), r.element(at0 + (u * 32 + lane) * kRowThreads) + i);
+                }
             }
         }
         __syncthreads();
