@@ -80,6 +80,39 @@ __device__ __forceinline__ int find_matrix(const Batch& b, int cta) {
     return i;
 }
 
+// Eight neighbouring elements, with vector accesses where `aligned` says that their address allows them.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, bool aligned, float (&v)[8]) {
+    if (aligned) {
+        constexpr int N = 16 / int(sizeof(T));
+        union { uint4 raw[8 / N]; T e[8]; } u;
+#pragma unroll
+        for (int i = 0; i < 8 / N; ++i) u.raw[i] = reinterpret_cast<const uint4*>(p)[i];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = float(u.e[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = float(p[e]);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, bool aligned, const float (&v)[8]) {
+    if (aligned) {
+        constexpr int N = 16 / int(sizeof(T));
+        union { uint4 raw[8 / N]; T e[8]; } u;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u.e[e] = T(v[e]);
+#pragma unroll
+        for (int i = 0; i < 8 / N; ++i) reinterpret_cast<uint4*>(p)[i] = u.raw[i];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = T(v[e]);
+    }
+}
+__device__ __forceinline__ bool rows_aligned(const void* p, long long stride, int size) {
+    return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t(stride) * size)) & 15u) == 0;
+}
+
 // Sum of squares of kNormElements elements per CTA, in fp64 (the squares of small updates leave the fp32 range); with a
 // momentum the running average is updated on the way.
 template <typename T, bool MUON>
@@ -90,20 +123,46 @@ __global__ void __launch_bounds__(256) norm_kernel(const __grid_constant__ Batch
     const long long total = (long long)m.rows * m.cols;
     const long long first = (long long)(int(blockIdx.x) - m.norm_first) * kNormElements;
     const int count = int(min((long long)kNormElements, total - first));
-    const int row0 = int(first / m.cols), col0 = int(first - (long long)row0 * m.cols);
     double s = 0.;
-    const unsigned cols = unsigned(m.cols);
-#pragma unroll 4
-    for (int i = threadIdx.x; i < count; i += 256) {
-        const unsigned at = unsigned(col0 + i), r = at / cols;
-        float u = load_float<T>(m.update, (row0 + (long long)r) * m.update_stride + (at - r * cols));
-        if constexpr (MUON) {
-            float* p = m.momentum + first + i;
-            const float now = mo.beta * *p + mo.one_minus_beta * u;
-            *p = now;
-            u = mo.nesterov ? mo.one_minus_beta * u + mo.beta * now : now;
+    // the update's element and the momentum's at the same place
+    auto blend = [&](float u, float& old) {
+        old = mo.beta * old + mo.one_minus_beta * u;
+        return mo.nesterov ? mo.one_minus_beta * u + mo.beta * old : old;
+    };
+    const T* update = static_cast<const T*>(m.update);
+    if (m.update_stride == m.cols && rows_aligned(update, 0, 1) && (!MUON || rows_aligned(m.momentum, 0, 1))) {
+        // one row as far as the norm is concerned
+#pragma unroll 2
+        for (int i = threadIdx.x * 8; i < count; i += 256 * 8) {
+            float u[8], old[8];
+            if (i + 8 <= count) {
+                load8(update + first + i, true, u);
+                if constexpr (MUON) {
+                    load8(m.momentum + first + i, true, old);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) u[e] = blend(u[e], old[e]);
+                    store8(m.momentum + first + i, true, old);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s += double(u[e]) * double(u[e]);
+            } else {
+                for (int e = i; e < count; ++e) {
+                    float v = float(update[first + e]);
+                    if constexpr (MUON) v = blend(v, m.momentum[first + e]);
+                    s += double(v) * double(v);
+                }
+            }
         }
-        s += double(u) * double(u);
+    } else {
+        const int row0 = int(first / m.cols), col0 = int(first - (long long)row0 * m.cols);
+        const unsigned cols = unsigned(m.cols);
+#pragma unroll 4
+        for (int i = threadIdx.x; i < count; i += 256) {
+            const unsigned at = unsigned(col0 + i), r = at / cols;
+            float u = float(update[(row0 + (long long)r) * m.update_stride + (at - r * cols)]);
+            if constexpr (MUON) u = blend(u, m.momentum[first + i]);
+            s += double(u) * double(u);
+        }
     }
     __shared__ double warp_sum[8];
 #pragma unroll
@@ -125,6 +184,27 @@ union Chunk {
     __half h[8];
 };
 
+// Eight columns: v c1, plus c0 (in_hi + in_lo), as planes.
+template <bool ADD>
+__device__ __forceinline__ void split8(const float* v, float c1, float c0, const uint4& in_hi, const uint4& in_lo, uint4& hi, uint4& lo) {
+    const __half2* ih = reinterpret_cast<const __half2*>(&in_hi);
+    const __half2* il = reinterpret_cast<const __half2*>(&in_lo);
+    __half2* oh = reinterpret_cast<__half2*>(&hi);
+    __half2* ol = reinterpret_cast<__half2*>(&lo);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float x = v[2 * e] * c1, y = v[2 * e + 1] * c1;
+        if (ADD) {
+            const float2 h = __half22float2(ih[e]), l = __half22float2(il[e]);
+            x += c0 * (h.x + l.x);
+            y += c0 * (h.y + l.y);
+        }
+        oh[e] = __floats2half2_rn(x, y);
+        const float2 back = __half22float2(oh[e]);
+        ol[e] = __floats2half2_rn(x - back.x, y - back.y);
+    }
+}
+
 // X = U / (|U| + eps) as planes: one 128 x 64 block per CTA, padding included.
 template <typename T, bool MUON>
 __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ Batch b, Momentum mo, float epsilon) {
@@ -145,30 +225,49 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ Batc
     const bool tall = m.rows > m.cols;
     const int wide_rows = tall ? m.cols : m.rows, wide_cols = tall ? m.rows : m.cols;
     const int row_tile = block / m.col_blocks, col_block = block - row_tile * m.col_blocks;
-    uint8_t* hi_block = reinterpret_cast<uint8_t*>(b.x[0]) + (m.x_block + block) * kBlockBytes;
-    uint8_t* lo_block = hi_block + kPlaneOffset;
+    // The block is laid out in shared memory, where its bytes' order costs nothing, and leaves as one bulk copy.
+    __shared__ __align__(128) uint8_t image[kBlockBytes];
+    const T* update = static_cast<const T*>(m.update);
+    const bool vectors = rows_aligned(update, m.update_stride, sizeof(T)), momentum_vectors = rows_aligned(m.momentum, m.cols, 4);
+    const float factor = kScaleX / norm;
+    const uint4 none = {};
+#pragma unroll 2
     for (int i = threadIdx.x; i < 128 * 8; i += 256) {
         const int row = tall ? i & 127 : i >> 3, chunk = tall ? i >> 7 : i & 7;      // neighbouring threads read along a row
-        const int r = row_tile * 128 + row;
-        Chunk hi, lo;
+        const int r = row_tile * 128 + row, c = col_block * 64 + chunk * 8;
+        float u[8], old[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int c = col_block * 64 + chunk * 8 + e;
-            float u = 0.f;
-            if (r < wide_rows && c < wide_cols) {
-                const long long rr = tall ? c : r, cc = tall ? r : c;
-                u = load_float<T>(m.update, rr * m.update_stride + cc);
-                if constexpr (MUON) {
-                    const float now = m.momentum[rr * m.cols + cc];
-                    u = mo.nesterov ? mo.one_minus_beta * u + mo.beta * now : now;
+        for (int e = 0; e < 8; ++e) u[e] = old[e] = 0.f;
+        if (!tall && r < wide_rows && c + 8 <= wide_cols) {
+            load8(update + r * m.update_stride + c, vectors, u);
+            if constexpr (MUON) load8(m.momentum + (long long)r * m.cols + c, momentum_vectors, old);
+        } else if (r < wide_rows) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (c + e < wide_cols) {
+                    const long long rr = tall ? c + e : r, cc = tall ? r : c + e;
+                    u[e] = float(update[rr * m.update_stride + cc]);
+                    if constexpr (MUON) old[e] = m.momentum[rr * m.cols + cc];
                 }
-                u = u / norm * kScaleX;
             }
-            split(u, hi.h[e], lo.h[e]);
         }
-        const uint32_t at = swizzled_offset(row, chunk);
-        *reinterpret_cast<uint4*>(hi_block + at) = hi.raw;
-        *reinterpret_cast<uint4*>(lo_block + at) = lo.raw;
+        if constexpr (MUON) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[e] = mo.nesterov ? mo.one_minus_beta * u[e] + mo.beta * old[e] : old[e];
+        }
+        uint4 hi, lo;
+        split8<false>(u, factor, 0.f, none, none, hi, lo);
+        uint8_t* at = image + swizzled_offset(row, chunk);
+        *reinterpret_cast<uint4*>(at) = hi;
+        *reinterpret_cast<uint4*>(at + kPlaneOffset) = lo;
+    }
+    fence_proxy_async();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        uint8_t* to = reinterpret_cast<uint8_t*>(b.x[0]) + (m.x_block + block) * kBlockBytes;
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(smem_u32(image)), "n"(kBlockBytes) : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
 }
 
@@ -181,26 +280,46 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Bat
     const bool tall = m.rows > m.cols;
     const int wide_rows = tall ? m.cols : m.rows, wide_cols = tall ? m.rows : m.cols;
     const int row_tile = block / m.col_blocks, col_block = block - row_tile * m.col_blocks;
-    const uint8_t* hi_block = reinterpret_cast<const uint8_t*>(b.x[which_x]) + (m.x_block + block) * kBlockBytes;
-    const uint8_t* lo_block = hi_block + kPlaneOffset;
+    __shared__ __align__(128) uint8_t image[kBlockBytes];
+    __shared__ uint64_t arrived;
+    if (threadIdx.x == 0) {
+        mbar_init(&arrived, 1);
+        fence_mbar_init();
+        mbar_arrive_expect_tx(&arrived, kBlockBytes);
+        bulk_copy_g2s(image, reinterpret_cast<const uint8_t*>(b.x[which_x]) + (m.x_block + block) * kBlockBytes, kBlockBytes, &arrived);
+    }
     T* out = static_cast<T*>(m.out);
-    const bool failed = b.arrived[b.n] != 0;
+    const bool vectors = rows_aligned(out, m.out_stride, sizeof(T));
+    __syncthreads();
+    const bool ok = mbar_wait_bounded(&arrived, 0) && b.arrived[b.n] == 0;
+#pragma unroll 2
     for (int i = threadIdx.x; i < 128 * 8; i += 256) {
         const int row = tall ? i & 127 : i >> 3, chunk = tall ? i >> 7 : i & 7;
-        const int r = row_tile * 128 + row;
-        if (r >= wide_rows) continue;
-        const uint32_t at = swizzled_offset(row, chunk);
+        const int r = row_tile * 128 + row, c = col_block * 64 + chunk * 8;
+        if (r >= wide_rows || c >= wide_cols) continue;
+        const uint8_t* at = image + swizzled_offset(row, chunk);
         Chunk hi, lo;
-        hi.raw = *reinterpret_cast<const uint4*>(hi_block + at);
-        lo.raw = *reinterpret_cast<const uint4*>(lo_block + at);
+        hi.raw = *reinterpret_cast<const uint4*>(at);
+        lo.raw = *reinterpret_cast<const uint4*>(at + kPlaneOffset);
+        float v[8], old[8];
+        const bool whole = !tall && c + 8 <= wide_cols;
+        if (MUON && whole) load8(out + r * m.out_stride + c, vectors, old);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const int c = col_block * 64 + chunk * 8 + e;
-            if (c >= wide_cols) break;
-            const long long o = tall ? c * m.out_stride + r : r * m.out_stride + c;
-            float x = (__half2float(hi.h[e]) + __half2float(lo.h[e])) * (1.f / kScaleX);
-            if (failed) x = __int_as_float(0x7fffffff);
-            out[o] = T(MUON ? float(out[o]) * mo.decay - m.rate * x : x);
+            v[e] = (__half2float(hi.h[e]) + __half2float(lo.h[e])) * (1.f / kScaleX);
+            if (!ok) v[e] = __int_as_float(0x7fffffff);
+            if (MUON && whole) v[e] = old[e] * mo.decay - m.rate * v[e];
+        }
+        if (whole) {
+            store8(out + r * m.out_stride + c, vectors, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (c + e < wide_cols) {
+                    T* to = out + (tall ? (c + e) * m.out_stride + r : r * m.out_stride + c + e);
+                    *to = T(MUON ? float(*to) * mo.decay - m.rate * v[e] : v[e]);
+                }
+            }
         }
     }
 }
@@ -307,60 +426,6 @@ __device__ __forceinline__ bool wait_counter(const unsigned* counter, unsigned v
 }
 __device__ __forceinline__ void fence_proxy_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
 __device__ __forceinline__ void writers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWriters) : "memory"); }
-
-// Eight neighbouring elements, with vector accesses where `aligned` says that their address allows them.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool aligned, float (&v)[8]) {
-    if (aligned) {
-        constexpr int N = 16 / int(sizeof(T));
-        union { uint4 raw[8 / N]; T e[8]; } u;
-#pragma unroll
-        for (int i = 0; i < 8 / N; ++i) u.raw[i] = reinterpret_cast<const uint4*>(p)[i];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = float(u.e[e]);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = float(p[e]);
-    }
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, bool aligned, const float (&v)[8]) {
-    if (aligned) {
-        constexpr int N = 16 / int(sizeof(T));
-        union { uint4 raw[8 / N]; T e[8]; } u;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) u.e[e] = T(v[e]);
-#pragma unroll
-        for (int i = 0; i < 8 / N; ++i) reinterpret_cast<uint4*>(p)[i] = u.raw[i];
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) p[e] = T(v[e]);
-    }
-}
-__device__ __forceinline__ bool rows_aligned(const void* p, long long stride, int size) {
-    return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t(stride) * size)) & 15u) == 0;
-}
-
-// Eight columns: v c1, plus c0 (in_hi + in_lo), as planes.
-template <bool ADD>
-__device__ __forceinline__ void split8(const float* v, float c1, float c0, const uint4& in_hi, const uint4& in_lo, uint4& hi, uint4& lo) {
-    const __half2* ih = reinterpret_cast<const __half2*>(&in_hi);
-    const __half2* il = reinterpret_cast<const __half2*>(&in_lo);
-    __half2* oh = reinterpret_cast<__half2*>(&hi);
-    __half2* ol = reinterpret_cast<__half2*>(&lo);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        float x = v[2 * e] * c1, y = v[2 * e + 1] * c1;
-        if (ADD) {
-            const float2 h = __half22float2(ih[e]), l = __half22float2(il[e]);
-            x += c0 * (h.x + l.x);
-            y += c0 * (h.y + l.y);
-        }
-        oh[e] = __floats2half2_rn(x, y);
-        const float2 back = __half22float2(oh[e]);
-        ol[e] = __floats2half2_rn(x - back.x, y - back.y);
-    }
-}
 
 struct ChainBarriers {
     uint64_t full[kStages], peer_full[kStages], empty[kStages], ready, drained, mixed_ready, mixed_drained, done;
