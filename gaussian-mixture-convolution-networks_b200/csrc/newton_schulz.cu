@@ -442,6 +442,54 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, unsigned parity) {
 struct WriterCounts {
     unsigned chunk, tile, k;
 };
+// 64 columns of a row in their place: v c1, plus c0 times what is there. The next chunk is read before this one is written,
+// which the compiler could not know to be safe.
+__device__ __forceinline__ void place_block(const float* v, uint8_t* rows, bool add, float c0, float c1, int lane) {
+    uint4 next_hi = {}, next_lo = {};
+    if (add) {
+        next_hi = *reinterpret_cast<const uint4*>(rows + swizzled_offset(lane, 0));
+        next_lo = *reinterpret_cast<const uint4*>(rows + swizzled_offset(lane, 0) + kPlaneOffset);
+    }
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {
+        uint8_t* at = rows + swizzled_offset(lane, g);
+        const uint4 in_hi = next_hi, in_lo = next_lo;
+        if (g < 7 && add) {
+            next_hi = *reinterpret_cast<const uint4*>(rows + swizzled_offset(lane, g + 1));
+            next_lo = *reinterpret_cast<const uint4*>(rows + swizzled_offset(lane, g + 1) + kPlaneOffset);
+        }
+        uint4 hi, lo;
+        split8<true>(v + g * 8, c1, c0, in_hi, in_lo, hi, lo);
+        *reinterpret_cast<uint4*>(at) = hi;
+        *reinterpret_cast<uint4*>(at + kPlaneOffset) = lo;
+    }
+}
+// A block's 32 rows leave, once they are in place.
+__device__ __forceinline__ void send_rows(const Planes& to, int row_block, int col_block, int quarter, const uint8_t* rows, int lane) {
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0 && row_block < to.row_blocks && col_block < to.col_blocks)
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to.block(row_block, col_block) + quarter * kWarpRows),
+                     "r"(smem_u32(rows)), "n"(kWarpRows)
+                     : "memory");
+}
+// The stage behind a tile is free: its barrier expects the two arrivals that the MMA threads' commits make for the others.
+__device__ __forceinline__ void release_stage(uint64_t* empty, int wide, int warp, int lane) {
+    if (lane == 0) {
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    }
+    __syncwarp();
+    if (wide) asm volatile("bar.sync %0, 128;" ::"r"(2 + (warp >> 2)) : "memory");
+    else writers_sync();
+    if (lane == 0 && (warp == 0 || (wide && warp == 4))) {
+        mbar_arrive(empty);
+        mbar_arrive(empty);
+    }
+}
+
+// WHOLE: one accumulation takes the whole axis.
+template <bool WHOLE>
 __device__ __forceinline__ bool write_product(Product p, const Walk& w, ChainBarriers& bar, uint8_t* stages, uint32_t tmem, int cta,
                                               WriterCounts& n, const Planes& to, float c0, float c1, int stages_per_chunk, float* partial) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -452,6 +500,56 @@ __device__ __forceinline__ bool write_product(Product p, const Walk& w, ChainBar
         int ti, tj, k0, k1;
         w.unit(p, u, ti, tj, k0, k1);
         const int diagonal = (2 * ti + cta) * 128 + (warp & 3) * 32 + lane - tj * 2 * half - col0;       // this row's
+        if constexpr (WHOLE) {
+            const int row_block = 2 * ti + cta;
+            // 32 columns at a time from tensor memory to their place, nothing kept in registers (with the sums of
+            // 128 columns in them the code is four times as long, and the time of a tile with it).
+            n.k += k1 - k0;
+            const bool shared_out = p == GRAM && w.splits > 1;
+            const unsigned k = n.k + (wide ? warp >> 2 : 0), s = k % kStages;
+            n.k += w.extra(p);
+            if (!warp_wait(&bar.ready, n.chunk & 1) || !warp_wait(&bar.mixed_ready, n.tile & 1)) return false;
+            if (!shared_out && !warp_wait(&bar.full[s], (k / kStages) & 1)) return false;
+            ++n.chunk;
+            tmem_fence_after();
+            const float loss = 0x1p-25f * 4.f * float(k1 - k0), made_good = 1.f + 0.7f * loss;
+            const float diagonal_good = 1.f + (p == GRAM ? 2.f : p == POLY ? 2.4f : 0.7f) * loss;
+#pragma unroll 1
+            for (int q = 0; q < half; q += 32) {
+                float v[32], mixed[32];
+                tmem_load32(tmem + lanes + col0 + q, v, tmem + kMixedColumns + lanes + col0 + q, mixed);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e] = v[e] * (q + e == diagonal ? diagonal_good : made_good) + mixed[e];
+                if (shared_out) {
+                    // [unit][CTA][column][row]
+                    float* out = partial + (((long long)u * 2 + cta) * (2 * half) + col0 + q) * 128 + (warp & 3) * 32 + lane;
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) out[e * 128] = v[e];
+                    continue;
+                }
+                uint8_t* rows = stages + s * kStageBytes + (wide ? q >> 6 : warp >> 2) * kBlockBytes + (warp & 3) * kWarpRows;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    uint8_t* at = rows + swizzled_offset(lane, ((q & 63) >> 3) + g);
+                    uint4 in_hi = {}, in_lo = {}, hi, lo;
+                    if (p != GRAM) {
+                        in_hi = *reinterpret_cast<const uint4*>(at);
+                        in_lo = *reinterpret_cast<const uint4*>(at + kPlaneOffset);
+                    }
+                    split8<true>(v + g * 8, c1, c0, in_hi, in_lo, hi, lo);
+                    *reinterpret_cast<uint4*>(at) = hi;
+                    *reinterpret_cast<uint4*>(at + kPlaneOffset) = lo;
+                }
+                if (q & 32) send_rows(to, row_block, ((tj * 2 * half + col0) >> 6) + (q >> 6), warp & 3, rows, lane);
+            }
+            tmem_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive_at(&bar.drained, 0);
+                mbar_arrive_at(&bar.mixed_drained, 0);
+            }
+            if (!shared_out) release_stage(&bar.empty[s], wide, warp, lane);
+        } else {
         float sum[128];
 #pragma unroll
         for (int i = 0; i < 128; ++i) sum[i] = 0.f;
@@ -504,50 +602,15 @@ __device__ __forceinline__ bool write_product(Product p, const Walk& w, ChainBar
         const unsigned k = n.k + (wide ? warp >> 2 : 0), s = k % kStages;
         n.k += wide ? 2 : 1;
         if (!warp_wait(&bar.full[s], (k / kStages) & 1)) return false;
-        const int row_block = 2 * ti + cta;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            if (j == 0 || wide) {
-                uint8_t* rows = stages + s * kStageBytes + (wide ? j : warp >> 2) * kBlockBytes + (warp & 3) * kWarpRows;
-                // in place; the next chunk is read before this one is written, which the compiler could not know to be safe
-                uint4 next_hi = {}, next_lo = {};
-                if (p != GRAM) {
-                    next_hi = *reinterpret_cast<const uint4*>(rows + swizzled_offset(lane, 0));
-                    next_lo = *reinterpret_cast<const uint4*>(rows + swizzled_offset(lane, 0) + kPlaneOffset);
-                }
-#pragma unroll
-                for (int g = 0; g < 8; ++g) {
-                    uint8_t* at = rows + swizzled_offset(lane, g);
-                    const uint4 in_hi = next_hi, in_lo = next_lo;
-                    if (g < 7 && p != GRAM) {
-                        next_hi = *reinterpret_cast<const uint4*>(rows + swizzled_offset(lane, g + 1));
-                        next_lo = *reinterpret_cast<const uint4*>(rows + swizzled_offset(lane, g + 1) + kPlaneOffset);
-                    }
-                    uint4 hi, lo;
-                    split8<true>(sum + j * 64 + g * 8, c1, c0, in_hi, in_lo, hi, lo);
-                    *reinterpret_cast<uint4*>(at) = hi;
-                    *reinterpret_cast<uint4*>(at + kPlaneOffset) = lo;
-                }
-                fence_proxy_async();
-                __syncwarp();
-                const int col_block = ((tj * 2 * half + col0) >> 6) + j;
-                if (lane == 0 && row_block < to.row_blocks && col_block < to.col_blocks)
-                    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to.block(row_block, col_block) + (warp & 3) * kWarpRows),
-                                 "r"(smem_u32(rows)), "n"(kWarpRows)
-                                 : "memory");
-            }
+        const int row_block = 2 * ti + cta;                           // declared here: a line higher up costs 500 bytes of spills
+        place_block(sum, stages + s * kStageBytes + (wide ? 0 : warp >> 2) * kBlockBytes + (warp & 3) * kWarpRows, p != GRAM, c0, c1, lane);
+        send_rows(to, row_block, (tj * 2 * half + col0) >> 6, warp & 3,
+                  stages + s * kStageBytes + (wide ? 0 : warp >> 2) * kBlockBytes + (warp & 3) * kWarpRows, lane);
+        if (wide) {
+            place_block(sum + 64, stages + s * kStageBytes + kBlockBytes + (warp & 3) * kWarpRows, p != GRAM, c0, c1, lane);
+            send_rows(to, row_block, ((tj * 2 * half + col0) >> 6) + 1, warp & 3, stages + s * kStageBytes + kBlockBytes + (warp & 3) * kWarpRows, lane);
         }
-        if (lane == 0) {
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-        }
-        __syncwarp();
-        // the stage is free: its barrier expects the two arrivals that the MMA warps' commits make for the others
-        if (wide) asm volatile("bar.sync %0, 128;" ::"r"(2 + (warp >> 2)) : "memory");
-        else writers_sync();
-        if (tid == 0 || (wide && tid == 128)) {
-            mbar_arrive(&bar.empty[s]);
-            mbar_arrive(&bar.empty[s]);
+        release_stage(&bar.empty[s], wide, warp, lane);
         }
     }
     return true;
@@ -590,6 +653,7 @@ struct Polynomial {
     int linear;
 };
 
+template <bool WHOLE>
 __global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_constant__ Batch b, int steps, Polynomial poly) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ ChainBarriers bar;
@@ -793,7 +857,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_co
             const Planes& to = p == STEP ? w.x(from_x ^ 1) : p == POLY || poly.linear ? w.poly : w.gram;
             const float c0 = p == STEP ? poly.step_from : p == POLY ? poly.poly_from : 0.f;
             const float c1 = p == STEP ? poly.step_factor : p == POLY ? poly.poly_factor : poly.gram_factor;
-            if (!write_product(p, w, bar, stages, tmem, cta, n, to, c0, c1, m.chunk, partial)) return false;
+            if (!write_product<WHOLE>(p, w, bar, stages, tmem, cta, n, to, c0, c1, m.chunk, partial)) return false;
             if (p == GRAM && w.splits > 1) {
                 arrive(true);
                 if (!wait(before + 1)) return false;
@@ -1608,8 +1672,8 @@ int chain_pairs(int* pairs) {
     attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
     config.attrs = &attribute;
     config.numAttrs = 1;
-    GMC_CUDA_TRY(cudaFuncSetAttribute(chain_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kChainSmem));
-    GMC_CUDA_TRY(cudaOccupancyMaxActiveClusters(pairs, chain_kernel, &config));
+    GMC_CUDA_TRY(cudaFuncSetAttribute(chain_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kChainSmem));
+    GMC_CUDA_TRY(cudaOccupancyMaxActiveClusters(pairs, chain_kernel<false>, &config));       // one CTA per multiprocessor either way
     if (*pairs > kPairs) *pairs = kPairs;
     if (*pairs < kMaxMatrices) return GMC_ERR_UNSUPPORTED;
     if (device < 64) known[device].store(*pairs);
@@ -1683,7 +1747,9 @@ int run_batch(const Batch& b, int steps, const Polynomial& poly, float epsilon, 
     attributes[1].val.cooperative = 1;
     config.attrs = attributes;
     config.numAttrs = 2;
-    GMC_CUDA_TRY(cudaLaunchKernelEx(&config, chain_kernel, b, steps, poly));
+    constexpr bool whole = !std::is_same<T, float>::value;
+    GMC_CUDA_TRY(cudaFuncSetAttribute(chain_kernel<whole>, cudaFuncAttributeMaxDynamicSharedMemorySize, kChainSmem));
+    GMC_CUDA_TRY(cudaLaunchKernelEx(&config, chain_kernel<whole>, b, steps, poly));
     finish_kernel<T, MUON><<<b.blocks, 256, 0, stream>>>(b, mo, steps & 1);
     GMC_LAUNCH_CHECK();
     return GMC_OK;
