@@ -464,28 +464,26 @@ __device__ __forceinline__ void place_block(const float* v, uint8_t* rows, bool 
         *reinterpret_cast<uint4*>(at + kPlaneOffset) = lo;
     }
 }
-// A block's 32 rows leave, once they are in place.
-__device__ __forceinline__ void send_rows(const Planes& to, int row_block, int col_block, int quarter, const uint8_t* rows, int lane) {
+// The stage behind a tile holds two neighbouring blocks of the result, complete once its warps (all, or the four of its half)
+// have come here: one copy takes them out. Then the stage is free: its barrier expects the two arrivals that the MMA threads'
+// commits make for the others.
+__device__ __forceinline__ void send_stage(const Planes& to, int row_block, int col_block, const uint8_t* stage, uint64_t* empty, int wide, int warp,
+                                           int lane) {
     fence_proxy_async();
-    __syncwarp();
-    if (lane == 0 && row_block < to.row_blocks && col_block < to.col_blocks)
-        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to.block(row_block, col_block) + quarter * kWarpRows),
-                     "r"(smem_u32(rows)), "n"(kWarpRows)
-                     : "memory");
-}
-// The stage behind a tile is free: its barrier expects the two arrivals that the MMA threads' commits make for the others.
-__device__ __forceinline__ void release_stage(uint64_t* empty, int wide, int warp, int lane) {
-    if (lane == 0) {
-        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-    }
-    __syncwarp();
     if (wide) asm volatile("bar.sync %0, 128;" ::"r"(2 + (warp >> 2)) : "memory");
     else writers_sync();
     if (lane == 0 && (warp == 0 || (wide && warp == 4))) {
+        const int blocks = row_block < to.row_blocks ? min(2, to.col_blocks - col_block) : 0;
+        if (blocks > 0)
+            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to.block(row_block, col_block)), "r"(smem_u32(stage)),
+                         "r"(blocks * kBlockBytes)
+                         : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         mbar_arrive(empty);
         mbar_arrive(empty);
     }
+    __syncwarp();
 }
 
 // WHOLE: one accumulation takes the whole axis.
@@ -501,14 +499,13 @@ __device__ __forceinline__ bool write_product(Product p, const Walk& w, ChainBar
         w.unit(p, u, ti, tj, k0, k1);
         const int diagonal = (2 * ti + cta) * 128 + (warp & 3) * 32 + lane - tj * 2 * half - col0;       // this row's
         if constexpr (WHOLE) {
-            const int row_block = 2 * ti + cta;
             // 32 columns at a time from tensor memory to their place, nothing kept in registers (with the sums of
             // 128 columns in them the code is four times as long, and the time of a tile with it).
             n.k += k1 - k0;
             const bool shared_out = p == GRAM && w.splits > 1;
             const unsigned k = n.k + (wide ? warp >> 2 : 0), s = k % kStages;
             n.k += w.extra(p);
-            if (!warp_wait(&bar.ready, n.chunk & 1) || !warp_wait(&bar.mixed_ready, n.tile & 1)) return false;
+            if (!warp_wait(&bar.ready, n.chunk & 1)) return false;
             if (!shared_out && !warp_wait(&bar.full[s], (k / kStages) & 1)) return false;
             ++n.chunk;
             tmem_fence_after();
@@ -540,15 +537,12 @@ __device__ __forceinline__ bool write_product(Product p, const Walk& w, ChainBar
                     *reinterpret_cast<uint4*>(at) = hi;
                     *reinterpret_cast<uint4*>(at + kPlaneOffset) = lo;
                 }
-                if (q & 32) send_rows(to, row_block, ((tj * 2 * half + col0) >> 6) + (q >> 6), warp & 3, rows, lane);
             }
             tmem_fence_before();
             __syncwarp();
-            if (lane == 0) {
-                mbar_arrive_at(&bar.drained, 0);
-                mbar_arrive_at(&bar.mixed_drained, 0);
-            }
-            if (!shared_out) release_stage(&bar.empty[s], wide, warp, lane);
+            if (lane == 0) mbar_arrive_at(&bar.drained, 0);
+            if (!shared_out)
+                send_stage(to, 2 * ti + cta, (tj * 2 * half + (wide ? col0 : 0)) >> 6, stages + s * kStageBytes, &bar.empty[s], wide, warp, lane);
         } else {
         float sum[128];
 #pragma unroll
@@ -602,15 +596,9 @@ __device__ __forceinline__ bool write_product(Product p, const Walk& w, ChainBar
         const unsigned k = n.k + (wide ? warp >> 2 : 0), s = k % kStages;
         n.k += wide ? 2 : 1;
         if (!warp_wait(&bar.full[s], (k / kStages) & 1)) return false;
-        const int row_block = 2 * ti + cta;                           // declared here: a line higher up costs 500 bytes of spills
         place_block(sum, stages + s * kStageBytes + (wide ? 0 : warp >> 2) * kBlockBytes + (warp & 3) * kWarpRows, p != GRAM, c0, c1, lane);
-        send_rows(to, row_block, (tj * 2 * half + col0) >> 6, warp & 3,
-                  stages + s * kStageBytes + (wide ? 0 : warp >> 2) * kBlockBytes + (warp & 3) * kWarpRows, lane);
-        if (wide) {
-            place_block(sum + 64, stages + s * kStageBytes + kBlockBytes + (warp & 3) * kWarpRows, p != GRAM, c0, c1, lane);
-            send_rows(to, row_block, ((tj * 2 * half + col0) >> 6) + 1, warp & 3, stages + s * kStageBytes + kBlockBytes + (warp & 3) * kWarpRows, lane);
-        }
-        release_stage(&bar.empty[s], wide, warp, lane);
+        if (wide) place_block(sum + 64, stages + s * kStageBytes + kBlockBytes + (warp & 3) * kWarpRows, p != GRAM, c0, c1, lane);
+        send_stage(to, 2 * ti + cta, (tj * 2 * half + (wide ? col0 : 0)) >> 6, stages + s * kStageBytes, &bar.empty[s], wide, warp, lane);
         }
     }
     return true;
@@ -691,7 +679,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_co
             mbar_init(&bar.peer_full[s], 1);
             mbar_init(&bar.empty[s], 2);
         }
-        mbar_init(&bar.ready, 1);
+        mbar_init(&bar.ready, WHOLE ? 2 : 1);                         // WHOLE: of both sums
         mbar_init(&bar.mixed_ready, 1);
         mbar_init(&bar.drained, 2 * (kWriters / 32));
         mbar_init(&bar.mixed_drained, 2 * (kWriters / 32));
@@ -801,7 +789,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_co
                     peer_phase ^= 1u << s;
                     // sums that are about to be overwritten are read
                     if (mixed) {
-                        if (kb == k0 && tile > 0 && !mbar_wait_cluster(&bar.mixed_drained, (tile - 1) & 1)) return false;
+                        if (kb == k0 && tile > 0 && !mbar_wait_cluster(WHOLE ? &bar.drained : &bar.mixed_drained, (tile - 1) & 1)) return false;
                     } else {
                         if (of_chunk == 0 && chunk > 0 && !mbar_wait_cluster(&bar.drained, (chunk - 1) & 1)) return false;
                     }
@@ -818,7 +806,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_co
                     }
                     mma_commit(&bar.empty[s]);
                     if (mixed) {
-                        if (kb == k1 - 1) mma_commit(&bar.mixed_ready);
+                        if (kb == k1 - 1) mma_commit(WHOLE ? &bar.ready : &bar.mixed_ready);
                     } else if (of_chunk == chunk_stages - 1 || kb == k1 - 1) {
                         mma_commit(&bar.ready);
                         ++chunk;
