@@ -1668,13 +1668,14 @@ int chain_pairs(int* pairs) {
     return GMC_OK;
 }
 
-constexpr long long kMaxSide = 32768;
+// The waits of the chain are bounded by 2^22 polls, 90 ms or more: a product of the largest matrix takes about 45 ms.
+constexpr long long kMaxSide = 32768, kMaxShortSide = 16384;
 
 int check_matrices(const gmc_matrix* matrices, int n) {
     if (n < 0 || (n > 0 && !matrices)) return n < 0 ? GMC_ERR_BAD_DIMS : GMC_ERR_NULL_POINTER;
     for (int i = 0; i < n; ++i) {
         const gmc_matrix& g = matrices[i];
-        if (g.rows < 1 || g.cols < 1 || g.rows > kMaxSide || g.cols > kMaxSide) return GMC_ERR_BAD_DIMS;
+        if (g.rows < 1 || g.cols < 1 || g.rows > kMaxSide || g.cols > kMaxSide || std::min(g.rows, g.cols) > kMaxShortSide) return GMC_ERR_BAD_DIMS;
         if (g.update_stride < g.cols || g.out_stride < g.cols) return GMC_ERR_BAD_DIMS;
     }
     return GMC_OK;

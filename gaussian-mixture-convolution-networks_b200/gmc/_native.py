@@ -85,9 +85,6 @@ _declare("gmc_log_probabilities_backward", [_c_void_p, _c_int] + [_c_void_p] * 8
 _declare("gmc_input_normalise", [_c_float_p, _c_void_p, _c_float_p, _c_float_p, ctypes.c_longlong, _c_int, _c_int, _c_int,
                                  _c_void_p, _c_void_p, _c_void_p])
 
-
-
-
 # struct gmc_matrix of the header: update, momentum, out, rows, cols, update_stride, out_stride, rate
 matrix_struct = struct.Struct("@PPPqqqqf4x")
 lib.gmc_orthogonalise_workspace_bytes.restype = ctypes.c_size_t

@@ -10,13 +10,18 @@ from torch import Tensor
 from gmc import _native
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
-MAX_SIDE = 32768
+MAX_SIDE, MAX_SHORT_SIDE = 32768, 16384
 
 
 def _coefficients(coefficients):
     if len(coefficients) != 3:
         raise _native.GmcError("coefficients are three numbers (a, b, c)")
     return [float(v) for v in coefficients]
+
+
+def _check_sides(rows: int, cols: int) -> None:
+    if max(rows, cols) > MAX_SIDE or min(rows, cols) > MAX_SHORT_SIDE:
+        raise _native.GmcError(f"matrices may be up to {MAX_SIDE} x {MAX_SHORT_SIDE}, got {rows} x {cols}")
 
 
 def _workspace(packed: bytes, n: int, device: torch.device):
@@ -32,8 +37,9 @@ def orthogonalise(updates: typing.Union[Tensor, typing.Sequence[Tensor]], steps:
                   coefficients: typing.Sequence[float] = COEFFICIENTS, epsilon: float = 1e-7):
     """The Newton-Schulz iterate of each matrix of `updates` ([..., rows, cols], or a list of such tensors of one type and
     device; float32, bfloat16 or float16, CUDA): X = U / (|U| + epsilon), then `steps` times X <- a X + (b A + c A A) X with
-    A = X X^T. Its singular values are near 1 whatever those of U were. Returns new tensors of the same shapes and type;
-    all products are accurate to fp32 rounding. A zero matrix gives zero, one with NaN or infinity gives NaN."""
+    A = X X^T. Its singular values are near 1 whatever those of U were. Returns new tensors of the same shapes and type, with
+    the error of a 32-bit evaluation for float32 and of the rounding for 16-bit types; not differentiable. A zero matrix gives
+    zero, one with NaN or infinity gives NaN. Matrices may be up to 32768 x 16384."""
     single = isinstance(updates, Tensor)
     tensors = [updates] if single else list(updates)
     a, b, c = _coefficients(coefficients)
@@ -45,6 +51,7 @@ def orthogonalise(updates: typing.Union[Tensor, typing.Sequence[Tensor]], steps:
         if t.dtype != tensors[0].dtype or t.device != tensors[0].device:
             raise _native.GmcError("updates of one call must have one type and device")
         rows, cols = t.shape[-2:]
+        _check_sides(rows, cols)
         t = t.detach()
         if t.dim() > 2 and not t.is_contiguous() or t.stride(-1) != 1 and cols > 1 or rows > 1 and t.stride(-2) < cols:
             t = t.contiguous()
@@ -106,6 +113,7 @@ def muon_update(params: typing.Sequence[Tensor], grads: typing.Sequence[Tensor],
             held.append(g)
         rows = p.shape[0]
         cols = p.numel() // rows
+        _check_sides(rows, cols)
         entries.append(_native.matrix_struct.pack(g.data_ptr(), m.data_ptr(), p.data_ptr(), rows, cols, cols, cols,
                                                   lr * math.sqrt(max(1.0, rows / cols))))
     packed = b"".join(entries)

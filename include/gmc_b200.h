@@ -345,7 +345,8 @@ int gmc_convolution_fitting_backward(const float* grad, const float* data, const
  * Masked classes (-inf) have probability 0. A row with nothing but -inf: log p = -inf, entropy 0, gradient 0. A row with
  * NaN or +inf: NaN log-probabilities, entropy and gradient. logits is [n_rows, n_classes] of `dtype` with unit class
  * stride and row_stride elements between rows (0 = one row for all); T in [1e-6, 1e6]; n_rows <= 2^27,
- * n_classes <= 2^30. Sums are fp32; outputs are fp32. Results do not depend on the launch order (no atomics).
+ * n_classes <= 2^30, and for the backward n_rows * ceil(n_classes * bytes per logit / 16384) < 2^31.
+ * Sums and outputs are fp32. The same call gives the same bits.
  *
  * Backward: dz_j = 1/T [ grad_target d(t, j) + sum_i grad_top[i] d(top_i, j) - p_j (grad_target + sum_i grad_top[i])
  *                        - p_j grad_entropy (log p_j + entropy) ]
@@ -368,14 +369,19 @@ int gmc_log_probabilities_backward(const void* logits, int dtype, const long lon
  * gmc_muon_update first updates the running average (fp32), m <- momentum m + (1 - momentum) U, takes U <- (nesterov) ?
  * (1 - momentum) U + momentum m : m, and then out <- decay out - rate X: out holds the parameters.
  * `matrices` is a HOST array; update, out are of `dtype` with unit column stride, *_stride elements (>= cols) between rows;
- * momentum is contiguous fp32. Matrices may differ in shape; 1 <= rows, cols <= 32768. A zero matrix gives zero; NaN or
- * infinity in a matrix makes that matrix NaN. out may be update (the same address and stride), no other overlap is allowed
- * within a call, and no matrix may appear twice. Products are accurate to fp32 rounding whatever `dtype`.
+ * momentum is contiguous fp32. Matrices may differ in shape; 1 <= rows, cols <= 32768, the smaller at most 16384. A zero
+ * matrix gives zero; NaN or infinity in a matrix makes that matrix NaN. out may be update (the same address and stride), no
+ * other overlap is allowed within a call, and no matrix may appear twice. Operands carry 22 bits, sums are fp32: for fp32 the
+ * error is that of an fp32 evaluation (0.2 to 1.2 times, measured); for 16-bit types sums over long axes are not split up
+ * (5e-5 of the result at 2048, against 2^-9 or 2^-12 for its rounding). How many CTAs share a sum depends on the other
+ * matrices of the call, and with it the last bits; the same call gives the same bits.
  * 1 <= steps <= 32; coefficients whose iterates reach 1.8 for a singular value in [0, 1], that are 100 or more, or with
  * |b| > 32 |c| > 0 are refused (GMC_ERR_UNSUPPORTED); 1e-30 <= epsilon <= 1e30; 0 <= momentum < 1.
  * workspace: gmc_orthogonalise_workspace_bytes (depends on the shapes only; 0 = none needed, or sizes out of range), aligned
- * to 1024 bytes, content undefined before and after; concurrent calls need one each. Nothing is allocated, kept or
- * synchronised.
+ * to 1024 bytes, content undefined before and after; concurrent calls need one each. Nothing is allocated or synchronised,
+ * and nothing kept but, per device, the number of CTA pairs that it holds. Matrices whose smaller side is above 128 (or that
+ * are too long for the shared memory of eight CTAs) run in a cooperative launch over the whole GPU; it needs 96
+ * multiprocessors (GMC_ERR_UNSUPPORTED otherwise). A wait in it that runs out gives NaN and check bit 1.
  * ---------------------------------------------------------------------------------------------- */
 typedef struct gmc_matrix {
     const void* update;

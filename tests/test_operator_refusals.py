@@ -58,6 +58,7 @@ def test_orthogonalise_argument_checks():
             return _native.lib.gmc_muon_update(m, n, dtype, steps, *abc, eps, beta, 1, 1.0, work, size, NULL)
         return _native.lib.gmc_orthogonalise(m, n, dtype, steps, *abc, eps, work, size, NULL)
 
+    assert run(rows=16385, cols=16385, us=16385, os_=16385) == 1
     assert run(rows=0) == 1 and run(cols=0) == 1 and run(rows=32769) == 1 and run(us=139) == 1 and run(os_=139) == 1 and run(n=-1) == 1
     assert run(dtype=3) == 4 and run(steps=0) == 4 and run(steps=33) == 4 and run(eps=0.0) == 4 and run(eps=float("nan")) == 4
     assert run(abc=(10.0, 0.0, 0.0)) == 4 and run(abc=(float("nan"), 0.0, 0.0)) == 4 and run(abc=(1.0, -4.0, 0.0)) == 4

@@ -62,6 +62,16 @@ def test_orthogonalise(m, n, dtype):
     assert torch.equal(u, before)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n", [(8, 9000), (16, 513), (17, 300), (64, 4096), (64, 4097), (65, 1536), (128, 1536), (128, 1537), (2000, 100),
+                                 (129, 5000), (256, 6000), (6000, 250), (1500, 4100)])
+def test_where_one_kernel_ends_and_the_next_begins(m, n, dtype):
+    """Both sides of the shapes that decide between fp32 tiles, one cluster, and the whole GPU; columns shared out; long axes."""
+    from gmc.optimisation import orthogonalise
+    u = _update(m, n, seed=m + n, dtype=dtype)
+    _check(orthogonalise(u), u)
+
+
 def test_a_long_inner_axis():
     """The sums of X X^T over 20000 columns, all of one sign on the diagonal."""
     from gmc.optimisation import orthogonalise
@@ -123,10 +133,10 @@ def test_batches_lists_and_strides():
     # how many CTAs share a matrix's sums depends on what else is in the call: every result is held to the bound by itself
     u = _update(3, 2, 70, 90)
     _check(orthogonalise(u), u)
-    for shape in ((101, 10, 12), (50, 130, 70), (2, 1, 300, 200)):
+    for shape in ((101, 10, 12), (50, 130, 70), (50, 150, 200), (2, 1, 300, 200)):
         many = _update(*shape)
         _check(orthogonalise(many), many)
-    shapes = [(30, 40), (300, 140), (1, 9), (130, 700), (64, 64), (64, 3000), (700, 90)]
+    shapes = [(30, 40), (300, 140), (1, 9), (130, 700), (64, 64), (64, 3000), (700, 90), (1000, 1000), (260, 3000)]
     mixed = [_update(m, n, seed=i) for i, (m, n) in enumerate(shapes)]
     for o, t in zip(orthogonalise(mixed), mixed):
         _check(o, t)
@@ -170,6 +180,46 @@ def test_muon_update(shapes, nesterov, dtype):
         step = torch.linalg.vector_norm(wp - old.double())
         assert torch.linalg.vector_norm(p.double() - wp) <= (2 * half + 3 * 2.0 ** -24) * torch.linalg.vector_norm(wp) \
             + (4 ** 5 * 3 * 2.0 ** -24 + 2.0 ** -12) * step
+
+
+def test_muon_update_of_many_matrices_and_strided_gradients():
+    """More matrices than one launch takes, of all kinds, with gradients that are transposed or broadcast views."""
+    from gmc.optimisation import muon_update
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    shapes = [(5 + i, 7 + 3 * i) for i in range(60)] + [(130 + i, 140 + i) for i in range(50)]
+    params = [torch.randn(s, device="cuda", generator=gen) for s in shapes]
+    grads = [_update(s[1], s[0], seed=i).t() if i % 2 else torch.randn(1, s[1], device="cuda", generator=gen).expand(s) for i, s in enumerate(shapes)]
+    momenta = [torch.zeros(s, device="cuda") for s in shapes]
+    want = [_muon_reference(p, g, m, 0.1, 0.9, 0.0, True) for p, g, m in zip(params, grads, momenta)]
+    before = [p.clone() for p in params]
+    muon_update(params, grads, momenta, 0.1, 0.9)
+    for p, (wp, _), old in zip(params, want, before):
+        step = torch.linalg.vector_norm(wp - old.double())
+        assert torch.linalg.vector_norm(p.double() - wp) <= 2.0 ** -23 * torch.linalg.vector_norm(wp) + (4 ** 5 * 3 * 2.0 ** -24 + 2.0 ** -12) * step
+
+
+def test_the_same_tensor_twice_is_refused():
+    from gmc._native import GmcError
+    from gmc.optimisation import muon_update, orthogonalise
+    p, g, m = (torch.zeros(3, 4, device="cuda") for _ in range(3))
+    with pytest.raises(GmcError, match="appears twice"):
+        muon_update([p, p], [g, g], [m, m.clone()], 0.1)
+    with pytest.raises(GmcError, match="contiguous"):
+        muon_update([p.t()], [g.t()], [m.t()], 0.1)
+    with pytest.raises(GmcError, match="float32"):
+        muon_update([p], [g], [m.bfloat16()], 0.1)
+    with pytest.raises(GmcError, match="one type"):
+        muon_update([p], [g.bfloat16()], [m], 0.1)
+    with pytest.raises(GmcError, match="one type"):
+        orthogonalise([p, g.bfloat16()])
+    with pytest.raises(GmcError, match="matrices"):
+        orthogonalise(torch.zeros(5, device="cuda"))
+    with pytest.raises(GmcError, match="up to 32768"):
+        orthogonalise(torch.zeros(1, 1, device="cuda").expand(40000, 3))
+    with pytest.raises(GmcError, match="unsupported parameter"):
+        orthogonalise(p, coefficients=(9.0, 0.0, 0.0))
+    with pytest.raises(GmcError, match="unsupported parameter"):
+        orthogonalise(p, steps=0)
 
 
 def test_optimiser_steps_and_state():
