@@ -69,10 +69,6 @@ struct Momentum {
     float decay;                // factor of the parameters
 };
 
-// The update's element: the given one, or the momentum's.
-template <typename T>
-__device__ __forceinline__ float load_float(const void* p, long long i) { return float(static_cast<const T*>(p)[i]); }
-
 template <int Matrix::*FIRST>
 __device__ __forceinline__ int find_matrix(const Batch& b, int cta) {
     int i = 0;
@@ -114,7 +110,7 @@ __device__ __forceinline__ bool rows_aligned(const void* p, long long stride, in
 }
 
 // Sum of squares of kNormElements elements per CTA, in fp64 (the squares of small updates leave the fp32 range); with a
-// momentum the running average is updated on the way.
+// momentum the running average is updated on the way. NORM_FIG
 template <typename T, bool MUON>
 __global__ void __launch_bounds__(256) norm_kernel(const __grid_constant__ Batch b, Momentum mo) {
     if (blockIdx.x == 0 && threadIdx.x <= unsigned(b.n)) b.arrived[threadIdx.x] = 0;        // for the chain
@@ -175,10 +171,6 @@ __global__ void __launch_bounds__(256) norm_kernel(const __grid_constant__ Batch
     }
 }
 
-__device__ __forceinline__ void split(float v, __half& hi, __half& lo) {
-    hi = __float2half_rn(v);
-    lo = __float2half_rn(v - __half2float(hi));
-}
 union Chunk {
     uint4 raw;
     __half h[8];
@@ -205,7 +197,7 @@ __device__ __forceinline__ void split8(const float* v, float c1, float c0, const
     }
 }
 
-// X = U / (|U| + eps) as planes: one 128 x 64 block per CTA, padding included.
+// X = U / (|U| + eps) as planes: one 128 x 64 block per CTA, padding included. Bound by the memory: SPLIT_FIG.
 template <typename T, bool MUON>
 __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ Batch b, Momentum mo, float epsilon) {
     const int which = find_matrix<&Matrix::block_first>(b, blockIdx.x);
@@ -271,7 +263,7 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ Batc
     }
 }
 
-// The last X as the output's type, or subtracted from the parameters.
+// The last X as the output's type, or subtracted from the parameters. FINISH_FIG
 template <typename T, bool MUON>
 __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Batch b, Momentum mo, int which_x) {
     const int which = find_matrix<&Matrix::block_first>(b, blockIdx.x);
@@ -338,9 +330,16 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Bat
 // as contiguous bulk copies.
 //
 // The tensor core adds into its fp32 accumulator without rounding to nearest: the sums fall short by about n 2^-24 of
-// themselves after n additions. For fp32 results hi hi is therefore accumulated over four stages (256 in K, 16 additions)
-// only and then added to registers, while other MMAs run, with the mean of the loss made good; hi lo and lo hi, 2^-11 as
-// large, have an accumulator of their own. Where results are rounded to 16 bits, one accumulation takes the whole axis.
+// themselves after n additions. For fp32 results hi hi is therefore accumulated over two to eight stages (128 to 512 in K,
+// 8 to 32 additions, by the matrix's size) only and then added to registers, while other MMAs run, with the mean of the loss
+// made good; hi lo and lo hi, 2^-11 as large, have an accumulator of their own. Where results are rounded to 16 bits, one
+// accumulation takes the whole axis, and both sums are ready and read at the same time.
+//
+// Measured (fp32, five steps, the launches around the chain included): 4095 x 6001 in bf16 5.14 ms, 360 TFLOP/s of the
+// polynomial's and 1081 of the tensor core's products, 0.77 of a large library product under the same power limit; bound by
+// the MMAs (a stage takes 1516 cycles, its MMAs 1536 at the nominal rate) and by the last tiles of a product, for which
+// the other pairs wait. 2048 x 2048: 676 us, 254 TFLOP/s; fp32 sums leave the tensor core every 512 in K. Below about 1000 rows
+// the latencies of a product (barrier, first loads, one tile's way out: 12 to 15 us) count for more than its MMAs.
 enum Product { GRAM, POLY, STEP };
 constexpr int kWriters = 256;
 constexpr int kChainThreads = kWriters + 128;
@@ -550,10 +549,10 @@ __device__ __forceinline__ bool write_product(Product p, const Walk& w, ChainBar
         for (int kb = k0; kb < k1; kb += stages_per_chunk, ++n.chunk) {
             if (!warp_wait(&bar.ready, n.chunk & 1)) return false;
             tmem_fence_after();
-            // The mean of what the chunk's n = 4 additions per stage have lost. X X^T: measured 2.0 n 2^-25 where all terms have
-            // one sign (the diagonal), 0.7 n 2^-25 where signs are random; 1.3 leaves a third of either. A A and B X: one term,
-            // with the diagonal's element, is much larger than the others, and the half of the additions that follow it lose
-            // half a step each, 0.72 n 2^-25 over all mantissas.
+            // The mean of what the chunk's n = 4 additions per stage have lost, as measured against 64-bit sums: 2.0 n 2^-25 on the
+            // diagonal of X X^T, where all terms have one sign; 2.4 n 2^-25 on A A's, where most of a sum comes with one term;
+            // 0.7 n 2^-25 where signs are random (off the diagonals) or one term of B X, the diagonal's, outweighs the others
+            // (the half of the additions that follow it lose half a step each).
             const float loss = 0x1p-25f * 4.f * float(min(stages_per_chunk, k1 - kb));
             const float made_good = 1.f + 0.7f * loss, diagonal_good = 1.f + (p == GRAM ? 2.f : p == POLY ? 2.4f : 0.7f) * loss;
 #pragma unroll
@@ -869,23 +868,23 @@ __global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_co
 // One cluster per matrix. Each CTA keeps X for its share of the columns in shared memory over all steps; per step every CTA
 // adds up all shares of X X^T over distributed shared memory, forms P = a I + b A + c A A for itself and multiplies its own
 // columns with it in place. Nothing goes through global memory between the update's elements and the result, and the products
-// are fp32. Up to 16 rows; above, the shared memory's bandwidth binds (64 x 160: 49 us) and the tensor cores are faster.
+// are fp32. Up to 16 rows; above, the shared memory's bandwidth binds (64 x 160: 49 us in this form, 41 on the tensor cores).
+// What bounds it is the chain of latencies, five barriers a step (SHORT_FIG).
 constexpr int kShortThreads = 512;
 constexpr int kShortWarps = kShortThreads / 32;
 constexpr int kShortRows = 16;
 struct ClusterBatch {
     Matrix m[kMaxMatrices];
 };
-// Sizes for X padded to MP rows: 4 x 4 tiles on and below the diagonal of X X^T, and groups of threads that share its sums.
-__host__ __device__ constexpr int short_padded_rows(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+// Sizes for X padded to MP = 8 or 16 rows: 4 x 4 tiles on and below the diagonal of X X^T.
+__host__ __device__ constexpr int short_padded_rows(int rows) { return rows <= 8 ? 8 : 16; }
 __host__ __device__ constexpr int short_tiles(int mp) { return (mp / 4) * (mp / 4 + 1) / 2; }
 __host__ __device__ constexpr int short_packed(int mp) { return short_tiles(mp) * 16; }
-__host__ __device__ constexpr int short_groups(int mp) { return mp == 64 ? kShortThreads / short_tiles(64) : 1; }
 __host__ __device__ constexpr int short_columns(int cols, int ranks) { return ((cols + ranks - 1) / ranks + 3) & ~3; }
 __host__ __device__ constexpr int short_pitch(int columns) { return ((columns + 27) / 32) * 32 + 4; }    // = 4 mod 32 banks, >= columns
 __host__ __device__ constexpr size_t short_smem(int rows, int cols, int ranks) {
     const int mp = short_padded_rows(rows);
-    return size_t(mp * short_pitch(short_columns(cols, ranks)) + 2 * mp * (mp + 4) + (2 + short_groups(mp)) * short_packed(mp)) * sizeof(float);
+    return size_t(mp * short_pitch(short_columns(cols, ranks)) + 2 * mp * (mp + 4) + 2 * short_packed(mp)) * sizeof(float);
 }
 
 // Sums 16 values over the warp's lanes; returns the sum of value lane / 2 (both lanes of a pair hold it).
@@ -932,45 +931,19 @@ __device__ __forceinline__ void tile_place(int tile, int& ti, int& tj) {
 
 // X X^T packed: element (4 i + j) of tile t at (4 i + j) * tiles + t. Tile (ti, tj) holds rows ti + side i and columns
 // tj + side j, so that neighbouring tiles read neighbouring rows, which the pitch puts into different banks.
-// MP = 64: a thread per tile and group of columns, the groups' sums added through shared memory; smaller: a warp per tile,
-// its lanes share the columns. done(e, value) is called once for every packed element.
+// A warp per tile, its lanes share the columns. done(e, value) is called once for every packed element.
 template <int MP, typename Done>
-__device__ __forceinline__ void symmetric_product(const float* from, int pitch, int length, float* partial, Done&& done) {
-    constexpr int side = MP / 4, tiles = short_tiles(MP), packed = short_packed(MP), groups = short_groups(MP);
-    const int tid = threadIdx.x;
-    if constexpr (groups > 1) {
-        const int tile = tid % tiles, group = tid / tiles;
-        if (group < groups) {
-            int ti, tj;
-            tile_place(tile, ti, tj);
-            float acc[16] = {};
-            tile_product(acc, from + ti * pitch, from + tj * pitch, side * pitch, group * 4, groups * 4, length);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) partial[group * packed + i * tiles + tile] = acc[i];
-        }
-        __syncthreads();
-        constexpr int each = (packed + kShortThreads - 1) / kShortThreads;
-        float v[each];
-#pragma unroll
-        for (int i = 0; i < each; ++i) {
-            const int e = tid + i * kShortThreads;
-            v[i] = 0.f;
-#pragma unroll
-            for (int g = 0; g < groups; ++g) v[i] += e < packed ? partial[g * packed + e] : 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < each; ++i)
-            if (tid + i * kShortThreads < packed) done(tid + i * kShortThreads, v[i]);
-    } else {
-        const int lane = tid & 31;
-        for (int tile = tid >> 5; tile < tiles; tile += kShortWarps) {
-            int ti, tj;
-            tile_place(tile, ti, tj);
-            float acc[16] = {};
-            tile_product(acc, from + ti * pitch, from + tj * pitch, side * pitch, lane * 4, 128, length);
-            const float v = warp_sum16(acc, lane);
-            if ((lane & 1) == 0) done((lane >> 1) * tiles + tile, v);
-        }
+__device__ __forceinline__ void symmetric_product(const float* from, int pitch, int length, Done&& done) {
+    constexpr int side = MP / 4, tiles = short_tiles(MP);
+    static_assert(tiles <= kShortWarps, "a warp per tile");
+    const int lane = threadIdx.x & 31, tile = threadIdx.x >> 5;
+    if (tile < tiles) {
+        int ti, tj;
+        tile_place(tile, ti, tj);
+        float acc[16] = {};
+        tile_product(acc, from + ti * pitch, from + tj * pitch, side * pitch, lane * 4, 128, length);
+        const float v = warp_sum16(acc, lane);
+        if ((lane & 1) == 0) done((lane >> 1) * tiles + tile, v);
     }
 }
 // Packed element -> its places (row, column) and (column, row) in a matrix of the given pitch.
@@ -1035,7 +1008,6 @@ __device__ __forceinline__ void short_matrix(const Matrix& m, int ranks, int ran
     float* gram = x + MP * pitch;                // A
     float* poly = gram + MP * gp;                // P = a I + b A + c A A
     float* share = poly + MP * gp;               // the CTA's share of A, packed; two buffers in turn
-    float* partial = share + 2 * packed;
 
     for (int i = tid * 4; i < MP * pitch; i += kShortThreads * 4) *reinterpret_cast<float4*>(x + i) = make_float4(0.f, 0.f, 0.f, 0.f);
     __syncthreads();
@@ -1057,7 +1029,7 @@ __device__ __forceinline__ void short_matrix(const Matrix& m, int ranks, int ran
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
             const bool in = o < outer;
-            u[j] = in ? load_float<T>(m.update, (first_row + o) * m.update_stride + first + i) : 0.f;
+            u[j] = in ? float(static_cast<const T*>(m.update)[(first_row + o) * m.update_stride + first + i]) : 0.f;
             if constexpr (MUON) old[j] = in ? m.momentum[(first_row + o) * m.cols + first + i] : 0.f;
             next(o, i);
         }
@@ -1099,45 +1071,30 @@ __device__ __forceinline__ void short_matrix(const Matrix& m, int ranks, int ran
         v.x *= factor, v.y *= factor, v.z *= factor, v.w *= factor;
         *reinterpret_cast<float4*>(x + i) = v;
     }
-    // where this thread's elements of the packed sums go (the same in every step)
-    constexpr int each = (packed + kShortThreads - 1) / kShortThreads;
-    int at[each], mirror[each];
-#pragma unroll
-    for (int i = 0; i < each; ++i) packed_places<MP>(min(tid + i * kShortThreads, packed - 1), gp, at[i], mirror[i]);
+    // where this thread's element of the packed sums goes (the same in every step)
+    static_assert(packed <= kShortThreads, "one element per thread");
+    const bool has = tid < packed;
+    int at = 0, mirror = 0;
+    if (has) packed_places<MP>(tid, gp, at, mirror);
     __syncthreads();
 
     for (int step = 0; step < steps; ++step) {
         // A: every CTA adds up all shares in their order. A share's buffer is written again two steps, so one barrier, later.
         float* mine = share + (step & 1) * packed;
-        symmetric_product<MP>(x, pitch, columns, partial, [&](int e, float v) { mine[e] = v; });
+        symmetric_product<MP>(x, pitch, columns, [&](int e, float v) { mine[e] = v; });
         if (ranks > 1) cluster.sync();
         else __syncthreads();
-        float v[each];
+        if (has) {
+            float v = 0.f;
 #pragma unroll
-        for (int i = 0; i < each; ++i) v[i] = 0.f;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            if (q < ranks) {
-                const float* theirs = ranks > 1 ? cluster.map_shared_rank(mine, q) : mine;
-#pragma unroll
-                for (int i = 0; i < each; ++i) v[i] += theirs[min(tid + i * kShortThreads, packed - 1)];
-            }
+            for (int q = 0; q < 8; ++q)
+                if (q < ranks) v += (ranks > 1 ? cluster.map_shared_rank(mine, q) : mine)[tid];
+            gram[at] = gram[mirror] = v;
         }
-#pragma unroll
-        for (int i = 0; i < each; ++i)
-            if (tid + i * kShortThreads < packed) gram[at[i]] = gram[mirror[i]] = v[i];
         __syncthreads();
-        symmetric_product<MP>(gram, gp, MP, partial, [&](int e, float v) {
+        symmetric_product<MP>(gram, gp, MP, [&](int e, float v) {
             int a, b;
-            if constexpr (short_groups(MP) > 1) {
-                const int i = (e - tid) / kShortThreads;
-                a = b = 0;
-#pragma unroll
-                for (int j = 0; j < each; ++j)
-                    if (i == j) a = at[j], b = mirror[j];
-            } else {
-                packed_places<MP>(e, gp, a, b);
-            }
+            packed_places<MP>(e, gp, a, b);
             poly[a] = poly[b] = cb * gram[a] + cc * v + (a == b ? ca : 0.f);
         });
         __syncthreads();
@@ -1161,7 +1118,7 @@ __device__ __forceinline__ void short_matrix(const Matrix& m, int ranks, int ran
 // rows x 64 columns). Per step: X X^T of the CTA's columns; the shares are added up over distributed shared memory, CTA q
 // summing rows q MP / ranks .. and handing them to all as planes; B = b A + c A A in A's place, each CTA for itself;
 // X <- a X + B X in place. All accumulators are in tensor memory; additions per accumulator are few (128 in K), so that the
-// losses of the module comment stay small. What bounds it is the chain of latencies, about eight barriers a step.
+// losses of the module comment stay small. What bounds it is the chain of latencies, about eight barriers a step (MID_FIG).
 constexpr int kMidThreads = 512;
 constexpr int kMidWarps = kMidThreads / 32;
 __host__ __device__ constexpr int mid_rows(int rows) { return rows <= 64 ? 64 : 128; }
@@ -1769,24 +1726,6 @@ void describe(const gmc_matrix& g, Matrix& m) {
 }
 
 // One launch of clusters of `ranks` CTAs, one per matrix.
-template <typename Kernel, typename... Args>
-int launch_clusters(Kernel kernel, int n, int ranks, int threads, size_t smem, size_t smem_limit, cudaStream_t stream, const Args&... args) {
-    GMC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem_limit)));
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(unsigned(n * ranks));
-    config.blockDim = dim3(unsigned(threads));
-    config.dynamicSmemBytes = smem;
-    config.stream = stream;
-    cudaLaunchAttribute attribute;
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = unsigned(ranks);
-    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-    config.attrs = &attribute;
-    config.numAttrs = 1;
-    GMC_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, args...));
-    return GMC_OK;
-}
-
 template <typename T, bool MUON>
 int run_clusters(const gmc_matrix* matrices, const int* which, int n, int steps, float ca, float cb, float cc, const Polynomial& poly, float epsilon,
                  const Momentum& mo, cudaStream_t stream) {
@@ -1803,6 +1742,9 @@ int run_clusters(const gmc_matrix* matrices, const int* which, int n, int steps,
         // of the shares costs more than the products save (64 x 160: 41 us with one CTA, 49 with four)
         while (ranks < 8 && (!fits(rows, cols, ranks) || (cols > 256 * ranks && 2 * ranks * n <= n_sm))) ranks *= 2;
     }
+    // A CTA holds its multiprocessor's tensor memory: two clusters that shared two multiprocessors in different orders would wait
+    // for each other's. A CTA of a cluster therefore takes more than half of the shared memory.
+    if (ranks > 1) smem = 116 * 1024;
     for (int i = 0; i < n; ++i)
         smem = std::max(smem, cluster_smem(std::min(b.m[i].rows, b.m[i].cols), std::max(b.m[i].rows, b.m[i].cols), ranks));
     auto kernel = any_short ? cluster_kernel<T, MUON, true> : cluster_kernel<T, MUON, false>;

@@ -108,6 +108,8 @@ def muon_update(params: typing.Sequence[Tensor], grads: typing.Sequence[Tensor],
         if p.data_ptr() in seen or m.data_ptr() in seen:
             raise _native.GmcError("a parameter or momentum appears twice")
         seen.update((p.data_ptr(), m.data_ptr()))
+        if g.data_ptr() in (p.data_ptr(), m.data_ptr()):
+            raise _native.GmcError("a gradient must not share its memory with its parameter or momentum")
         if not g.is_contiguous():
             g = g.contiguous()
             held.append(g)

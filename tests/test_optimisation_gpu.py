@@ -64,7 +64,7 @@ def test_orthogonalise(m, n, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("m,n", [(8, 9000), (16, 513), (17, 300), (64, 4096), (64, 4097), (65, 1536), (128, 1536), (128, 1537), (2000, 100),
-                                 (129, 5000), (256, 6000), (6000, 250), (1500, 4100)])
+                                 (16, 32768), (32768, 3), (129, 5000), (256, 6000), (6000, 250), (1500, 4100)])
 def test_where_one_kernel_ends_and_the_next_begins(m, n, dtype):
     """Both sides of the shapes that decide between fp32 tiles, one cluster, and the whole GPU; columns shared out; long axes."""
     from gmc.optimisation import orthogonalise
@@ -204,6 +204,8 @@ def test_the_same_tensor_twice_is_refused():
     p, g, m = (torch.zeros(3, 4, device="cuda") for _ in range(3))
     with pytest.raises(GmcError, match="appears twice"):
         muon_update([p, p], [g, g], [m, m.clone()], 0.1)
+    with pytest.raises(GmcError, match="share its memory"):
+        muon_update([p], [m], [m], 0.1)
     with pytest.raises(GmcError, match="contiguous"):
         muon_update([p.t()], [g.t()], [m.t()], 0.1)
     with pytest.raises(GmcError, match="float32"):
@@ -298,6 +300,23 @@ def test_two_calls_at_once():
             got.append(orthogonalise(v))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_clusters_of_several_calls_at_once():
+    """Small clusters from several streams, more of them than fit side by side: none may wait for what another one holds."""
+    from gmc.optimisation import orthogonalise
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    u = [torch.randn(30, m, n, device="cuda", generator=gen) for m, n in ((64, 500), (40, 600), (100, 700), (12, 900))]
+    want = [orthogonalise(v) for v in u]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in u]
+    for _ in range(5):
+        got = []
+        for s, v in zip(streams, u):
+            with torch.cuda.stream(s):
+                got.append(orthogonalise(v))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_a_training_step_of_the_network():
