@@ -167,6 +167,9 @@ __device__ __forceinline__ void write_alternative(const Outputs& out, Key key, l
 }
 
 // ---- short rows: one warp per row, the row in registers ---------------------------------------------------------------
+// At most 1024 classes. Bound by one chain of latencies (launch, load, two reductions over the warp, stores): 5.3 us for one row
+// of 10 classes and for 256 rows of 40 with the caches cold, where the bytes alone would take 0.02 us. The alternatives are
+// found by n_top maxima over the warp, each below the one before.
 template <typename T, int E>
 __global__ void __launch_bounds__(kSmallThreads) forward_small_kernel(const T* __restrict__ logits, const long long* __restrict__ targets,
                                                                       long long n_rows, int n_classes, long long row_stride,
@@ -269,8 +272,15 @@ __device__ __forceinline__ int rank_among(const Key* keys, int n, Key key) {
 // Alternatives without a second look at most of the row. After the sums every thread knows its largest element; the n_top-th
 // largest of the 32 maxima of groups of eight threads is a value that at least n_top elements reach, and few more than that
 // do (about 30 for 20 of independent values). The threads whose maximum reaches it read their elements again and collect
-// those that do; a collected element's place is the number of larger ones. Where too many are equal (a constant row), the
+// those that do; a collected element's place is the number of larger ones (the order of the atomic additions that hand out the
+// collecting places does not matter). Where too many are equal (a constant row), the
 // warps go through all their elements and keep sorted lists instead.
+//
+// Bound by the memory where there are many rows: 4093 x 32003 in bf16 58 us, 4.5 TB/s, held below the copy's 6.5 by the two
+// exponential-unit and six other instructions per pair of classes (in fp32, half the classes per byte: 1021 x 100003 with
+// three alternatives 76 us, 5.4 TB/s); by latencies where there are few: one row of 50257 in bf16 over eight CTAs 10 us, of which
+// the cluster's launch and barriers, the reductions and the alternatives are 8; 64 rows of 131072 with 20 alternatives 16 us,
+// 1 TB/s. Four vectors in flight and four CTAs per multiprocessor: with more vectors the registers leave room for three.
 constexpr int kCollected = 512;
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kRowThreads, 4) forward_row_kernel(const T* __restrict__ logits, const long long* __restrict__ targets,
@@ -525,7 +535,9 @@ __global__ void __launch_bounds__(kSmallThreads) backward_small_kernel(const T* 
         given_class<T>(g, in, top_indices, z, dz, row, n_top, i, 0, n_classes, inv_t, k);
 }
 
-// Long rows: a CTA per stretch of kStretch vectors of a row.
+// Long rows: a CTA per stretch of kStretch vectors of a row. Bound by the memory, one read and one write: 4093 x 32003 in bf16
+// 91 us, 5.8 TB/s; 1021 x 100003 in fp32 135 us, 6.0 TB/s. Written past the caches (__stcs), which leaves the L2 cache to the
+// rows that the forward pass has read last.
 constexpr int kStretch = kRowThreads * kUnroll;
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads) backward_row_kernel(const T* __restrict__ logits, const long long* __restrict__ targets,
