@@ -10,6 +10,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace gmc {
@@ -25,6 +27,7 @@ constexpr int kUnroll = 4;               // 16-byte vectors a thread has in flig
 constexpr int kSmallThreads = 128;       // short rows: one warp per row, four rows per CTA
 constexpr int kSmallClasses = 1024;      // at most 32 elements per lane
 constexpr float kLowest = -1e20f;        // bound of x: e is 0 far above it for every temperature allowed, 0 * kLowest = -0
+constexpr float kNearLowest = -1e35f;    // z above it: z minus any finite 16-bit maximum stays in the fp32 range
 constexpr float kMinTemperature = 1e-6f, kMaxTemperature = 1e6f;
 
 __device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
@@ -55,6 +58,33 @@ template <typename T> __device__ __forceinline__ uint4 masked_vector();         
 template <> __device__ __forceinline__ uint4 masked_vector<float>() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
 template <> __device__ __forceinline__ uint4 masked_vector<__nv_bfloat16>() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
 template <> __device__ __forceinline__ uint4 masked_vector<__half>() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
+
+// Largest and smallest of a thread's vectors, NaN left out. 16-bit types are compared in pairs.
+template <typename T>
+__device__ __forceinline__ void extremes(const Vec<T> (&v)[kUnroll], float& largest, float& smallest) {
+    if constexpr (sizeof(T) == 2) {
+        using Pair = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+        Pair hi, lo;
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const Pair* p = reinterpret_cast<const Pair*>(&v[u].raw);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                hi = u + i == 0 ? p[0] : __hmax2(hi, p[i]);
+                lo = u + i == 0 ? p[0] : __hmin2(lo, p[i]);
+            }
+        }
+        largest = fmaxf(to_float<T>(hi.x), to_float<T>(hi.y));
+        smallest = fminf(to_float<T>(lo.x), to_float<T>(lo.y));
+    } else {
+        largest = v[0].at(0);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+            for (int i = 0; i < Vec<T>::N; ++i) largest = fmaxf(largest, v[u].at(i));
+        smallest = neg_inf();                                                       // comparing again would cost what the bound costs
+    }
+}
 
 // Order of the alternatives as one number: larger value first, then lower index. NaN ranks behind -inf; 0 is no element.
 __device__ __forceinline__ Key make_key(float z, unsigned index) {
@@ -106,12 +136,24 @@ __device__ __forceinline__ void add_element(float z, float base, float k, float&
     t += e * fmaxf(x, kLowest);
 }
 
-// Two elements at once: packed additions and products take one issue slot for both.
+// Two elements at once: packed additions and products take one issue slot for both. BOUND: x may be -inf.
+template <bool BOUND>
 __device__ __forceinline__ void add_pair(float2 z, float2 minus_base, float2 k, float2& s, float2& t) {
     const float2 x = __fadd2_rn(z, minus_base), y = __fmul2_rn(x, k);
     const float2 e = make_float2(ex2_approx(y.x), ex2_approx(y.y));
     s = __fadd2_rn(s, e);
-    t = __ffma2_rn(e, make_float2(fmaxf(x.x, kLowest), fmaxf(x.y, kLowest)), t);
+    t = __ffma2_rn(e, BOUND ? make_float2(fmaxf(x.x, kLowest), fmaxf(x.y, kLowest)) : x, t);
+}
+template <bool BOUND, typename T>
+__device__ __forceinline__ void add_vectors(const Vec<T> (&v)[kUnroll], float base, float k, Stat& st) {
+    float2 s = make_float2(0.f, 0.f), t = s;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+        for (int i = 0; i < Vec<T>::N; i += 2)
+            add_pair<BOUND>(make_float2(v[u].at(i), v[u].at(i + 1)), make_float2(-base, -base), make_float2(k, k), s, t);
+    st.s += s.x + s.y;
+    st.t += t.x + t.y;
 }
 
 struct Outputs {
@@ -276,11 +318,10 @@ __device__ __forceinline__ int rank_among(const Key* keys, int n, Key key) {
 // collecting places does not matter). Where too many are equal (a constant row), the
 // warps go through all their elements and keep sorted lists instead.
 //
-// Bound by the memory where there are many rows: 4093 x 32003 in bf16 58 us, 4.5 TB/s, held below the copy's 6.5 by the two
-// exponential-unit and six other instructions per pair of classes (in fp32, half the classes per byte: 1021 x 100003 with
-// three alternatives 76 us, 5.4 TB/s); by latencies where there are few: one row of 50257 in bf16 over eight CTAs 10 us, of which
-// the cluster's launch and barriers, the reductions and the alternatives are 8; 64 rows of 131072 with 20 alternatives 16 us,
-// 1 TB/s. Four vectors in flight and four CTAs per multiprocessor: with more vectors the registers leave room for three.
+// Many rows of 16-bit logits are bound by issue: 4093 x 32003 in bf16 57 us, 4.6 TB/s of the copy's 6.5, with 70 % of the issue
+// slots and 61 % of the exponential unit in use. fp32 has half the classes per byte: 1021 x 100003 with four alternatives 76 us,
+// 5.4 TB/s. Few rows are bound by latencies (launch of the cluster, first loads, three reductions, the alternatives): 64 rows of
+// 131072 in bf16 with eight alternatives 16 us, 1 TB/s; one row of 50257 with 20 alternatives 15 us with the caches cold.
 constexpr int kCollected = 512;
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kRowThreads, 4) forward_row_kernel(const T* __restrict__ logits, const long long* __restrict__ targets,
@@ -310,28 +351,19 @@ __global__ void __launch_bounds__(kRowThreads, 4) forward_row_kernel(const T* __
     Vec<T> next[kUnroll];                                                           // on its way while the last ones are added up
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) next[u] = r.load(r.first + tid + u * kRowThreads);
-    for (int at = r.first + tid; at < r.end; at += kRowThreads * kUnroll) {
+    for (int of_warp = r.first + warp * 32; of_warp < r.end; of_warp += kRowThreads * kUnroll) {
         Vec<T> v[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             v[u] = next[u];
-            next[u] = r.load(at + (kUnroll + u) * kRowThreads);
+            next[u] = r.load(of_warp + lane + (kUnroll + u) * kRowThreads);
         }
-        float m = v[0].at(0);
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-            for (int i = 0; i < N; ++i) m = fmaxf(m, v[u].at(i));
+        float m, least;
+        extremes<T>(v, m, least);
         if (m > st.m) raise(st, m, k);
-        const float minus_base = st.m == neg_inf() ? 0.f : -st.m;
-        float2 s2 = make_float2(0.f, 0.f), t2 = s2;
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-            for (int i = 0; i < N; i += 2)
-                add_pair(make_float2(v[u].at(i), v[u].at(i + 1)), make_float2(minus_base, minus_base), make_float2(k, k), s2, t2);
-        st.s += s2.x + s2.y;
-        st.t += t2.x + t2.y;
+        const float base = st.m == neg_inf() ? 0.f : st.m;
+        if (sizeof(T) == 2 && __all_sync(0xffffffffu, least > kNearLowest)) add_vectors<false, T>(v, base, k, st);
+        else add_vectors<true, T>(v, base, k, st);
     }
     if (has_tail) {
         const float z = to_float<T>(r.z[tail_first + tid]);

@@ -146,6 +146,26 @@ def test_masks(dtype, c):
     _check(z, t, min(c, 16))
 
 
+@pytest.mark.parametrize("others", [-3e38, -1e36, -2e35, -1e34, 0.0])
+def test_logits_at_both_ends_of_the_range(others):
+    """Two classes share a maximum of 3e38: probabilities 1/2 and 0 exactly (differences of 1e35 and more), so the entropy and the
+    target's log-probability are ln 2 to the three roundings of a logarithm and its products."""
+    from gmc.classification import log_probabilities
+    z = torch.full((3, 5000), others, device="cuda")
+    z[:, [7, 4001]] = 3e38
+    z = z.bfloat16().requires_grad_(True)
+    t = torch.full((3,), 4001, device="cuda")
+    r = log_probabilities(z, t, n_top=2)
+    ln2 = 0.6931471805599453
+    for v in (r.entropy, -r.target, -r.top[:, 0], -r.top[:, 1]):
+        assert (v.double() - ln2).abs().max() <= 4 * 2.0 ** -24
+    assert (r.top_indices == torch.tensor([7, 4001], device="cuda")).all()
+    (g,) = torch.autograd.grad(r.target.sum(), z)
+    want = torch.zeros_like(g)
+    want[:, 7], want[:, 4001] = -0.5, 0.5
+    assert (g.double() - want.double()).abs().max() <= 2.0 ** -9
+
+
 @pytest.mark.parametrize("c", [20, 1024, 1025, 70000])
 def test_nan_and_infinity_make_the_row_nan(c):
     from gmc.classification import log_probabilities
