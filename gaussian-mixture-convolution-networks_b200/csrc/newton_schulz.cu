@@ -447,7 +447,7 @@ __device__ __forceinline__ void fence_proxy_async_all() { asm volatile("fence.pr
 __device__ __forceinline__ void writers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWriters) : "memory"); }
 
 struct ChainBarriers {
-    uint64_t full[kStages], peer_full[kStages], empty[kStages], ready, drained, mixed_ready, mixed_drained, done;
+    uint64_t full[kStages], peer_full[kStages], empty[kStages], ready[2], drained[2], mixed_ready, mixed_drained, done;
 };
 
 // One lane polls for its warp.
@@ -457,9 +457,11 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, unsigned parity) {
     return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
-// Writers: the tiles of one product. `chunk`, `tile`, `k` count the chunks, tiles and stages since the launch.
+// Writers: the tiles of one product. `tile`, `k` count the tiles and stages since the launch, `phase` has a bit per place of a
+// chunk's sums. Narrow tiles leave 128 columns of tensor memory for a second place, taken by every other chunk of a tile, which
+// is summed up while the next one is multiplied; in a wide tile the MMAs wait for it (1400 cycles a chunk).
 struct WriterCounts {
-    unsigned chunk, tile, k;
+    unsigned phase, tile, k;
 };
 // 64 columns of a row in their place: v c1, plus c0 times what is there. The next chunk is read before this one is written,
 // which the compiler could not know to be safe.
@@ -524,9 +526,8 @@ __device__ __forceinline__ bool write_product(Product p, const Walk& w, ChainBar
             const bool shared_out = p == GRAM && w.splits > 1;
             const unsigned k = n.k + (wide ? warp >> 2 : 0), s = k % kStages;
             n.k += w.extra(p);
-            if (!warp_wait(&bar.ready, n.chunk & 1)) return false;
+            if (!warp_wait(&bar.ready[0], n.tile & 1)) return false;
             if (!shared_out && !warp_wait(&bar.full[s], (k / kStages) & 1)) return false;
-            ++n.chunk;
             tmem_fence_after();
             const float loss = 0x1p-25f * 4.f * float(k1 - k0), made_good = 1.f + 0.7f * loss;
             const float diagonal_good = 1.f + (p == GRAM ? 2.f : p == POLY ? 2.4f : 0.7f) * loss;
@@ -559,15 +560,17 @@ __device__ __forceinline__ bool write_product(Product p, const Walk& w, ChainBar
             }
             tmem_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_at(&bar.drained, 0);
+            if (lane == 0) mbar_arrive_at(&bar.drained[0], 0);
             if (!shared_out)
                 send_stage(to, 2 * ti + cta, (tj * 2 * half + (wide ? col0 : 0)) >> 6, stages + s * kStageBytes, &bar.empty[s], wide, warp, lane);
         } else {
         float sum[128];
 #pragma unroll
         for (int i = 0; i < 128; ++i) sum[i] = 0.f;
-        for (int kb = k0; kb < k1; kb += stages_per_chunk, ++n.chunk) {
-            if (!warp_wait(&bar.ready, n.chunk & 1)) return false;
+        unsigned place = 0;
+        for (int kb = k0; kb < k1; kb += stages_per_chunk, place ^= wide ? 0 : 1) {
+            if (!warp_wait(&bar.ready[place], (n.phase >> place) & 1)) return false;
+            n.phase ^= 1u << place;
             tmem_fence_after();
             // The mean of what the chunk's n = 4 additions per stage have lost, as measured against 64-bit sums: 2.0 n 2^-25 on the
             // diagonal of X X^T, where all terms have one sign; 2.4 n 2^-25 on A A's, where most of a sum comes with one term;
@@ -579,14 +582,14 @@ __device__ __forceinline__ bool write_product(Product p, const Walk& w, ChainBar
             for (int q = 0; q < 4; ++q) {
                 if (q < 2 || wide) {
                     float v[32];
-                    tmem_load32(tmem + lanes + col0 + q * 32, v);
+                    tmem_load32(tmem + place * 128 + lanes + col0 + q * 32, v);
 #pragma unroll
                     for (int i = 0; i < 32; ++i) sum[q * 32 + i] += v[i] * (q * 32 + i == diagonal ? diagonal_good : made_good);
                 }
             }
             tmem_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_at(&bar.drained, 0);
+            if (lane == 0) mbar_arrive_at(&bar.drained[place], 0);
         }
         if (!warp_wait(&bar.mixed_ready, n.tile & 1)) return false;
         tmem_fence_after();
@@ -698,9 +701,11 @@ __global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_co
             mbar_init(&bar.peer_full[s], 1);
             mbar_init(&bar.empty[s], 2);
         }
-        mbar_init(&bar.ready, WHOLE ? 2 : 1);                         // WHOLE: of both sums
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar.ready[i], WHOLE ? 2 : 1);                  // WHOLE: of both sums
+            mbar_init(&bar.drained[i], 2 * (kWriters / 32));
+        }
         mbar_init(&bar.mixed_ready, 1);
-        mbar_init(&bar.drained, 2 * (kWriters / 32));
         mbar_init(&bar.mixed_drained, 2 * (kWriters / 32));
         mbar_init(&bar.done, 2);
         fence_mbar_init();
@@ -788,13 +793,15 @@ __global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_co
         const bool mixed = tid == kWriters + 64;
         const uint32_t sums = mixed ? tmem_address + kMixedColumns : tmem_address;
         const int chunk_stages = m.chunk;
-        unsigned s = 0, phase = 0, peer_phase = 0, chunk = 0, tile = 0;                // peer_phase: one bit per stage
+        unsigned s = 0, phase = 0, peer_phase = 0, tile = 0;          // peer_phase: one bit per stage
+        unsigned used = 0, drained_phase = 0;                         // one bit per place of a chunk's sums
         const bool ok = each_product([&](Product p, int, unsigned) {
             const int groups_b = w.wide(p) ? 2 : 1;
             for (int u = w.pair; u < w.units(p); u += w.pairs, ++tile) {
                 int ti, tj, k0, k1;
                 w.unit(p, u, ti, tj, k0, k1);
                 int of_chunk = 0;
+                unsigned place = 0;
                 const int below_a = p == GRAM ? k1 : (ti + 1) * 4, below_b = p == GRAM ? k1 : p == STEP ? -1 : (tj * groups_b / 2 + 1) * 4;
                 for (int kb = k0; kb < k1; ++kb) {
                     const uint32_t a = smem_u32(stages + s * kStageBytes), bb = a + kBlockBytes;
@@ -808,9 +815,14 @@ __global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_co
                     peer_phase ^= 1u << s;
                     // sums that are about to be overwritten are read
                     if (mixed) {
-                        if (kb == k0 && tile > 0 && !mbar_wait_cluster(WHOLE ? &bar.drained : &bar.mixed_drained, (tile - 1) & 1)) return false;
-                    } else {
-                        if (of_chunk == 0 && chunk > 0 && !mbar_wait_cluster(&bar.drained, (chunk - 1) & 1)) return false;
+                        if (kb == k0 && tile > 0 && !mbar_wait_cluster(WHOLE ? &bar.drained[0] : &bar.mixed_drained, (tile - 1) & 1)) return false;
+                    } else if (of_chunk == 0) {
+                        if (!WHOLE && groups_b == 1 && kb > k0) place ^= 1;
+                        if ((used >> place) & 1) {
+                            if (!mbar_wait_cluster(&bar.drained[place], (drained_phase >> place) & 1)) return false;
+                            drained_phase ^= 1u << place;
+                        }
+                        used |= 1u << place;
                     }
                     tmem_fence_after();
                     if (mixed) {
@@ -821,14 +833,13 @@ __global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_co
                         }
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) mma_f16(sums, a_hi + i * step_a, b_hi + i * step_b, instruction, of_chunk > 0 || i > 0);
+                        for (int i = 0; i < 4; ++i) mma_f16(sums + place * 128, a_hi + i * step_a, b_hi + i * step_b, instruction, of_chunk > 0 || i > 0);
                     }
                     mma_commit(&bar.empty[s]);
                     if (mixed) {
-                        if (kb == k1 - 1) mma_commit(WHOLE ? &bar.ready : &bar.mixed_ready);
+                        if (kb == k1 - 1) mma_commit(WHOLE ? &bar.ready[0] : &bar.mixed_ready);
                     } else if (of_chunk == chunk_stages - 1 || kb == k1 - 1) {
-                        mma_commit(&bar.ready);
-                        ++chunk;
+                        mma_commit(&bar.ready[place]);
                     }
                     if (++of_chunk == chunk_stages) of_chunk = 0;
                     if (++s == kStages) s = 0, phase ^= 1;
