@@ -1528,9 +1528,9 @@ int ceil_div(long long a, long long b) { return int((a + b - 1) / b); }
 
 // Cycles of a product with a number of pairs, for the choice of tiles and pairs: measured per 64 in K 1520 cycles at 256
 // columns (the MMAs' own time is 1536) and 1440 at 128 (the barriers' latencies, behind the operands' traffic in shared
-// memory); a tile costs about 8000 and 6000 more to start and to write.
-long long product_cycles(long long tiles, int wide, long long k_blocks, int pairs) {
-    return (tiles + pairs - 1) / pairs * (wide ? 1520 * k_blocks + 8000 : 1440 * k_blocks + 6000);
+// memory); a tile costs about 8000 and 6000 more to start and to write, and a wide one 1400 for each further chunk.
+long long product_cycles(long long tiles, int wide, long long k_blocks, int pairs, int chunk) {
+    return (tiles + pairs - 1) / pairs * (wide ? 1520 * k_blocks + 8000 + (k_blocks - 1) / chunk * 1400 : 1440 * k_blocks + 6000);
 }
 long long step_tiles(const Matrix& m, int wide) { return (long long)((m.row_tiles + 1) / 2) * ((m.col_blocks + (wide ? 3 : 1)) / (wide ? 4 : 2)); }
 
@@ -1544,15 +1544,15 @@ long long plan(Matrix& m, int pairs) {
         for (int splits = 1; splits <= 32; splits *= 2) {
             if (splits > 1 && (tiles * splits > pairs || m.col_blocks < 4 * splits)) break;
             const long long reduce = splits > 1 ? 22000 + 400 * splits * ((tiles * (wide ? 64 : 32) + pairs * 16 - 1) / (pairs * 16)) : 0;
-            const long long t = product_cycles(tiles * splits, wide, m.col_blocks / splits, pairs) + reduce;
+            const long long t = product_cycles(tiles * splits, wide, m.col_blocks / splits, pairs, m.chunk) + reduce;
             if (best < 0 || t < best) best = t, m.gram_wide = wide, m.splits = splits;
         }
     }
     total += best;
-    const long long p0 = product_cycles(symmetric_tiles(m.row_tiles, 0), 0, 2 * m.row_tiles, pairs);
-    const long long p1 = product_cycles(symmetric_tiles(m.row_tiles, 1), 1, 2 * m.row_tiles, pairs);
+    const long long p0 = product_cycles(symmetric_tiles(m.row_tiles, 0), 0, 2 * m.row_tiles, pairs, m.chunk);
+    const long long p1 = product_cycles(symmetric_tiles(m.row_tiles, 1), 1, 2 * m.row_tiles, pairs, m.chunk);
     m.poly_wide = p1 <= p0;
-    const long long s0 = product_cycles(step_tiles(m, 0), 0, 2 * m.row_tiles, pairs), s1 = product_cycles(step_tiles(m, 1), 1, 2 * m.row_tiles, pairs);
+    const long long s0 = product_cycles(step_tiles(m, 0), 0, 2 * m.row_tiles, pairs, m.chunk), s1 = product_cycles(step_tiles(m, 1), 1, 2 * m.row_tiles, pairs, m.chunk);
     m.step_wide = s1 <= s0;
     return total + (p1 <= p0 ? p1 : p0) + (s1 <= s0 ? s1 : s0) + barrier;
 }
