@@ -358,8 +358,8 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Bat
 // Measured (fp32, five steps, the launches around the chain included): 4095 x 6001 in bf16 5.14 ms, 360 TFLOP/s of the
 // polynomial's and 1081 of the tensor core's products, 0.77 of a large library product under the same power limit; bound by
 // the MMAs (a stage takes 1516 cycles, its MMAs 1536 at the nominal rate) and by the last tiles of a product, for which
-// the other pairs wait. 2048 x 2048: 676 us, 254 TFLOP/s; fp32 sums leave the tensor core every 512 in K. Below about 1000 rows
-// the latencies of a product (barrier, first loads, one tile's way out: 12 to 15 us) count for more than its MMAs.
+// the other pairs wait. 2048 x 2048: 679 us, 253 TFLOP/s; fp32 sums leave the tensor core every 512 in K. Below about 1000 rows
+// the latencies of a product (barrier, first loads, one tile's way out: 11 to 13 us) count for more than its MMAs.
 enum Product { GRAM, POLY, STEP };
 constexpr int kWriters = 256;
 constexpr int kChainThreads = kWriters + 128;
