@@ -450,11 +450,17 @@ struct ChainBarriers {
     uint64_t full[kStages], peer_full[kStages], empty[kStages], ready[2], drained[2], mixed_ready, mixed_drained, done;
 };
 
-// One lane polls for its warp.
+// One lane polls for its warp. What it has acquired holds for the other lanes from the barrier on; a shuffle alone orders no
+// memory, and they go on to read what other threads, or copies, have written.
+__device__ __forceinline__ bool to_warp(bool ok) {
+    const int all = __shfl_sync(0xffffffffu, int(ok), 0);
+    __syncwarp();
+    return all != 0;
+}
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, unsigned parity) {
-    int ok = 1;
+    bool ok = true;
     if ((threadIdx.x & 31) == 0) ok = mbar_wait_bounded(bar, parity);
-    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+    return to_warp(ok);
 }
 
 // Writers: the tiles of one product. `tile`, `k` count the tiles and stages since the launch, `phase` has a bit per place of a
@@ -864,9 +870,9 @@ __global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_co
             if (tid == 0) asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(counter) : "memory");
         };
         auto wait = [&](unsigned arrivals) {                          // the warp goes on when its first lane has seen the counter
-            int ok = 1;
+            bool ok = true;
             if ((tid & 31) == 0) ok = wait_counter(counter, arrivals * ctas);
-            return __shfl_sync(0xffffffffu, ok, 0) != 0;
+            return to_warp(ok);
         };
         const uint32_t tmem = tmem_address;
         const bool ok = each_product([&](Product p, int from_x, unsigned before) {

@@ -302,6 +302,19 @@ def test_two_calls_at_once():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(200, 20000), (300, 6000), (6, 400, 1500), (513, 769)])
+def test_repeated_calls_are_identical(shape, dtype):
+    """Sums of X X^T that several CTAs share are read back by others in every step: the same bits call after call, with other
+    values in the workspace in between."""
+    from gmc.optimisation import orthogonalise
+    u, other = _update(*shape, seed=1, dtype=dtype), _update(*shape, seed=2, dtype=dtype)
+    want = orthogonalise(u)
+    for _ in range(10):
+        orthogonalise(other)
+        assert torch.equal(orthogonalise(u), want)
+
+
 def test_clusters_of_several_calls_at_once():
     """Small clusters from several streams, more of them than fit side by side: none may wait for what another one holds."""
     from gmc.optimisation import orthogonalise
