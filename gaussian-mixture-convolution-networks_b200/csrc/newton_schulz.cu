@@ -62,6 +62,7 @@ struct Batch {
     float* partial;             // tiles of X X^T over shares of the columns
     unsigned* arrived;          // one counter per matrix, then the failure flag
     int norm_ctas, pairs, blocks;
+    int lost_wait;              // writing warp of the launch whose first wait counts as run out (a test's), or -1
 };
 struct Momentum {
     float beta, one_minus_beta;
@@ -513,10 +514,13 @@ __device__ __forceinline__ void send_stage(const Planes& to, int row_block, int 
     __syncwarp();
 }
 
-// WHOLE: one accumulation takes the whole axis.
+// WHOLE: one accumulation takes the whole axis. `ok` becomes false when a wait runs out. The warp then goes on without
+// waiting: the others meet it at barriers that know no limit, and every access stays where it belongs. The result is
+// given up for NaN at the end.
 template <bool WHOLE>
-__device__ __forceinline__ bool write_product(Product p, const Walk& w, ChainBarriers& bar, uint8_t* stages, uint32_t tmem, int cta,
-                                              WriterCounts& n, const Planes& to, float c0, float c1, int stages_per_chunk, float* partial) {
+__device__ __forceinline__ void write_product(Product p, const Walk& w, ChainBarriers& bar, uint8_t* stages, uint32_t tmem, int cta,
+                                              WriterCounts& n, const Planes& to, float c0, float c1, int stages_per_chunk, float* partial,
+                                              bool& ok) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
     const int wide = w.wide(p), half = wide ? 128 : 64, col0 = (warp >> 2) * half;
@@ -532,8 +536,8 @@ __device__ __forceinline__ bool write_product(Product p, const Walk& w, ChainBar
             const bool shared_out = p == GRAM && w.splits > 1;
             const unsigned k = n.k + (wide ? warp >> 2 : 0), s = k % kStages;
             n.k += w.extra(p);
-            if (!warp_wait(&bar.ready[0], n.tile & 1)) return false;
-            if (!shared_out && !warp_wait(&bar.full[s], (k / kStages) & 1)) return false;
+            ok = ok && warp_wait(&bar.ready[0], n.tile & 1);
+            if (!shared_out) ok = ok && warp_wait(&bar.full[s], (k / kStages) & 1);
             tmem_fence_after();
             const float loss = 0x1p-25f * 4.f * float(k1 - k0), made_good = 1.f + 0.7f * loss;
             const float diagonal_good = 1.f + (p == GRAM ? 2.f : p == POLY ? 2.4f : 0.7f) * loss;
@@ -575,7 +579,7 @@ __device__ __forceinline__ bool write_product(Product p, const Walk& w, ChainBar
         for (int i = 0; i < 128; ++i) sum[i] = 0.f;
         unsigned place = 0;
         for (int kb = k0; kb < k1; kb += stages_per_chunk, place ^= wide ? 0 : 1) {
-            if (!warp_wait(&bar.ready[place], (n.phase >> place) & 1)) return false;
+            ok = ok && warp_wait(&bar.ready[place], (n.phase >> place) & 1);
             n.phase ^= 1u << place;
             tmem_fence_after();
             // The mean of what the chunk's n = 4 additions per stage have lost, as measured against 64-bit sums: 2.0 n 2^-25 on the
@@ -597,7 +601,7 @@ __device__ __forceinline__ bool write_product(Product p, const Walk& w, ChainBar
             __syncwarp();
             if (lane == 0) mbar_arrive_at(&bar.drained[place], 0);
         }
-        if (!warp_wait(&bar.mixed_ready, n.tile & 1)) return false;
+        ok = ok && warp_wait(&bar.mixed_ready, n.tile & 1);
         tmem_fence_after();
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -623,13 +627,12 @@ __device__ __forceinline__ bool write_product(Product p, const Walk& w, ChainBar
         // the stages behind the tile's: two blocks each. Wide: warps 0-3 have the first one's, warps 4-7 the second one's.
         const unsigned k = n.k + (wide ? warp >> 2 : 0), s = k % kStages;
         n.k += wide ? 2 : 1;
-        if (!warp_wait(&bar.full[s], (k / kStages) & 1)) return false;
+        ok = ok && warp_wait(&bar.full[s], (k / kStages) & 1);
         place_block(sum, stages + s * kStageBytes + (wide ? 0 : warp >> 2) * kBlockBytes + (warp & 3) * kWarpRows, p != GRAM, c0, c1, lane);
         if (wide) place_block(sum + 64, stages + s * kStageBytes + kBlockBytes + (warp & 3) * kWarpRows, p != GRAM, c0, c1, lane);
         send_stage(to, 2 * ti + cta, (tj * 2 * half + (wide ? col0 : 0)) >> 6, stages + s * kStageBytes, &bar.empty[s], wide, warp, lane);
         }
     }
-    return true;
 }
 
 // Writers: adds up the shares of X X^T, 32 rows x 32 columns per warp at a time, in the shares' order.
@@ -722,6 +725,8 @@ __global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_co
     tmem_fence_after();
 
     // For each product in turn: f(product, X's buffer, arrivals on the counter that its inputs need). Stops when f fails.
+    // The threads that load and multiply stop, each for itself: nothing waits for them without a limit but the end. The
+    // writers do not (write_product).
     auto each_product = [&](auto&& f) {
         for (int step = 0; step < steps; ++step) {
 #pragma unroll 1                                                      // one copy of the code: three do not fit the instruction cache
@@ -875,16 +880,18 @@ __global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_co
             return to_warp(ok);
         };
         const uint32_t tmem = tmem_address;
-        const bool ok = each_product([&](Product p, int from_x, unsigned before) {
+        bool ok = int(blockIdx.x) * (kWriters / 32) + warp != b.lost_wait;
+        if (!ok && (tid & 31) == 0) report_check(CHECK_MBARRIER_TIMEOUT);
+        each_product([&](Product p, int from_x, unsigned before) {
             // a pair without tiles in a product must not arrive for the next one early: the counter has no names
-            if (!wait(before)) return false;
+            ok = ok && wait(before);
             const Planes& to = p == STEP ? w.x(from_x ^ 1) : p == POLY || poly.linear ? w.poly : w.gram;
             const float c0 = p == STEP ? poly.step_from : p == POLY ? poly.poly_from : 0.f;
             const float c1 = p == STEP ? poly.step_factor : p == POLY ? poly.poly_factor : poly.gram_factor;
-            if (!write_product<WHOLE>(p, w, bar, stages, tmem, cta, n, to, c0, c1, m.chunk, partial)) return false;
+            write_product<WHOLE>(p, w, bar, stages, tmem, cta, n, to, c0, c1, m.chunk, partial, ok);
             if (p == GRAM && w.splits > 1) {
                 arrive(true);
-                if (!wait(before + 1)) return false;
+                ok = ok && wait(before + 1);
                 reduce_gram(w, cta, partial, to, c1);
             }
             arrive(p == GRAM && w.splits > 1);
@@ -1804,7 +1811,7 @@ int run_clusters(const gmc_matrix* matrices, const int* which, int n, int steps,
 
 template <typename T, bool MUON>
 int run_typed(const gmc_matrix* matrices, int n, int steps, float ca, float cb, float cc, const Polynomial& poly, float epsilon, const Momentum& mo,
-              void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+              void* workspace, size_t workspace_bytes, cudaStream_t stream, int lost_wait) {
     int which[kMaxMatrices], count = 0;
     for (int kind = 0; kind < KINDS; ++kind) {
         for (int i = 0; i <= n; ++i) {
@@ -1819,6 +1826,7 @@ int run_typed(const gmc_matrix* matrices, int n, int steps, float ca, float cb, 
                     if (int s = chain_pairs(&pairs)) return s;
                     fill(matrices, which, count, pairs, std::is_same<T, float>::value, &b, &bytes, static_cast<uint8_t*>(workspace));
                     if (bytes > workspace_bytes) return GMC_ERR_WORKSPACE;
+                    b.lost_wait = lost_wait;
                     if (int s = run_batch<T, MUON>(b, steps, poly, epsilon, mo, stream)) return s;
                 }
                 count = 0;
@@ -1846,7 +1854,7 @@ size_t workspace_bytes_of(const gmc_matrix* matrices, int n) {
 
 template <bool MUON>
 int run(const gmc_matrix* matrices, int n, int dtype, int steps, float ca, float cb, float cc, float epsilon, const Momentum& mo,
-        void* workspace, size_t workspace_bytes, void* stream) {
+        void* workspace, size_t workspace_bytes, void* stream, int lost_wait = -1) {
     if (int s = check_matrices(matrices, n)) return s;
     if (dtype < GMC_FLOAT32 || dtype > GMC_FLOAT16) return GMC_ERR_UNSUPPORTED;
     if (!(epsilon >= 1e-30f && epsilon <= 1e30f)) return GMC_ERR_UNSUPPORTED;
@@ -1859,9 +1867,9 @@ int run(const gmc_matrix* matrices, int n, int dtype, int steps, float ca, float
     if (need > 0 && !workspace) return GMC_ERR_NULL_POINTER;
     if (need > workspace_bytes) return GMC_ERR_WORKSPACE;
     cudaStream_t cs = as_stream(stream);
-    if (dtype == GMC_FLOAT32) return run_typed<float, MUON>(matrices, n, steps, ca, cb, cc, poly, epsilon, mo, workspace, workspace_bytes, cs);
-    if (dtype == GMC_BFLOAT16) return run_typed<__nv_bfloat16, MUON>(matrices, n, steps, ca, cb, cc, poly, epsilon, mo, workspace, workspace_bytes, cs);
-    return run_typed<__half, MUON>(matrices, n, steps, ca, cb, cc, poly, epsilon, mo, workspace, workspace_bytes, cs);
+    if (dtype == GMC_FLOAT32) return run_typed<float, MUON>(matrices, n, steps, ca, cb, cc, poly, epsilon, mo, workspace, workspace_bytes, cs, lost_wait);
+    if (dtype == GMC_BFLOAT16) return run_typed<__nv_bfloat16, MUON>(matrices, n, steps, ca, cb, cc, poly, epsilon, mo, workspace, workspace_bytes, cs, lost_wait);
+    return run_typed<__half, MUON>(matrices, n, steps, ca, cb, cc, poly, epsilon, mo, workspace, workspace_bytes, cs, lost_wait);
 }
 
 }  // namespace
@@ -1879,6 +1887,12 @@ extern "C" int gmc_orthogonalise(const gmc_matrix* matrices, int n_matrices, int
                                  float epsilon, void* workspace, size_t workspace_bytes, void* stream) {
     const gmc::Momentum none = {0.f, 1.f, 0, 1.f};
     return gmc::run<false>(matrices, n_matrices, dtype, steps, a, b, c, epsilon, none, workspace, workspace_bytes, stream);
+}
+
+extern "C" int gmc_debug_orthogonalise_lost_wait(const gmc_matrix* matrices, int n_matrices, int dtype, int steps, float a, float b, float c,
+                                                 float epsilon, void* workspace, size_t workspace_bytes, int lost_wait, void* stream) {
+    const gmc::Momentum none = {0.f, 1.f, 0, 1.f};
+    return gmc::run<false>(matrices, n_matrices, dtype, steps, a, b, c, epsilon, none, workspace, workspace_bytes, stream, lost_wait);
 }
 
 extern "C" int gmc_muon_update(const gmc_matrix* matrices, int n_matrices, int dtype, int steps, float a, float b, float c,

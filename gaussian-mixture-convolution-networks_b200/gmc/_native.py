@@ -91,6 +91,8 @@ lib.gmc_orthogonalise_workspace_bytes.restype = ctypes.c_size_t
 lib.gmc_orthogonalise_workspace_bytes.argtypes = [_c_void_p, _c_int]
 _declare("gmc_orthogonalise", [_c_void_p] + [_c_int] * 3 + [ctypes.c_float] * 4
          + [_c_void_p, ctypes.c_size_t, _c_void_p])
+_declare("gmc_debug_orthogonalise_lost_wait", [_c_void_p] + [_c_int] * 3 + [ctypes.c_float] * 4
+         + [_c_void_p, ctypes.c_size_t, _c_int, _c_void_p])
 _declare("gmc_muon_update", [_c_void_p] + [_c_int] * 3 + [ctypes.c_float] * 5 + [_c_int, ctypes.c_float]
          + [_c_void_p, ctypes.c_size_t, _c_void_p])
 

@@ -393,6 +393,11 @@ typedef struct gmc_matrix {
 size_t gmc_orthogonalise_workspace_bytes(const gmc_matrix* matrices, int n_matrices);
 int gmc_orthogonalise(const gmc_matrix* matrices, int n_matrices, int dtype, int steps, float a, float b, float c, float epsilon,
                       void* workspace, size_t workspace_bytes, void* stream);
+/* Diagnostic: gmc_orthogonalise in which the first wait of one warp of the cooperative launch (CTA * 8 + 0 .. 7) counts as run
+ * out, for testing what happens then. The launch ends, the results of its matrices are NaN and the check word gets bit 1;
+ * the context stays usable. */
+int gmc_debug_orthogonalise_lost_wait(const gmc_matrix* matrices, int n_matrices, int dtype, int steps, float a, float b, float c,
+                                      float epsilon, void* workspace, size_t workspace_bytes, int lost_wait, void* stream);
 int gmc_muon_update(const gmc_matrix* matrices, int n_matrices, int dtype, int steps, float a, float b, float c, float epsilon,
                     float momentum, int nesterov, float decay, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -315,6 +315,29 @@ def test_repeated_calls_are_identical(shape, dtype):
         assert torch.equal(orthogonalise(u), want)
 
 
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("m,n", [(200, 20000), (300, 700), (1500, 4100)])
+def test_a_wait_that_runs_out_gives_nan_and_an_error(m, n, dtype):
+    """One warp's first wait counts as run out, early and late in the grid, in tiles of either width and with shared sums: the
+    other warps, which have seen what it has not, still meet it at every barrier, and the launch ends by itself."""
+    from gmc import _native
+    from gmc.optimisation import orthogonalise
+    u = _update(m, n, seed=1, dtype=DTYPES[dtype])
+    out = torch.zeros_like(u)
+    packed = _native.matrix_struct.pack(u.data_ptr(), 0, out.data_ptr(), m, n, n, n, 0.0)
+    size = _native.lib.gmc_orthogonalise_workspace_bytes(packed, 1)
+    hold = torch.empty(size + 1024, dtype=torch.uint8, device="cuda")
+    address = (hold.data_ptr() + 1023) // 1024 * 1024
+    assert _native.device_check_word() == 0
+    for lost in (0, 5, 8 + 2, 8 * 3 + 7):
+        assert _native.lib.gmc_debug_orthogonalise_lost_wait(packed, 1, dtype, 5, *COEFFICIENTS, 1e-7, address, size, lost,
+                                                             _native.stream_of(u)) == 0
+        assert _native.device_check_word() == 1
+        assert out.isnan().all()
+    _check(orthogonalise(u), u)
+    assert _native.device_check_word() == 0
+
+
 def test_clusters_of_several_calls_at_once():
     """Small clusters from several streams, more of them than fit side by side: none may wait for what another one holds."""
     from gmc.optimisation import orthogonalise
