@@ -36,6 +36,8 @@ constexpr int kStageBytes = 2 * kBlockBytes;     // both operands, 64 wide in K
 constexpr int kStages = 3;
 constexpr int kWarpRows = kBlockBytes / 4;       // a writing warp's 32 rows of a block
 constexpr int kChainSmem = kStages * kStageBytes + 1024;
+constexpr int kWholeAxis = 1 << 20;              // Matrix::chunk: one accumulation, whatever the axis
+constexpr int kWholeStages = 32, kLongChunk = 16;    // 16-bit results: the longest such axis, and the chunk beyond it
 constexpr float kScaleX = 32768.f;               // |X| stays below 1.8, the largest fp16 number is 65504
 constexpr int kNormElements = 4096;              // elements of a matrix per CTA of the norm
 
@@ -62,6 +64,7 @@ struct Batch {
     float* partial;             // tiles of X X^T over shares of the columns
     unsigned* arrived;          // one counter per matrix, then the failure flag
     int norm_ctas, pairs, blocks;
+    bool whole;                 // every matrix has chunk = kWholeAxis
     int lost_wait;              // writing warp of the launch whose first wait counts as run out (a test's), or -1
 };
 struct Momentum {
@@ -353,8 +356,8 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Bat
 // The tensor core adds into its fp32 accumulator without rounding to nearest: the sums fall short by about n 2^-24 of
 // themselves after n additions. For fp32 results hi hi is therefore accumulated over two to eight stages (128 to 512 in K,
 // 8 to 32 additions, by the matrix's size) only and then added to registers, while other MMAs run, with the mean of the loss
-// made good; hi lo and lo hi, 2^-11 as large, have an accumulator of their own. Where results are rounded to 16 bits, one
-// accumulation takes the whole axis, and both sums are ready and read at the same time.
+// made good; hi lo and lo hi, 2^-11 as large, have an accumulator of their own. Where results are rounded to 16 bits and no
+// sum is longer than 2048, one accumulation takes the whole axis, and both sums are ready and read at the same time.
 //
 // Measured (fp32, five steps, the launches around the chain included): 4095 x 6001 in bf16 5.14 ms, 360 TFLOP/s of the
 // polynomial's and 1081 of the tensor core's products, 0.77 of a large library product under the same power limit; bound by
@@ -1577,15 +1580,30 @@ long long most_units(const Matrix& m) {
     return gram > step ? gram : step;
 }
 
+// Stages of the longest sum among a matrix's products.
+int longest_sum(const Matrix& m) { return std::max(2 * m.row_tiles, ceil_div(m.col_blocks, m.splits)); }
+
+// Hands out `pairs` CTA pairs: one each, the others to whoever takes longest.
+void hand_out(Batch& b, int pairs) {
+    long long cycles[kMaxMatrices];
+    for (int i = 0; i < b.n; ++i) cycles[i] = plan(b.m[i], 1);
+    for (int left = pairs - b.n; left > 0; --left) {
+        int most = -1;
+        for (int i = 0; i < b.n; ++i)
+            if (b.m[i].pairs < most_units(b.m[i]) && (most < 0 || cycles[i] > cycles[most])) most = i;
+        if (most < 0) break;
+        cycles[most] = plan(b.m[most], b.m[most].pairs + 1);
+    }
+}
+
 void describe(const gmc_matrix& g, Matrix& m);
 
-// Lays out the workspace and hands out `pairs` CTA pairs: one each, the others to whoever takes longest.
+// Lays out the workspace and hands out the pairs.
 void fill(const gmc_matrix* matrices, const int* which, int n, int pairs, bool fp32, Batch* batch, size_t* bytes, uint8_t* workspace) {
     Batch& b = *batch;
     b.n = n;
     long long x_blocks = 0, gram_blocks = 0, partials = 0;
     b.norm_ctas = b.blocks = 0;
-    long long cycles[kMaxMatrices];
     for (int i = 0; i < n; ++i) {
         const gmc_matrix& g = matrices[which[i]];
         Matrix& m = b.m[i];
@@ -1594,9 +1612,8 @@ void fill(const gmc_matrix* matrices, const int* which, int n, int pairs, bool f
         m.row_tiles = ceil_div(wide_rows, 128);
         m.col_blocks = 2 * ceil_div(wide_cols, 128);
         // fp32 results: against the plain fp32 evaluation's error, 256 x 4000 has 1.2 times with two stages and 2.3 with four,
-        // 700 x 2000 0.9 with four and 1.6 with eight, 2048 x 2048 0.7 with eight and the time is 810, 720 and 680 us; 16-bit
-        // results: the whole axis, 5e-5 of the result at 2048 against half a step of 2^-9 or 2^-12
-        m.chunk = !fp32 ? 1 << 20 : wide_rows <= 512 ? 2 : wide_rows <= 1024 ? 4 : 8;
+        // 700 x 2000 0.9 with four and 1.6 with eight, 2048 x 2048 0.7 with eight and the time is 810, 720 and 680 us
+        m.chunk = !fp32 ? kWholeAxis : wide_rows <= 512 ? 2 : wide_rows <= 1024 ? 4 : 8;
         m.norm_first = b.norm_ctas;
         m.block_first = b.blocks;
         m.x_block = x_blocks;
@@ -1606,14 +1623,17 @@ void fill(const gmc_matrix* matrices, const int* which, int n, int pairs, bool f
         b.blocks += int(blocks);
         x_blocks += blocks;
         gram_blocks += 2LL * m.row_tiles * m.row_tiles;
-        cycles[i] = plan(m, 1);
     }
-    for (int left = pairs - n; left > 0; --left) {
-        int most = -1;
-        for (int i = 0; i < n; ++i)
-            if (b.m[i].pairs < most_units(b.m[i]) && (most < 0 || cycles[i] > cycles[most])) most = i;
-        if (most < 0) break;
-        cycles[most] = plan(b.m[most], b.m[most].pairs + 1);
+    hand_out(b, pairs);
+    // 16-bit results: one accumulation per sum while none is longer than 2048. The error before the last rounding is then 4e-6 to 2e-5
+    // of the result (0.9 to 4 times the plain fp32 evaluation's; half a step is 2e-3 or 2.4e-4) and grows with the length
+    // beyond: 4.8e-5 at 4095 x 6001, 8.7e-5 at 16384 x 32768 (random signs). In chunks of 1024 it is 1.4e-5 and 5e-6, and the
+    // time 5.55 ms for 5.17 and 455 ms for 443; chunks of 2048 would take 5.42 ms for 2.7e-5, of 512 5.75 ms for 7e-6.
+    b.whole = !fp32;
+    for (int i = 0; i < n; ++i) b.whole = b.whole && longest_sum(b.m[i]) <= kWholeStages;
+    if (!fp32 && !b.whole) {
+        for (int i = 0; i < n; ++i) b.m[i].chunk = kLongChunk;
+        hand_out(b, pairs);
     }
     b.pairs = 0;
     bool splittable = false;
@@ -1738,9 +1758,9 @@ int run_batch(const Batch& b, int steps, const Polynomial& poly, float epsilon, 
     attributes[1].val.cooperative = 1;
     config.attrs = attributes;
     config.numAttrs = 2;
-    constexpr bool whole = !std::is_same<T, float>::value;
-    GMC_CUDA_TRY(cudaFuncSetAttribute(chain_kernel<whole>, cudaFuncAttributeMaxDynamicSharedMemorySize, kChainSmem));
-    GMC_CUDA_TRY(cudaLaunchKernelEx(&config, chain_kernel<whole>, b, steps, poly));
+    auto chain = b.whole ? chain_kernel<true> : chain_kernel<false>;
+    GMC_CUDA_TRY(cudaFuncSetAttribute(chain, cudaFuncAttributeMaxDynamicSharedMemorySize, kChainSmem));
+    GMC_CUDA_TRY(cudaLaunchKernelEx(&config, chain, b, steps, poly));
     finish_kernel<T, MUON><<<b.blocks, 256, 0, stream>>>(b, mo, steps & 1);
     GMC_LAUNCH_CHECK();
     return GMC_OK;

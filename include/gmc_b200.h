@@ -372,8 +372,8 @@ int gmc_log_probabilities_backward(const void* logits, int dtype, const long lon
  * momentum is contiguous fp32. Matrices may differ in shape; 1 <= rows, cols <= 32768, the smaller at most 16384. A zero
  * matrix gives zero; NaN or infinity in a matrix makes that matrix NaN. out may be update (the same address and stride), no
  * other overlap is allowed within a call, and no matrix may appear twice. Operands carry 22 bits, sums are fp32: for fp32 the
- * error is that of an fp32 evaluation (0.2 to 1.2 times, measured); for 16-bit types sums over long axes are not split up
- * (5e-5 of the result at 2048, against 2^-9 or 2^-12 for its rounding). How many CTAs share a sum depends on the other
+ * error is that of an fp32 evaluation (0.2 to 1.7 times, measured); for 16-bit types it is up to 2e-5 of the result before
+ * the rounding to their half step of 2^-9 or 2^-12, from sums that are split up every 2048 terms or less. How many CTAs share a sum depends on the other
  * matrices of the call, and with it the last bits; the same call gives the same bits.
  * 1 <= steps <= 32; coefficients whose iterates reach 1.8 for a singular value in [0, 1], that are 100 or more, or with
  * |b| > 32 |c| > 0 are refused (GMC_ERR_UNSUPPORTED); 1e-30 <= epsilon <= 1e30; 0 <= momentum < 1.

@@ -79,6 +79,25 @@ def test_a_long_inner_axis():
     _check(orthogonalise(u), u)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("signs", ["random", "one"])
+@pytest.mark.parametrize("m,n", [(200, 20000), (1500, 4100), (2048, 2048), (2000, 30000), (4095, 6001)])
+def test_16_bit_results_of_long_axes_before_their_rounding(m, n, signs, dtype):
+    """The rounding's own error is known (that of the rounded 64-bit result); what the evaluation adds to it is independent of
+    where a value lies between two 16-bit numbers, so that the squares add up, and may be what the bound above allows an
+    fp32 result: four times the plain evaluation's error and 2^-17."""
+    from gmc.optimisation import orthogonalise
+    g = torch.Generator(device="cuda").manual_seed(m + n)
+    u = torch.randn(m, n, device="cuda", generator=g) if signs == "random" else 0.1 + torch.rand(m, n, device="cuda", generator=g)
+    u = u.to(dtype)
+    got = orthogonalise(u).double()
+    ref = _plain(u.double(), 5, COEFFICIENTS, 1e-7)
+    norm = torch.linalg.matrix_norm
+    bound = 4 * norm(_plain(u.float(), 5, COEFFICIENTS, 1e-7).double() - ref) + 2.0 ** -17 * norm(ref)
+    added = (got - ref).square().sum() - (ref.to(dtype).double() - ref).square().sum()
+    assert added.clamp_min(0).sqrt() <= bound, f"{(added.clamp_min(0).sqrt() / norm(ref)).item():.3e} against {(bound / norm(ref)).item():.3e}"
+
+
 @pytest.mark.parametrize("m,n", [(20, 50), (200, 333)])
 def test_inputs_at_the_edges(m, n):
     """Rank one, nearly rank one, one element, equal elements, very small and very large values, orthogonal rows."""
