@@ -1704,22 +1704,21 @@ int check_matrices(const gmc_matrix* matrices, int n) {
 }
 
 // Bounds of the iterates and of b A + c A A for singular values in [0, 1], and from them the planes' scales: powers of two
-// that keep every value below the largest fp16 number. The extrema of x (a + b x^2 + c x^4) and of b l + c l^2 lie at the
-// end of the interval or where the derivative is zero.
+// that keep every value below the largest fp16 number. The extrema of x (a + b x^2 + c x^4) and of b l + c l^2, l = x^2, lie at
+// the end of the interval or where the derivative is zero: at the roots of 5c l^2 + 3b l + a, of which one is taken from the
+// product of both, so that nothing cancels however small c is (c = 0: the first is infinite), and at -b / 2c.
 int make_polynomial(int steps, float a, float b, float c, Polynomial* out) {
     if (steps < 1 || steps > 32) return GMC_ERR_UNSUPPORTED;
     const double da = a, db = b, dc = c;
     if (!(fabs(da) < 100. && fabs(db) < 100. && fabs(dc) < 100.)) return GMC_ERR_UNSUPPORTED;
-    const double root = sqrt(fmax(0., 9. * db * db - 20. * da * dc));
+    const double q = -0.5 * (3. * db + copysign(sqrt(fmax(0., 9. * db * db - 20. * da * dc)), db));
     double top = 1., most = 1., poly = 0.;
     for (int s = 0; s < steps; ++s) {
         const double end = top * top;
-        double at[4] = {end, end, end, end};
-        if (dc != 0.) at[1] = (-3. * db + root) / (10. * dc), at[2] = (-3. * db - root) / (10. * dc), at[3] = -db / (2. * dc);
-        else if (db != 0.) at[1] = -da / (3. * db);
+        const double at[4] = {end, q / (5. * dc), da / q, -db / (2. * dc)};
         double next = 0.;
         for (double l : at) {
-            if (!(l > 0. && l <= end)) continue;
+            if (!(l > 0. && l <= end)) continue;                      // infinite or not a number among others
             const double f = l * (db + dc * l);
             next = fmax(next, fabs(sqrt(l) * (da + f)));
             poly = fmax(poly, fabs(f));

@@ -375,8 +375,8 @@ int gmc_log_probabilities_backward(const void* logits, int dtype, const long lon
  * error is that of an fp32 evaluation (0.2 to 1.7 times, measured); for 16-bit types it is up to 2e-5 of the result before
  * the rounding to their half step of 2^-9 or 2^-12, from sums that are split up every 2048 terms or less. How many CTAs share a sum depends on the other
  * matrices of the call, and with it the last bits; the same call gives the same bits.
- * 1 <= steps <= 32; coefficients whose iterates reach 1.8 for a singular value in [0, 1], that are 100 or more, or with
- * |b| > 32 |c| > 0 are refused (GMC_ERR_UNSUPPORTED); 1e-30 <= epsilon <= 1e30; 0 <= momentum < 1.
+ * 1 <= steps <= 32; coefficients whose iterates reach 1.8 for a singular value in [0, 1], or that are 100 or more, are
+ * refused (GMC_ERR_UNSUPPORTED); 1e-30 <= epsilon <= 1e30; 0 <= momentum < 1.
  * workspace: gmc_orthogonalise_workspace_bytes (depends on the shapes only; 0 = none needed, or sizes out of range), aligned
  * to 1024 bytes, content undefined before and after; concurrent calls need one each. Nothing is allocated or synchronised,
  * and nothing kept but, per device, the number of CTA pairs that it holds. Matrices whose smaller side is above 128 (or that

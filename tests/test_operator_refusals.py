@@ -71,6 +71,19 @@ def test_orthogonalise_argument_checks():
     assert _native.lib.gmc_orthogonalise_workspace_bytes(_native.matrix_struct.pack(16, 0, 16, 0, 5, 5, 5, 0.0), 1) == 0
 
 
+@pytest.mark.parametrize("c", [1e-20, -1e-20, 1e-30, 1e-16, 1e-8, 0.0])
+def test_coefficients_are_bounded_however_small_the_last_one_is(c):
+    """x (a + b x^2) with a = 3.4, b = -2.4 reaches 1.557 at x^2 = a / -3b and leaves the range from there; with a = 3, b = -2 it
+    stays below 1.415 for ever. A c this small changes neither. (A workspace that is too small is found after the coefficients.)"""
+    from gmc import _native
+    m = _native.matrix_struct.pack(16, 0, 16, 130, 140, 140, 140, 0.0)
+
+    def run(a, b):
+        return _native.lib.gmc_orthogonalise(m, 1, 0, 5, a, b, c, 1e-7, 1024, 64, NULL)
+
+    assert run(3.4, -2.4) == 4 and run(3.0, -2.0) == 10
+
+
 def test_optimisation_refuses_what_it_cannot_do():
     from gmc._native import GmcError
     from gmc.optimisation import Muon, muon_update, orthogonalise

@@ -138,6 +138,20 @@ def test_steps_and_coefficients(m, n, steps, coefficients):
     _check(orthogonalise(u, steps=steps, coefficients=coefficients), u, steps, coefficients)
 
 
+@pytest.mark.parametrize("c", [0.0, 1e-20, -1e-20, 1e-9])
+@pytest.mark.parametrize("m,n", [(24, 70), (150, 200)])
+def test_iterates_above_one_with_a_last_coefficient_near_zero(m, n, c):
+    """Two equal singular values, 1 / sqrt 2 of the norm, go to sqrt 2 and stay there (up to their sign) under x (3 - 2 x^2): the
+    range of X and A that the operands' scale has to hold."""
+    from gmc.optimisation import orthogonalise
+    u = torch.zeros(m, n, device="cuda")
+    u[m // 3, 5] = u[m - 1, n - 2] = 1.0
+    # the slope at sqrt 2 is 3 - 6 x^2 = -9: an error there grows to 9^4 of itself in four more steps; c adds c x^5 = 5.7 c a step
+    want = torch.zeros_like(u, dtype=torch.float64)
+    want[m // 3, 5] = want[m - 1, n - 2] = 2 ** 0.5                # +, then -, +, -, + after five steps
+    assert (orthogonalise(u, coefficients=(3.0, -2.0, c)).double() - want).abs().max() <= 2 * 9 ** 4 * (4 * 2.0 ** -22 + 5.7 * abs(c))
+
+
 @pytest.mark.parametrize("m,n", [(48, 100), (400, 256)])
 def test_singular_values_end_near_one(m, n):
     from gmc.optimisation import orthogonalise
