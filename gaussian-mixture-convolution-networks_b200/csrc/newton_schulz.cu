@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ Batc
     __syncthreads();
     s = 0.;
     for (int w = 0; w < 8; ++w) s += warp_sum[w];
-    const float norm = float(sqrt(s) + double(epsilon));
+    const float factor = float(double(kScaleX) / (sqrt(s) + double(epsilon)));        // the norm itself may leave the fp32 range
     const bool tall = m.rows > m.cols;
     const int wide_rows = tall ? m.cols : m.rows, wide_cols = tall ? m.rows : m.cols;
     const int row_tile = block / m.col_blocks, col_block = block - row_tile * m.col_blocks;
@@ -228,7 +228,6 @@ __global__ void __launch_bounds__(256) split_kernel(const __grid_constant__ Batc
     __shared__ __align__(128) uint8_t image[kBlockBytes];
     const T* update = static_cast<const T*>(m.update);
     const bool vectors = rows_aligned(update, m.update_stride, sizeof(T)), momentum_vectors = rows_aligned(m.momentum, m.cols, 4);
-    const float factor = kScaleX / norm;
     const uint4 none = {};
 #pragma unroll 2
     for (int i = threadIdx.x; i < 128 * 8; i += 256) {
@@ -1112,10 +1111,12 @@ __device__ __forceinline__ void short_matrix(const Matrix& m, int ranks, int ran
         for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         s = __shfl_sync(0xffffffffu, s, 0);
     }
-    const float factor = float(1. / (sqrt(s) + double(epsilon)));
+    // 1 / norm is no normal fp32 number for norms above 2^126: X is made smaller by a power of two first
+    const double norm = sqrt(s) + double(epsilon);
+    const float before = norm > 0x1p100 ? 0x1p-100f : 1.f, factor = float(1. / (norm * double(before)));
     for (int i = tid * 4; i < MP * pitch; i += kShortThreads * 4) {
         float4 v = *reinterpret_cast<float4*>(x + i);
-        v.x *= factor, v.y *= factor, v.z *= factor, v.w *= factor;
+        v.x = v.x * before * factor, v.y = v.y * before * factor, v.z = v.z * before * factor, v.w = v.w * before * factor;
         *reinterpret_cast<float4*>(x + i) = v;
     }
     // where this thread's element of the packed sums goes (the same in every step)

@@ -118,6 +118,19 @@ def test_inputs_at_the_edges(m, n):
     assert (orthogonalise(torch.zeros(m, n, device="cuda")) == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n", [(2, 3), (12, 30), (8, 32768), (16, 20000), (20000, 16), (20, 50), (100, 3000), (200, 333), (333, 200), (300, 5000)])
+def test_norms_beyond_the_range_of_fp32(m, n, dtype):
+    """Finite updates whose norm is not a finite fp32 number, the same by a power of two as an ordinary one: the same result, to
+    the same bound."""
+    from gmc.optimisation import orthogonalise
+    u = _update(m, n, seed=n, dtype=dtype)
+    u = u * 2.0 ** -math.frexp(u.abs().max().item())[1]           # the largest element in [0.5, 1)
+    huge = u * 2.0 ** 127 * 2                                     # in [2^127, 2^128)
+    assert torch.isfinite(huge).all() and torch.linalg.matrix_norm(huge.double()) > torch.finfo(torch.float32).max * (m > 10)
+    _check(orthogonalise(huge, epsilon=1e-30), u, epsilon=1e-30)
+
+
 @pytest.mark.parametrize("m,n", [(12, 30), (140, 260)])
 def test_nan_and_infinity_stay_in_their_matrix(m, n):
     from gmc.optimisation import orthogonalise
