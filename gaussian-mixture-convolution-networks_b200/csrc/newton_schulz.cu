@@ -1831,7 +1831,7 @@ int run_clusters(const gmc_matrix* matrices, const int* which, int n, int steps,
 
 template <typename T, bool MUON>
 int run_typed(const gmc_matrix* matrices, int n, int steps, float ca, float cb, float cc, const Polynomial& poly, float epsilon, const Momentum& mo,
-              void* workspace, size_t workspace_bytes, cudaStream_t stream, int lost_wait) {
+              void* workspace, size_t workspace_bytes, int pairs, cudaStream_t stream, int lost_wait) {
     int which[kMaxMatrices], count = 0;
     for (int kind = 0; kind < KINDS; ++kind) {
         for (int i = 0; i <= n; ++i) {
@@ -1842,8 +1842,6 @@ int run_typed(const gmc_matrix* matrices, int n, int steps, float ca, float cb, 
                 } else {
                     Batch b;
                     size_t bytes = 0;
-                    int pairs = 0;
-                    if (int s = chain_pairs(&pairs)) return s;
                     fill(matrices, which, count, pairs, std::is_same<T, float>::value, &b, &bytes, static_cast<uint8_t*>(workspace));
                     if (bytes > workspace_bytes) return GMC_ERR_WORKSPACE;
                     b.lost_wait = lost_wait;
@@ -1886,10 +1884,13 @@ int run(const gmc_matrix* matrices, int n, int dtype, int steps, float ca, float
     const size_t need = workspace_bytes_of(matrices, n);
     if (need > 0 && !workspace) return GMC_ERR_NULL_POINTER;
     if (need > workspace_bytes) return GMC_ERR_WORKSPACE;
+    int pairs = 0;                                                    // asked for before anything is changed in place
+    if (need > 0)
+        if (int s = chain_pairs(&pairs)) return s;
     cudaStream_t cs = as_stream(stream);
-    if (dtype == GMC_FLOAT32) return run_typed<float, MUON>(matrices, n, steps, ca, cb, cc, poly, epsilon, mo, workspace, workspace_bytes, cs, lost_wait);
-    if (dtype == GMC_BFLOAT16) return run_typed<__nv_bfloat16, MUON>(matrices, n, steps, ca, cb, cc, poly, epsilon, mo, workspace, workspace_bytes, cs, lost_wait);
-    return run_typed<__half, MUON>(matrices, n, steps, ca, cb, cc, poly, epsilon, mo, workspace, workspace_bytes, cs, lost_wait);
+    if (dtype == GMC_FLOAT32) return run_typed<float, MUON>(matrices, n, steps, ca, cb, cc, poly, epsilon, mo, workspace, workspace_bytes, pairs, cs, lost_wait);
+    if (dtype == GMC_BFLOAT16) return run_typed<__nv_bfloat16, MUON>(matrices, n, steps, ca, cb, cc, poly, epsilon, mo, workspace, workspace_bytes, pairs, cs, lost_wait);
+    return run_typed<__half, MUON>(matrices, n, steps, ca, cb, cc, poly, epsilon, mo, workspace, workspace_bytes, pairs, cs, lost_wait);
 }
 
 }  // namespace

@@ -1,5 +1,8 @@
 """CPU: what the training-step operators refuse before any GPU work is issued."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -101,3 +104,45 @@ def test_optimisation_refuses_what_it_cannot_do():
     with pytest.raises(GmcError, match="two or more axes"):
         Muon([torch.nn.Parameter(torch.zeros(5))])
     muon_update([], [], [], 0.1)
+
+
+FAKE_RUNTIME = """
+int launches;
+int cudaGetDevice(int* device) { *device = 0; return 0; }
+int cudaDeviceGetAttribute(int* value, int attribute, int device) { *value = 148; return 0; }
+int cudaFuncSetAttribute(const void* f, int attribute, int value) { return 0; }
+int cudaOccupancyMaxActiveClusters(int* n, const void* f, const void* config) { *n = PAIRS; return 0; }
+int cudaLaunchKernelExC(const void* config, const void* f, void** arguments) { ++launches; return 0; }
+int cudaLaunchKernel() { ++launches; return 0; }
+int cudaGetLastError(void) { return 0; }
+"""
+CALL = """
+import ctypes, struct, sys
+fake, lib = ctypes.CDLL(sys.argv[1]), ctypes.CDLL(sys.argv[2])
+pack = lambda rows, cols: struct.pack("@PPPqqqqf4x", 16, 16, 16, rows, cols, cols, cols, 0.1)
+lib.gmc_muon_update.argtypes = ([ctypes.c_char_p] + [ctypes.c_int] * 3 + [ctypes.c_float] * 4 + [ctypes.BETA]
+                                + [ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p])
+status = lib.gmc_muon_update(pack(64, 160) + pack(300, 500), 2, 0, 5, 3.4445, -4.775, 2.0315, 1e-7, 0.9, 1, 1.0, 1024, 1 << 30, None)
+print(status, ctypes.c_int.in_dll(fake, "launches").value)
+"""
+
+
+@pytest.mark.parametrize("pairs,expected", [(47, "4 0"), (48, "0 5"), (74, "0 5")])
+def test_a_device_that_cannot_hold_the_call_is_refused_before_anything_is_launched(tmp_path, pairs, expected):
+    """A fake of the runtime counts launches: the cooperative kernel that the larger matrix needs wants 48 pairs of CTAs. Where they
+    are missing, the smaller matrix's parameters must not have moved."""
+    from gmc import _native
+    source, fake = tmp_path / "fake.c", tmp_path / "fake.so"
+    source.write_text(FAKE_RUNTIME.replace("PAIRS", str(pairs)))
+    subprocess.run(["gcc", "-shared", "-fPIC", "-w", "-o", fake, source], check=True)
+    beta = {4: "c_float", 8: "c_double"}[ctypes.sizeof(_native.lib.gmc_muon_update.argtypes[8])]
+    out = subprocess.run([sys.executable, "-c", CALL.replace("BETA", beta), str(fake), _native.lib._name], capture_output=True, text=True,
+                         env=dict(os.environ, LD_PRELOAD=str(fake), LD_LIBRARY_PATH=os.pathsep.join(
+                             filter(None, [os.path.dirname(_runtime_path()), os.environ.get("LD_LIBRARY_PATH")]))))
+    assert out.stdout.strip() == expected, out.stdout + out.stderr
+
+
+def _runtime_path():
+    """The CUDA runtime that this process has loaded with the library."""
+    with open("/proc/self/maps") as maps:
+        return next(line.split()[-1] for line in maps if "libcudart.so" in line)
