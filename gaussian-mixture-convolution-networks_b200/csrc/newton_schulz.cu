@@ -1917,9 +1917,10 @@ extern "C" int gmc_debug_orthogonalise_lost_wait(const gmc_matrix* matrices, int
 }
 
 extern "C" int gmc_muon_update(const gmc_matrix* matrices, int n_matrices, int dtype, int steps, float a, float b, float c,
-                               float epsilon, float momentum, int nesterov, float decay, void* workspace, size_t workspace_bytes,
+                               float epsilon, double momentum, int nesterov, float decay, void* workspace, size_t workspace_bytes,
                                void* stream) {
-    if (!(momentum >= 0.f && momentum < 1.f)) return GMC_ERR_UNSUPPORTED;
-    const gmc::Momentum mo = {momentum, 1.f - momentum, nesterov != 0, decay};
+    if (!(momentum >= 0. && momentum < 1.)) return GMC_ERR_UNSUPPORTED;
+    // the new gradient's weight is rounded once: 1 - float(0.9999) would be off by 2e-4 of itself
+    const gmc::Momentum mo = {float(momentum), float(1. - momentum), nesterov != 0, decay};
     return gmc::run<true>(matrices, n_matrices, dtype, steps, a, b, c, epsilon, mo, workspace, workspace_bytes, stream);
 }

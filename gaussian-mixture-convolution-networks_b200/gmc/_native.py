@@ -93,7 +93,7 @@ _declare("gmc_orthogonalise", [_c_void_p] + [_c_int] * 3 + [ctypes.c_float] * 4
          + [_c_void_p, ctypes.c_size_t, _c_void_p])
 _declare("gmc_debug_orthogonalise_lost_wait", [_c_void_p] + [_c_int] * 3 + [ctypes.c_float] * 4
          + [_c_void_p, ctypes.c_size_t, _c_int, _c_void_p])
-_declare("gmc_muon_update", [_c_void_p] + [_c_int] * 3 + [ctypes.c_float] * 5 + [_c_int, ctypes.c_float]
+_declare("gmc_muon_update", [_c_void_p] + [_c_int] * 3 + [ctypes.c_float] * 4 + [ctypes.c_double, _c_int, ctypes.c_float]
          + [_c_void_p, ctypes.c_size_t, _c_void_p])
 
 

@@ -399,7 +399,7 @@ int gmc_orthogonalise(const gmc_matrix* matrices, int n_matrices, int dtype, int
 int gmc_debug_orthogonalise_lost_wait(const gmc_matrix* matrices, int n_matrices, int dtype, int steps, float a, float b, float c,
                                       float epsilon, void* workspace, size_t workspace_bytes, int lost_wait, void* stream);
 int gmc_muon_update(const gmc_matrix* matrices, int n_matrices, int dtype, int steps, float a, float b, float c, float epsilon,
-                    float momentum, int nesterov, float decay, void* workspace, size_t workspace_bytes, void* stream);
+                    double momentum, int nesterov, float decay, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * gmc_mhem_fit_forward for callers that have no scratch memory to give. (No counterpart in the reference, which

@@ -228,6 +228,24 @@ def test_muon_update(shapes, nesterov, dtype):
             + (4 ** 5 * 3 * 2.0 ** -24 + 2.0 ** -12) * step
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("momentum", [0.0, 0.9, 0.95, 0.999, 0.9999])
+@pytest.mark.parametrize("shapes", [[(16, 40)], [(64, 160)], [(300, 129), (9, 700)]])
+def test_the_weights_of_the_running_average(shapes, momentum, dtype):
+    """Each of b m and (1 - b) g carries the roundings of its factor, of the product and of the sum: three half steps of fp32.
+    Nothing is kept of the momenta, and then much, so that either term is seen."""
+    from gmc.optimisation import muon_update
+    for share in (0.0, 1.0):
+        params = [torch.zeros(s, device="cuda", dtype=dtype) for s in shapes]
+        grads = [_update(*s, seed=i, dtype=dtype) for i, s in enumerate(shapes)]
+        momenta = [share * _update(*s, seed=50 + i) for i, s in enumerate(shapes)]
+        old = [m.clone() for m in momenta]
+        muon_update(params, grads, momenta, 0.1, momentum)
+        for m, o, g in zip(momenta, old, grads):
+            kept, new = momentum * o.double(), (1 - momentum) * g.double()
+            assert ((m.double() - (kept + new)).abs() <= 3 * 2.0 ** -24 * (kept.abs() + new.abs()) + 2.0 ** -149).all()
+
+
 def test_muon_update_of_many_matrices_and_strided_gradients():
     """More matrices than one launch takes, of all kinds, with gradients that are transposed or broadcast views."""
     from gmc.optimisation import muon_update
