@@ -4,6 +4,7 @@ import typing
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from gmc import _native
 
@@ -78,10 +79,12 @@ def log_probabilities(logits: Tensor, targets: typing.Optional[Tensor] = None, n
     most 32) asks for the likeliest classes. Masked classes hold -inf; a row with nothing else has log-probabilities -inf,
     entropy 0 and gradient 0. NaN and +inf in a row make its values and gradient NaN.
 
-    target, entropy and top are differentiable once with respect to the logits. Logits whose classes are not adjacent in
+    target, entropy and top are differentiable once with respect to the logits, in reverse mode. Logits whose classes are not adjacent in
     memory are copied; rows may be any distance apart."""
     if not isinstance(logits, Tensor) or logits.dim() < 1 or logits.shape[-1] < 1:
         raise _native.GmcError("logits must be a tensor [..., n_classes] with at least one class")
+    if forward_ad.unpack_dual(logits).tangent is not None:
+        raise _native.GmcError("log_probabilities has no forward-mode derivative")
     code = _native.dtype_code(logits, "logits")
     c = logits.shape[-1]
     if not 0 <= n_top <= min(MAX_TOP, c):

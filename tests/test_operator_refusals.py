@@ -50,6 +50,23 @@ def test_log_probabilities_refuses_what_it_cannot_do():
         log_probabilities([1.0, 2.0])
 
 
+def test_log_probabilities_refuses_forward_mode_derivatives():
+    """A dual tensor does not require a gradient; its tangent must not be dropped in silence."""
+    from torch.autograd import forward_ad
+
+    from gmc._native import GmcError
+    from gmc.classification import log_probabilities
+    z = torch.zeros(2, 3)
+    with forward_ad.dual_level():
+        with pytest.raises(GmcError, match="forward-mode"):
+            log_probabilities(forward_ad.make_dual(z, torch.ones(2, 3)))
+        with pytest.raises(GmcError, match="no CPU implementation"):
+            log_probabilities(z)
+    with pytest.raises(GmcError, match="forward-mode"):
+        with forward_ad.dual_level():
+            log_probabilities(forward_ad.make_dual(torch.nn.Parameter(z), torch.ones(2, 3)) * 2)
+
+
 def test_orthogonalise_argument_checks():
     from gmc import _native
     address = 1024
