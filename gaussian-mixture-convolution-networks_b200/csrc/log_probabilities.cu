@@ -156,6 +156,12 @@ __device__ __forceinline__ void add_vectors(const Vec<T> (&v)[kUnroll], float ba
     st.t += t.x + t.y;
 }
 
+// (z - m) / T: the difference of two finite logits may leave the fp32 range where the quotient does not.
+__device__ __forceinline__ float scaled(float z, float m, float inv_t) {
+    const float x = z - m;
+    return x == neg_inf() && z != neg_inf() ? z * inv_t - m * inv_t : x * inv_t;
+}
+
 struct Outputs {
     float* target;                // [n_rows] or null
     float* entropy;               // [n_rows]
@@ -196,7 +202,7 @@ __device__ __forceinline__ float write_row(const Outputs& out, const Stat& st, c
             report_check(CHECK_CLASS_RANGE);
             v = quiet_nan();
         } else {
-            v = empty ? neg_inf() : (g.z - st.m) * inv_t - log_s;
+            v = empty ? neg_inf() : scaled(g.z, st.m, inv_t) - log_s;
         }
         out.target[row] = v;
     }
@@ -205,7 +211,7 @@ __device__ __forceinline__ float write_row(const Outputs& out, const Stat& st, c
 __device__ __forceinline__ void write_alternative(const Outputs& out, Key key, long long row, int n_top, int place, float m, float log_s,
                                                   bool empty, float inv_t) {
     out.top_indices[row * n_top + place] = (long long)key_index(key);
-    out.top[row * n_top + place] = empty ? neg_inf() : (key_value(key) - m) * inv_t - log_s;
+    out.top[row * n_top + place] = empty ? neg_inf() : scaled(key_value(key), m, inv_t) - log_s;
 }
 
 // ---- short rows: one warp per row, the row in registers ---------------------------------------------------------------

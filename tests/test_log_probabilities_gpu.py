@@ -166,6 +166,29 @@ def test_logits_at_both_ends_of_the_range(others):
     assert (g.double() - want.double()).abs().max() <= 2.0 ** -9
 
 
+@pytest.mark.parametrize("temperature", [1.0, 2.0, 1e6])
+@pytest.mark.parametrize("c", [6, 1024, 3001, 70000])
+def test_logits_further_apart_than_the_range(c, temperature):
+    """z - max is -6e38, beyond fp32, and log p, its quotient by T, need not be. The bound is u (S + 4 |y|) with the whole |y|, up to
+    6.4e32 here: 1 / T, the two products by it and their difference are rounded once each."""
+    from gmc.classification import log_probabilities
+    g = torch.Generator(device="cuda").manual_seed(c)
+    z = torch.randn(5, c, device="cuda", generator=g)
+    z[:, 0] = 3e38
+    z[1, 1:], z[2, 3], z[3, 1:], z[4, c - 1] = -3e38, -3e38, -math.inf, -3.4e38
+    z[3, 4] = -3e38
+    t, n_top = torch.tensor([1, c - 1, 3, 4, c - 1], device="cuda"), min(c, 5)
+    z.requires_grad_(True)
+    r = log_probabilities(z, t, n_top, temperature)
+    (grad,) = torch.autograd.grad(r.target.sum() + r.entropy.sum(), z)
+    ref = _reference(z, t, n_top, temperature, -100, [torch.ones(5), torch.ones(5), torch.zeros(5, n_top)])
+    y_t, y_k = ref["y"].gather(1, t.cpu().unsqueeze(1)).squeeze(1).abs(), ref["y"].gather(1, ref["top_indices"]).abs()
+    _close(r.target, ref["target"], U * (_scale(c) + 4 * y_t), "target")
+    _close(r.top, ref["top"], U * (_scale(c) + 4 * y_k), "top")
+    _close(r.entropy, ref["entropy"], U * 2 * _scale(c) * (1 + math.log2(c)), "entropy")
+    _close(grad, ref["grad"], ref["grad_tolerance"] + U * ref["grad"].abs() + 2.0 ** -149, "gradient")
+
+
 @pytest.mark.parametrize("c", [20, 1024, 1025, 70000])
 def test_nan_and_infinity_make_the_row_nan(c):
     from gmc.classification import log_probabilities
