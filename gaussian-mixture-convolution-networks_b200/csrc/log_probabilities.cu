@@ -501,6 +501,7 @@ struct Incoming {
 };
 struct RowGradient {                // grad_j = p_j (a + b x_j), x_j = z_j - m, plus the given classes' own terms
     float m, a, b, g_target, log2_s;
+    float lowest;                   // bound of x_j far below where p_j is 0, for which b times it stays finite
     long long target;
     bool empty, bad;
 };
@@ -521,13 +522,14 @@ __device__ __forceinline__ RowGradient row_gradient(const Incoming& in, const fl
     const float g_h = in.entropy ? in.entropy[row] : 0.f;
     g.a = -inv_t * (sum + g_h * (h - log_s));
     g.b = -inv_t * g_h * inv_t;
+    g.lowest = -1000.f / inv_t;
     return g;
 }
 __device__ __forceinline__ float2 gradient_pair(const RowGradient& g, float2 z, float k) {
     const float2 x = __fadd2_rn(z, make_float2(-g.m, -g.m));
     const float2 y = __ffma2_rn(x, make_float2(k, k), make_float2(-g.log2_s, -g.log2_s));
     const float2 p = make_float2(ex2_approx(y.x), ex2_approx(y.y));
-    return __fmul2_rn(p, __ffma2_rn(make_float2(fmaxf(x.x, kLowest), fmaxf(x.y, kLowest)), make_float2(g.b, g.b), make_float2(g.a, g.a)));
+    return __fmul2_rn(p, __ffma2_rn(make_float2(fmaxf(x.x, g.lowest), fmaxf(x.y, g.lowest)), make_float2(g.b, g.b), make_float2(g.a, g.a)));
 }
 __device__ __forceinline__ float gradient_at(const RowGradient& g, float z, float k) { return gradient_pair(g, make_float2(z, z), k).x; }
 // One thread: the whole gradient at the i-th given class (0 = the target, 1.. = the alternatives) of a row, written once

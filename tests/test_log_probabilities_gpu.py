@@ -189,6 +189,24 @@ def test_logits_further_apart_than_the_range(c, temperature):
     _close(grad, ref["grad"], ref["grad_tolerance"] + U * ref["grad"].abs() + 2.0 ** -149, "gradient")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("temperature,scale", [(1e-6, 1e8), (1e-3, 1e14), (1.0, 1e30), (1e6, 1e30)])
+@pytest.mark.parametrize("c", [20, 1024, 3001])
+def test_large_incoming_gradients_of_the_entropy(c, temperature, scale, dtype):
+    """A class of probability 0 gets no gradient, masked or not, however large the incoming one (a loss scale over a small
+    temperature): here one class has all of the probability and its own gradient -p g (log p + H) / T is 0 as well."""
+    from gmc.classification import log_probabilities
+    z = torch.full((3, c), -math.inf, device="cuda", dtype=dtype)
+    z[0, 1], z[1, 2], z[2, c - 1] = 1.0, 0.0, 60000.0
+    if temperature <= 1.0:
+        z[1, 5:] = -4000.0
+        z[2, :4] = -30000.0
+    z.requires_grad_(True)
+    r = log_probabilities(z, temperature=temperature)
+    (grad,) = torch.autograd.grad(r.entropy, z, torch.full_like(r.entropy, scale))
+    assert (r.entropy == 0).all() and (grad == 0).all()
+
+
 @pytest.mark.parametrize("c", [20, 1024, 1025, 70000])
 def test_nan_and_infinity_make_the_row_nan(c):
     from gmc.classification import log_probabilities
