@@ -135,10 +135,13 @@ class Muon(torch.optim.Optimizer):
                  steps: int = 5, coefficients: typing.Sequence[float] = COEFFICIENTS, epsilon: float = 1e-7):
         super().__init__(params, dict(lr=lr, momentum=momentum, weight_decay=weight_decay, nesterov=nesterov, steps=steps,
                                       coefficients=tuple(_coefficients(coefficients)), epsilon=epsilon))
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.dim() < 2:
-                    raise _native.GmcError(f"Muon takes parameters with two or more axes, got {tuple(p.shape)}")
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() < 2:
+                self.param_groups.pop()
+                raise _native.GmcError(f"Muon takes parameters with two or more axes, got {tuple(p.shape)}")
 
     @torch.no_grad()
     def step(self, closure=None):

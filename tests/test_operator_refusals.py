@@ -123,6 +123,17 @@ def test_optimisation_refuses_what_it_cannot_do():
     muon_update([], [], [], 0.1)
 
 
+def test_muon_refuses_parameters_with_one_axis_in_later_groups():
+    from gmc._native import GmcError
+    from gmc.optimisation import Muon
+    opt = Muon([torch.nn.Parameter(torch.zeros(5, 3))])
+    with pytest.raises(GmcError, match="two or more axes"):
+        opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(4, 3)), torch.nn.Parameter(torch.zeros(5))]})
+    assert len(opt.param_groups) == 1
+    opt.add_param_group({"params": torch.nn.Parameter(torch.zeros(4, 3)), "lr": 0.5})
+    assert [g["lr"] for g in opt.param_groups] == [0.02, 0.5]
+
+
 FAKE_RUNTIME = """
 int launches;
 int cudaGetDevice(int* device) { *device = 0; return 0; }
