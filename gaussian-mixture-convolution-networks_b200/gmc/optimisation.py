@@ -170,6 +170,6 @@ class Muon(torch.optim.Optimizer):
         # the base class converts states to the parameter's type; the momentum stays in 32 bits
         for group, saved in zip(self.param_groups, state_dict["param_groups"]):
             for p, key in zip(group["params"], saved["params"]):
-                if key in state_dict["state"]:
-                    buffer = state_dict["state"][key]["momentum_buffer"]
+                buffer = state_dict["state"].get(key, {}).get("momentum_buffer")
+                if buffer is not None:
                     self.state[p]["momentum_buffer"] = buffer.detach().to(device=p.device, dtype=torch.float32, copy=True).contiguous()

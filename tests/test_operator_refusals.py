@@ -134,6 +134,18 @@ def test_muon_refuses_parameters_with_one_axis_in_later_groups():
     assert [g["lr"] for g in opt.param_groups] == [0.02, 0.5]
 
 
+def test_muon_loads_states_without_a_momentum():
+    """A parameter whose state was only looked at has an empty one; it is saved and loaded like any other."""
+    from gmc.optimisation import Muon
+    params = [torch.nn.Parameter(torch.zeros(5, 3)), torch.nn.Parameter(torch.zeros(3, 4, dtype=torch.bfloat16))]
+    opt, other = Muon(params), Muon(params)
+    assert opt.state[params[0]] == {}
+    opt.state[params[1]]["momentum_buffer"] = torch.full((3, 4), 1 / 3)
+    other.load_state_dict(opt.state_dict())
+    assert "momentum_buffer" not in other.state[params[0]]
+    assert torch.equal(other.state[params[1]]["momentum_buffer"], torch.full((3, 4), 1 / 3))
+
+
 FAKE_RUNTIME = """
 int launches;
 int cudaGetDevice(int* device) { *device = 0; return 0; }
