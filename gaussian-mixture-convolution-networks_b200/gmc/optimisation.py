@@ -85,7 +85,7 @@ def muon_update(params: typing.Sequence[Tensor], grads: typing.Sequence[Tensor],
 
     Parameters and gradients share one type (float32, bfloat16 or float16); momenta are float32, shaped like the parameters.
     A parameter with more than two axes counts as the matrix [shape[0], everything else]. Parameters and momenta must be
-    contiguous and may not appear twice."""
+    contiguous and may not appear twice; no gradient may share their memory."""
     if not len(params) == len(grads) == len(momenta):
         raise _native.GmcError("params, grads and momenta must have one entry per parameter")
     if not params:
@@ -95,7 +95,7 @@ def muon_update(params: typing.Sequence[Tensor], grads: typing.Sequence[Tensor],
     a, b, c = _coefficients(coefficients)
     first = params[0]
     code = _native.dtype_code(first, "params")
-    entries, held, seen = [], [], set()
+    entries, held, seen, read = [], [], set(), set()
     for p, g, m in zip(params, grads, momenta):
         if p.dtype != first.dtype or g.dtype != first.dtype or p.device != first.device or g.device != first.device:
             raise _native.GmcError("parameters and gradients of one call must have one type and device")
@@ -105,19 +105,20 @@ def muon_update(params: typing.Sequence[Tensor], grads: typing.Sequence[Tensor],
             raise _native.GmcError(f"a gradient must be dense and shaped like its parameter, got {tuple(g.shape)}")
         if m.shape != p.shape or m.dtype != torch.float32 or m.device != p.device or not m.is_contiguous():
             raise _native.GmcError("momenta must be contiguous float32, shaped like their parameters and on their device")
-        if p.data_ptr() in seen or m.data_ptr() in seen:
+        if p.data_ptr() in seen or m.data_ptr() in seen or p.data_ptr() == m.data_ptr():
             raise _native.GmcError("a parameter or momentum appears twice")
         seen.update((p.data_ptr(), m.data_ptr()))
-        if g.data_ptr() in (p.data_ptr(), m.data_ptr()):
-            raise _native.GmcError("a gradient must not share its memory with its parameter or momentum")
         if not g.is_contiguous():
             g = g.contiguous()
             held.append(g)
+        read.add(g.data_ptr())
         rows = p.shape[0]
         cols = p.numel() // rows
         _check_sides(rows, cols)
         entries.append(_native.matrix_struct.pack(g.data_ptr(), m.data_ptr(), p.data_ptr(), rows, cols, cols, cols,
                                                   lr * math.sqrt(max(1.0, rows / cols))))
+    if read & seen:
+        raise _native.GmcError("a gradient must not share its memory with a parameter or momentum")
     packed = b"".join(entries)
     with torch.cuda.device_of(first):
         hold, address, size = _workspace(packed, len(entries), first.device)

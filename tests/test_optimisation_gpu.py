@@ -288,6 +288,24 @@ def test_the_same_tensor_twice_is_refused():
         orthogonalise(p, steps=0)
 
 
+def test_memory_shared_between_arguments_is_refused():
+    """It would be read while it is written. Nothing is changed by the refused call; one gradient for two parameters is fine."""
+    from gmc._native import GmcError
+    from gmc.optimisation import muon_update
+    p, q, m, k = (torch.randn(30, 40, device="cuda") for _ in range(4))
+    g = _update(30, 40)
+    before = [t.clone() for t in (p, q, m, k)]
+    for grads in ([q, g], [g, p], [k, g], [g, m], [p, g], [g, k]):
+        with pytest.raises(GmcError, match="share its memory"):
+            muon_update([p, q], grads, [m, k], 0.1)
+    for params, momenta in (([p, q], [m, q]), ([p, q], [q, k]), ([p], [p])):
+        with pytest.raises(GmcError, match="appears twice"):
+            muon_update(params, [g] * len(params), momenta, 0.1)
+    assert all(torch.equal(a, b) for a, b in zip(before, (p, q, m, k)))
+    muon_update([p, q], [g, g], [m, k], 0.1)
+    assert not torch.equal(q, before[1])
+
+
 def test_optimiser_steps_and_state():
     """Three steps of the class on an fp32 and a bf16 parameter against the restatement; the state survives a save and load in
     32 bits; parameters without a gradient are left alone."""
