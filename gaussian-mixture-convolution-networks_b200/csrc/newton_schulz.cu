@@ -1599,22 +1599,18 @@ void hand_out(Batch& b, int pairs) {
 
 void describe(const gmc_matrix& g, Matrix& m);
 
-// Lays out the workspace and hands out the pairs.
-void fill(const gmc_matrix* matrices, const int* which, int n, int pairs, bool fp32, Batch* batch, size_t* bytes, uint8_t* workspace) {
-    Batch& b = *batch;
+// Describes the matrices of a launch and lays out its workspace; returns the workspace's size.
+size_t lay_out(const gmc_matrix* matrices, const int* which, int n, uint8_t* workspace, Batch& b) {
     b.n = n;
-    long long x_blocks = 0, gram_blocks = 0, partials = 0;
+    long long x_blocks = 0, gram_blocks = 0;
     b.norm_ctas = b.blocks = 0;
+    bool splittable = false;
     for (int i = 0; i < n; ++i) {
         const gmc_matrix& g = matrices[which[i]];
         Matrix& m = b.m[i];
-        const long long wide_rows = g.rows < g.cols ? g.rows : g.cols, wide_cols = g.rows < g.cols ? g.cols : g.rows;
         describe(g, m);
-        m.row_tiles = ceil_div(wide_rows, 128);
-        m.col_blocks = 2 * ceil_div(wide_cols, 128);
-        // fp32 results: against the plain fp32 evaluation's error, 256 x 4000 has 1.2 times with two stages and 2.3 with four,
-        // 700 x 2000 0.9 with four and 1.6 with eight, 2048 x 2048 0.7 with eight and the time is 810, 720 and 680 us
-        m.chunk = !fp32 ? kWholeAxis : wide_rows <= 512 ? 2 : wide_rows <= 1024 ? 4 : 8;
+        m.row_tiles = ceil_div(std::min(m.rows, m.cols), 128);
+        m.col_blocks = 2 * ceil_div(std::max(m.rows, m.cols), 128);
         m.norm_first = b.norm_ctas;
         m.block_first = b.blocks;
         m.x_block = x_blocks;
@@ -1624,26 +1620,6 @@ void fill(const gmc_matrix* matrices, const int* which, int n, int pairs, bool f
         b.blocks += int(blocks);
         x_blocks += blocks;
         gram_blocks += 2LL * m.row_tiles * m.row_tiles;
-    }
-    hand_out(b, pairs);
-    // 16-bit results: one accumulation per sum while none is longer than 2048. The error before the last rounding is then 4e-6 to 2e-5
-    // of the result (0.9 to 4 times the plain fp32 evaluation's; half a step is 2e-3 or 2.4e-4) and grows with the length
-    // beyond: 4.8e-5 at 4095 x 6001, 8.7e-5 at 16384 x 32768 (random signs). In chunks of 1024 it is 1.4e-5 and 5e-6, and the
-    // time 5.55 ms for 5.17 and 455 ms for 443; chunks of 2048 would take 5.42 ms for 2.7e-5, of 512 5.75 ms for 7e-6.
-    b.whole = !fp32;
-    for (int i = 0; i < n; ++i) b.whole = b.whole && longest_sum(b.m[i]) <= kWholeStages;
-    if (!fp32 && !b.whole) {
-        for (int i = 0; i < n; ++i) b.m[i].chunk = kLongChunk;
-        hand_out(b, pairs);
-    }
-    b.pairs = 0;
-    bool splittable = false;
-    for (int i = 0; i < n; ++i) {
-        Matrix& m = b.m[i];
-        m.pair_first = b.pairs;
-        b.pairs += m.pairs;
-        m.partial_first = partials;
-        if (m.splits > 1) partials += (long long)symmetric_tiles(m.row_tiles, m.gram_wide) * m.splits * 256 * (m.gram_wide ? 256 : 128);
         splittable = splittable || m.row_tiles <= 16;
     }
     size_t at = 0;
@@ -1661,7 +1637,37 @@ void fill(const gmc_matrix* matrices, const int* which, int n, int pairs, bool f
     // size holds for any number of pairs up to kPairs
     b.partial = reinterpret_cast<float*>(take(splittable ? size_t(kPairs) * 256 * 256 * sizeof(float) : 0));
     b.arrived = reinterpret_cast<unsigned*>(take(size_t(n + 1) * sizeof(unsigned)));
-    *bytes = at;
+    return at;
+}
+
+// The launch's plan: chunks, tiles, shares and pairs.
+void make_plan(Batch& b, int pairs, bool fp32) {
+    for (int i = 0; i < b.n; ++i) {
+        const int rows = std::min(b.m[i].rows, b.m[i].cols);
+        // fp32 results: against the plain fp32 evaluation's error, 256 x 4000 has 1.2 times with two stages and 2.3 with four,
+        // 700 x 2000 0.9 with four and 1.6 with eight, 2048 x 2048 0.7 with eight and the time is 810, 720 and 680 us
+        b.m[i].chunk = !fp32 ? kWholeAxis : rows <= 512 ? 2 : rows <= 1024 ? 4 : 8;
+    }
+    hand_out(b, pairs);
+    // 16-bit results: one accumulation per sum while none is longer than 2048. The error before the last rounding is then 4e-6 to 2e-5
+    // of the result (0.9 to 4 times the plain fp32 evaluation's; half a step is 2e-3 or 2.4e-4) and grows with the length
+    // beyond: 4.8e-5 at 4095 x 6001, 8.7e-5 at 16384 x 32768 (random signs). In chunks of 1024 it is 1.4e-5 and 5e-6, and the
+    // time 5.55 ms for 5.17 and 455 ms for 443; chunks of 2048 would take 5.42 ms for 2.7e-5, of 512 5.75 ms for 7e-6.
+    b.whole = !fp32;
+    for (int i = 0; i < b.n; ++i) b.whole = b.whole && longest_sum(b.m[i]) <= kWholeStages;
+    if (!fp32 && !b.whole) {
+        for (int i = 0; i < b.n; ++i) b.m[i].chunk = kLongChunk;
+        hand_out(b, pairs);
+    }
+    b.pairs = 0;
+    long long partials = 0;
+    for (int i = 0; i < b.n; ++i) {
+        Matrix& m = b.m[i];
+        m.pair_first = b.pairs;
+        b.pairs += m.pairs;
+        m.partial_first = partials;
+        if (m.splits > 1) partials += (long long)symmetric_tiles(m.row_tiles, m.gram_wide) * m.splits * 256 * (m.gram_wide ? 256 : 128);
+    }
 }
 
 // Pairs of CTAs of the chain that the current device holds at once: a property of the device, asked for once per device.
@@ -1841,9 +1847,8 @@ int run_typed(const gmc_matrix* matrices, int n, int steps, float ca, float cb, 
                     if (int s = run_clusters<T, MUON>(matrices, which, count, steps, ca, cb, cc, poly, epsilon, mo, stream)) return s;
                 } else {
                     Batch b;
-                    size_t bytes = 0;
-                    fill(matrices, which, count, pairs, std::is_same<T, float>::value, &b, &bytes, static_cast<uint8_t*>(workspace));
-                    if (bytes > workspace_bytes) return GMC_ERR_WORKSPACE;
+                    if (lay_out(matrices, which, count, static_cast<uint8_t*>(workspace), b) > workspace_bytes) return GMC_ERR_WORKSPACE;
+                    make_plan(b, pairs, std::is_same<T, float>::value);
                     b.lost_wait = lost_wait;
                     if (int s = run_batch<T, MUON>(b, steps, poly, epsilon, mo, stream)) return s;
                 }
@@ -1861,9 +1866,7 @@ size_t workspace_bytes_of(const gmc_matrix* matrices, int n) {
         if (i < n && kind_of(matrices[i]) == CHAIN) which[count++] = i;
         if (count == kMaxMatrices || (i == n && count > 0)) {
             Batch b;
-            size_t bytes = 0;
-            fill(matrices, which, count, kPairs, true, &b, &bytes, nullptr);
-            most = bytes > most ? bytes : most;
+            most = std::max(most, lay_out(matrices, which, count, nullptr, b));
             count = 0;
         }
     }
