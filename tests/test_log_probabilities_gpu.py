@@ -119,6 +119,28 @@ def test_forward_and_gradient(dtype, n, c, n_top):
     _check(z, t, n_top)
 
 
+@pytest.mark.parametrize("n,c,n_top,spread", [(5, 40, 3, 3.0), (3, 1024, 8, 3.0), (4, 4099, 4, 3.0), (2, 50257, 20, 3.0), (2, 131072, 32, 3.0),
+                                              (3, 1500, 2, 0.1), (2, 70001, 0, 6.0)])
+def test_small_gradients_of_fp16_logits(n, c, n_top, spread):
+    """Most elements of a long row's gradient are subnormal fp16 numbers: their own rounding is half a step, 2^-25, whatever their
+    size, beside half a step of the value above the smallest normal number."""
+    from gmc.classification import log_probabilities
+    z, t = _logits(n, c, torch.float16, 300 + c, spread)
+    z.requires_grad_(True)
+    g = torch.Generator(device="cuda").manual_seed(c)
+    grads = [torch.randn(n, device="cuda", generator=g), torch.randn(n, device="cuda", generator=g),
+             torch.randn(n, n_top, device="cuda", generator=g)]
+    ref = _reference(z, t, n_top, 1.0, -100, grads)
+    r = log_probabilities(z, t, n_top)
+    values = [r.target, r.entropy] + ([r.top] if n_top else [])
+    (got,) = torch.autograd.grad(values, z, grads[:len(values)])
+    info = torch.finfo(torch.float16)
+    own = torch.where(ref["grad"].abs() < info.smallest_normal, torch.full_like(ref["grad"], 2.0 ** -25), info.eps / 2 * ref["grad"].abs())
+    # a value within the evaluation's error of the border between two steps may go either way: the rounding is of the computed value
+    _close(got, ref["grad"], ref["grad_tolerance"] * (1 + info.eps) + own, "gradient")
+    assert (got != 0).sum() >= (ref["grad"].abs() > 2.0 ** -24).sum()
+
+
 @pytest.mark.parametrize("temperature", [1e-6, 0.05, 0.7, 3.0, 1e6])
 @pytest.mark.parametrize("c", [17, 3001])
 def test_temperatures(temperature, c):

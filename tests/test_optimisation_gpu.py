@@ -79,6 +79,30 @@ def test_a_long_inner_axis():
     _check(orthogonalise(u), u)
 
 
+@pytest.mark.parametrize("m,n", [(1, 1), (16, 40), (64, 160), (64, 2000), (128, 1536), (129, 127), (200, 20000), (1025, 1031), (32768, 3),
+                                 (300, 9000), (6000, 250)])
+def test_fp16_results_down_to_the_smallest_numbers(m, n):
+    """The file's bound with fp16's own absolute error: half a step where values are subnormal, 2^-25."""
+    from gmc.optimisation import orthogonalise
+    u = _update(m, n, seed=m + n, dtype=torch.float16)
+    got = orthogonalise(u)
+    ref, plain = _plain(u.double(), 5, COEFFICIENTS, 1e-7), _plain(u.float(), 5, COEFFICIENTS, 1e-7).double()
+    norm = torch.linalg.matrix_norm
+    bound = 4 * norm(plain - ref) + (2.0 ** -17 + torch.finfo(torch.float16).eps / 2) * norm(ref) \
+        + torch.finfo(torch.float16).smallest_normal * 2.0 ** -11 * math.sqrt(m * n)
+    assert norm(got.double() - ref) <= bound, f"{(norm(got.double() - ref) / norm(ref)).item():.3e} against {(bound / norm(ref)).item():.3e}"
+
+
+@pytest.mark.parametrize("m,n", [(20, 3000), (100, 1000), (256, 6000), (1500, 4100), (4100, 1500), (2048, 2048)])
+def test_updates_of_one_sign(m, n):
+    """Updates behind a rectifier have one sign: the tensor core's sums then lose bits in one direction everywhere."""
+    from gmc.optimisation import orthogonalise
+    g = torch.Generator(device="cuda").manual_seed(m * n)
+    for u in (0.1 + torch.rand(m, n, device="cuda", generator=g), torch.rand(m, n, device="cuda", generator=g).square(),
+              -torch.rand(m, n, device="cuda", generator=g).relu() * (torch.rand(m, 1, device="cuda", generator=g) < 0.3)):
+        _check(orthogonalise(u), u)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("signs", ["random", "one"])
 @pytest.mark.parametrize("m,n", [(200, 20000), (1500, 4100), (2048, 2048), (2000, 30000), (4095, 6001)])
