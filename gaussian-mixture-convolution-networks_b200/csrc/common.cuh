@@ -25,17 +25,13 @@ void set_last_cuda_error(cudaError_t e);
 
 // One word per translation unit (the library is built without relocatable device code). Kernels OR
 // a code into it when a bounded wait gives up or a self check fails; gmc_device_check_word() reads
-// and clears the word of every unit through the reader that GMC_DEFINE_TU_CHECK_READER defines.
+// and clears the words of all units, whose places the functions that GMC_DEFINE_TU_CHECK_WORD defines tell.
 static __device__ int g_device_check_word;
 
-#define GMC_DEFINE_TU_CHECK_READER(name)                                                          \
-    int gmc_tu_check_##name(int* word) {                                                          \
-        int w = 0;                                                                                \
-        const int zero = 0;                                                                       \
-        GMC_CUDA_TRY(cudaMemcpyFromSymbol(&w, ::gmc::g_device_check_word, sizeof(int)));          \
-        if (w != 0) GMC_CUDA_TRY(cudaMemcpyToSymbol(::gmc::g_device_check_word, &zero, sizeof(int))); \
-        *word |= w;                                                                               \
-        return GMC_OK;                                                                            \
+#define GMC_DEFINE_TU_CHECK_WORD(name)                                                                              \
+    int gmc_tu_check_##name(int** word) {                                                                           \
+        GMC_CUDA_TRY(cudaGetSymbolAddress(reinterpret_cast<void**>(word), ::gmc::g_device_check_word));             \
+        return GMC_OK;                                                                                              \
     }
 
 enum DeviceCheck : int {

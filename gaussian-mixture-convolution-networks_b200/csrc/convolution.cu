@@ -130,7 +130,7 @@ int check_conv_args(int n_batch, int n_channels_in, int n_components, int n_chan
 }  // namespace
 }  // namespace gmc
 
-GMC_DEFINE_TU_CHECK_READER(convolution)
+GMC_DEFINE_TU_CHECK_WORD(convolution)
 
 extern "C" int gmc_convolution_forward(const float* data, const float* kernels, float* out, int n_batch,
                                        int n_channels_in, int n_components, int n_channels_out,

@@ -996,7 +996,7 @@ int launch_convfit_forward(const float* data, const float* kernels, const Dims& 
 }  // namespace
 }  // namespace gmc
 
-GMC_DEFINE_TU_CHECK_READER(convolution_fitting)
+GMC_DEFINE_TU_CHECK_WORD(convolution_fitting)
 
 extern "C" int gmc_convolution_fitting_forward(const float* data, const float* kernels, int n_batch, int n_channels_in,
                                                int n_components, int n_channels_out, int n_kernel_components,

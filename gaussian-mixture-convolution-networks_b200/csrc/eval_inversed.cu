@@ -997,7 +997,7 @@ int launch_backward(const float* grad_out, const float* mixture, const float* xe
 }  // namespace
 }  // namespace gmc
 
-GMC_DEFINE_TU_CHECK_READER(eval_inversed)
+GMC_DEFINE_TU_CHECK_WORD(eval_inversed)
 
 extern "C" int gmc_eval_inversed_forward(const float* mixture, const float* xes, float* out, int n_batch, int n_layers,
                                          int n_components, int n_dims, int n_batch_xes, int n_layers_xes, int n_xes,

@@ -77,7 +77,7 @@ inline size_t round64(size_t n) { return (n + 63) & ~size_t(63); }   // keeps ev
 }  // namespace
 }  // namespace gmc
 
-int gmc_tu_check_eval_inversed(int* word);   // reads and clears the check word of the evaluation kernels (eval_inversed.cu)
+int gmc_tu_check_eval_inversed(int** word);   // the check word of the evaluation kernels (eval_inversed.cu)
 
 extern "C" int gmc_eval_inversed_host(const float* mixture, const float* xes, const float* grad_out, float* out,
                                       float* grad_mixture, float* grad_xes, int n_batch, int n_layers,
@@ -222,8 +222,10 @@ extern "C" int gmc_eval_inversed_host(const float* mixture, const float* xes, co
     GMC_CUDA_TRY(e2);
     GMC_CUDA_TRY(e3);
     // everything is synchronised here anyway: a kernel that gave up (bounded wait) turns into an error status
-    int word = 0;
-    if (int s = gmc_tu_check_eval_inversed(&word)) return s;
+    int word = 0, *place = nullptr;
+    if (int s = gmc_tu_check_eval_inversed(&place)) return s;
+    GMC_CUDA_TRY(cudaMemcpy(&word, place, sizeof(int), cudaMemcpyDeviceToHost));
+    if (word != 0) GMC_CUDA_TRY(cudaMemset(place, 0, sizeof(int)));
     return word != 0 ? GMC_ERR_DEVICE_CHECK : GMC_OK;
 }
 

@@ -322,7 +322,7 @@ int lbvh_aabbs_launch(const float* mixture, long long n_mixtures, int n_componen
 
 }  // namespace gmc
 
-GMC_DEFINE_TU_CHECK_READER(lbvh)
+GMC_DEFINE_TU_CHECK_WORD(lbvh)
 
 extern "C" int gmc_lbvh_build(const float* mixture, long long n_mixtures, int n_components, int n_dims,
                               uint64_t* sorted_keys, int16_t* nodes, void* stream) {

@@ -729,7 +729,7 @@ int check_sizes(int dtype, long long n_rows, long long n_classes, long long row_
 }  // namespace
 }  // namespace gmc
 
-GMC_DEFINE_TU_CHECK_READER(log_probabilities)
+GMC_DEFINE_TU_CHECK_WORD(log_probabilities)
 
 extern "C" int gmc_log_probabilities_forward(const void* logits, int dtype, const long long* targets, long long n_rows,
                                              long long n_classes, long long row_stride, float temperature, long long ignore_index,

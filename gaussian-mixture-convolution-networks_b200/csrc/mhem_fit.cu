@@ -956,7 +956,7 @@ int launch_fit_backward(const float* grad, const float* mixture, long long n_mix
 }  // namespace
 }  // namespace gmc
 
-GMC_DEFINE_TU_CHECK_READER(mhem_fit)
+GMC_DEFINE_TU_CHECK_WORD(mhem_fit)
 
 extern "C" size_t gmc_mhem_fit_attribute_floats(int n_components, int n_dims, int reduction_n) {
     if (n_components < 2 || (n_dims != 2 && n_dims != 3) || (reduction_n != 2 && reduction_n != 4)) return 0;

@@ -1899,7 +1899,7 @@ int run(const gmc_matrix* matrices, int n, int dtype, int steps, float ca, float
 }  // namespace
 }  // namespace gmc
 
-GMC_DEFINE_TU_CHECK_READER(newton_schulz)
+GMC_DEFINE_TU_CHECK_WORD(newton_schulz)
 
 extern "C" size_t gmc_orthogonalise_workspace_bytes(const gmc_matrix* matrices, int n_matrices) {
     using namespace gmc;

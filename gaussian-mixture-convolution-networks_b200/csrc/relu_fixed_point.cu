@@ -516,7 +516,7 @@ int launch_relu_fixed_point(const float* mixtures, const float* constants, float
 }  // namespace
 }  // namespace gmc
 
-GMC_DEFINE_TU_CHECK_READER(relu_fixed_point)
+GMC_DEFINE_TU_CHECK_WORD(relu_fixed_point)
 
 extern "C" int gmc_relu_fixed_point_layer(const float* mixtures, const float* constants, float* out_mixtures,
                                           float* out_constants, float* out_initial, long long n_mixtures,

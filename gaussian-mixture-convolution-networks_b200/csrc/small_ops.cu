@@ -338,7 +338,7 @@ __global__ void index_check_probe_kernel(const float* one, long long index, long
 }  // namespace
 }  // namespace gmc
 
-GMC_DEFINE_TU_CHECK_READER(small_ops)
+GMC_DEFINE_TU_CHECK_WORD(small_ops)
 
 extern "C" int gmc_symeig(const float* matrices, float* eigenvalues, float* eigenvectors, long long n_matrices,
                           int n_dims, void* stream) {

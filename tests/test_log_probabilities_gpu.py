@@ -339,6 +339,24 @@ def test_a_target_out_of_range_is_reported(c):
     assert _native.device_check_word() == 0
 
 
+def test_reports_of_several_kernels_are_read_and_cleared_together():
+    from gmc import _native
+    from gmc.classification import log_probabilities
+    u = torch.randn(200, 300, device="cuda")
+    packed = _native.matrix_struct.pack(u.data_ptr(), 0, u.data_ptr(), 200, 300, 300, 300, 0.0)
+    size = _native.lib.gmc_orthogonalise_workspace_bytes(packed, 1)
+    hold = torch.empty(size + 1024, dtype=torch.uint8, device="cuda")
+    stream = _native.stream_of(u)
+    assert _native.lib.gmc_sync_and_check(stream) == 0
+    _native.check(_native.lib.gmc_debug_orthogonalise_lost_wait(packed, 1, 0, 5, 3.4445, -4.775, 2.0315, 1e-7,
+                                                                (hold.data_ptr() + 1023) // 1024 * 1024, size, 0, stream), "")
+    log_probabilities(torch.zeros(1, 4, device="cuda"), torch.tensor([4], device="cuda"))
+    assert _native.device_check_word() == 1 | 8
+    assert _native.device_check_word() == 0
+    log_probabilities(torch.zeros(1, 4, device="cuda"), torch.tensor([-1], device="cuda"))
+    assert _native.lib.gmc_sync_and_check(stream) == 7 and _native.lib.gmc_sync_and_check(stream) == 0
+
+
 @pytest.mark.parametrize("c", [12, 2500])
 def test_gradient_against_differences(c):
     """Central differences of the forward values along random directions: cut-off error h^2 / 6 |f'''| with |f'''| <= 12 |v|^3
