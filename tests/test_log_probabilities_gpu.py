@@ -278,6 +278,35 @@ def test_strides_and_alignment(dtype, c):
     _check(wide[::2, :c], t[::2].contiguous(), 6)
 
 
+@pytest.mark.parametrize("n,c", [(36000, 65537), (2500000, 900)])
+def test_offsets_beyond_32_bits(n, c):
+    """More than 2^31 logits in both kernels: the first rows, those around the 2^31st element and the last ones, and their gradients."""
+    from gmc.classification import log_probabilities
+    some = torch.cat([torch.arange(3), 2 ** 31 // c + torch.arange(-2, 3), n - 1 - torch.arange(3)]).cuda()
+    rows, t_some = _logits(len(some), c, torch.bfloat16, 3)
+    z = torch.zeros(n, c, device="cuda", dtype=torch.bfloat16)
+    z[some] = rows
+    t = torch.zeros(n, dtype=torch.int64, device="cuda")
+    t[some] = t_some
+    z.requires_grad_(True)
+    r = log_probabilities(z, t, n_top=2)
+    one = torch.ones(n, device="cuda")
+    (grad,) = torch.autograd.grad([r.target, r.entropy], z, [one, one])
+    ref = _reference(rows, t_some, 2, 1.0, -100, [torch.ones(len(some)), torch.ones(len(some)), torch.zeros(len(some), 2)])
+    y = ref["y"].gather(1, torch.where(t_some == -100, 0, t_some).cpu().unsqueeze(1)).squeeze(1).abs()
+    _close(r.target[some], ref["target"], U * (_scale(c) + 4 * y), "target")
+    _close(r.entropy[some], ref["entropy"], U * 2 * _scale(c) * (1 + math.log2(c)), "entropy")
+    assert torch.equal(r.top_indices[some].cpu(), ref["top_indices"])
+    _close(grad[some], ref["grad"], ref["grad_tolerance"] + 2.0 ** -8 * ref["grad"].abs() + torch.finfo(torch.float32).smallest_normal, "gradient")
+    # all other rows are uniform: the target's gradient is 1 - 1 / c, the others' -1 / c, the entropy's 0
+    others = torch.ones(n, dtype=torch.bool, device="cuda")
+    others[some] = False
+    u = U * (_scale(c) + 16)
+    assert ((r.entropy - math.log(c)).abs()[others] <= 2 * u * (1 + math.log2(c))).all()
+    assert ((grad[:, 0].float() - (1 - 1 / c)).abs()[others] <= 2.0 ** -8).all()
+    assert ((grad[:, c - 1].float() * c + 1).abs()[others] <= 2.0 ** -8 + 64 * u).all()
+
+
 def test_the_gradient_of_a_broadcast_row_is_summed():
     from gmc.classification import log_probabilities
     row = torch.randn(1, 2000, device="cuda", requires_grad=True)

@@ -360,6 +360,32 @@ def test_optimiser_steps_and_state():
     assert torch.equal(params[2], idle) and params[2] not in opt.state
 
 
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("m,n", [(1, 5), (5, 9), (9, 5), (16, 2000), (64, 160), (160, 64), (100, 1000), (130, 9), (200, 333), (333, 200),
+                                 (700, 1031)])
+@pytest.mark.parametrize("gap,first", [(0, 0), (3, 1), (8, 8)])
+def test_strided_results_in_place_of_the_update_and_beside_it(m, n, dtype, gap, first):
+    """The C entry with rows apart: what lies between them, before and behind stays as it was, with the result in the update's own
+    place and elsewhere."""
+    from gmc import _native
+    u = _update(m, n, seed=m * n, dtype=DTYPES[dtype])
+    stride = n + gap
+    for in_place in (True, False):
+        source = torch.full((first + (m + 1) * stride,), 7.0, device="cuda", dtype=u.dtype)
+        source[first:first + m * stride].view(m, stride)[:, :n] = u
+        target = source if in_place else torch.full_like(source, 9.0)
+        before, place = target.clone(), first * u.element_size()
+        packed = _native.matrix_struct.pack(source.data_ptr() + place, 0, target.data_ptr() + place, m, n, stride, stride, 0.0)
+        size = _native.lib.gmc_orthogonalise_workspace_bytes(packed, 1)
+        hold = torch.empty(size + 1024, dtype=torch.uint8, device="cuda")
+        _native.check(_native.lib.gmc_orthogonalise(packed, 1, dtype, 5, *COEFFICIENTS, 1e-7, (hold.data_ptr() + 1023) // 1024 * 1024, size,
+                                                    _native.stream_of(u)), "")
+        _check(target[first:first + m * stride].view(m, stride)[:, :n], u)
+        for t in (target, before):
+            t[first:first + m * stride].view(m, stride)[:, :n] = 0.0
+        assert torch.equal(target, before)
+
+
 def test_captured_and_replayed_on_another_stream():
     from gmc.optimisation import muon_update, orthogonalise
     shapes = [(20, 45), (200, 150)]
