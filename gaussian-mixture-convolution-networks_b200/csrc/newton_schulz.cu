@@ -576,63 +576,63 @@ __device__ __forceinline__ void write_product(Product p, const Walk& w, ChainBar
             if (!shared_out)
                 send_stage(to, 2 * ti + cta, (tj * 2 * half + (wide ? col0 : 0)) >> 6, stages + s * kStageBytes, &bar.empty[s], wide, warp, lane);
         } else {
-        float sum[128];
+            float sum[128];
 #pragma unroll
-        for (int i = 0; i < 128; ++i) sum[i] = 0.f;
-        unsigned place = 0;
-        for (int kb = k0; kb < k1; kb += stages_per_chunk, place ^= wide ? 0 : 1) {
-            ok = ok && warp_wait(&bar.ready[place], (n.phase >> place) & 1);
-            n.phase ^= 1u << place;
+            for (int i = 0; i < 128; ++i) sum[i] = 0.f;
+            unsigned place = 0;
+            for (int kb = k0; kb < k1; kb += stages_per_chunk, place ^= wide ? 0 : 1) {
+                ok = ok && warp_wait(&bar.ready[place], (n.phase >> place) & 1);
+                n.phase ^= 1u << place;
+                tmem_fence_after();
+                // The mean of what the chunk's n = 4 additions per stage have lost, as measured against 64-bit sums: 2.0 n 2^-25 on the
+                // diagonal of X X^T, where all terms have one sign; 2.4 n 2^-25 on A A's, where most of a sum comes with one term;
+                // 0.7 n 2^-25 where signs are random (off the diagonals) or one term of B X, the diagonal's, outweighs the others
+                // (the half of the additions that follow it lose half a step each).
+                const float loss = 0x1p-25f * 4.f * float(min(stages_per_chunk, k1 - kb));
+                const float made_good = 1.f + 0.7f * loss, diagonal_good = 1.f + (p == GRAM ? 2.f : p == POLY ? 2.4f : 0.7f) * loss;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if (q < 2 || wide) {
+                        float v[32];
+                        tmem_load32(tmem + place * 128 + lanes + col0 + q * 32, v);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) sum[q * 32 + i] += v[i] * (q * 32 + i == diagonal ? diagonal_good : made_good);
+                    }
+                }
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_at(&bar.drained[place], 0);
+            }
+            ok = ok && warp_wait(&bar.mixed_ready, n.tile & 1);
             tmem_fence_after();
-            // The mean of what the chunk's n = 4 additions per stage have lost, as measured against 64-bit sums: 2.0 n 2^-25 on the
-            // diagonal of X X^T, where all terms have one sign; 2.4 n 2^-25 on A A's, where most of a sum comes with one term;
-            // 0.7 n 2^-25 where signs are random (off the diagonals) or one term of B X, the diagonal's, outweighs the others
-            // (the half of the additions that follow it lose half a step each).
-            const float loss = 0x1p-25f * 4.f * float(min(stages_per_chunk, k1 - kb));
-            const float made_good = 1.f + 0.7f * loss, diagonal_good = 1.f + (p == GRAM ? 2.f : p == POLY ? 2.4f : 0.7f) * loss;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 if (q < 2 || wide) {
                     float v[32];
-                    tmem_load32(tmem + place * 128 + lanes + col0 + q * 32, v);
+                    tmem_load32(tmem + kMixedColumns + lanes + col0 + q * 32, v);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) sum[q * 32 + i] += v[i] * (q * 32 + i == diagonal ? diagonal_good : made_good);
+                    for (int i = 0; i < 32; ++i) sum[q * 32 + i] += v[i];
                 }
             }
             tmem_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_at(&bar.drained[place], 0);
-        }
-        ok = ok && warp_wait(&bar.mixed_ready, n.tile & 1);
-        tmem_fence_after();
+            if (lane == 0) mbar_arrive_at(&bar.mixed_drained, 0);
+            n.k += k1 - k0;
+            if (p == GRAM && w.splits > 1) {
+                // [unit][CTA][column][row]
+                float* out = partial + (((long long)u * 2 + cta) * (2 * half) + col0) * 128 + (warp & 3) * 32 + lane;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            if (q < 2 || wide) {
-                float v[32];
-                tmem_load32(tmem + kMixedColumns + lanes + col0 + q * 32, v);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) sum[q * 32 + i] += v[i];
+                for (int i = 0; i < 128; ++i)
+                    if (i < 64 || wide) out[i * 128] = sum[i];
+                continue;
             }
-        }
-        tmem_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_at(&bar.mixed_drained, 0);
-        n.k += k1 - k0;
-        if (p == GRAM && w.splits > 1) {
-            // [unit][CTA][column][row]
-            float* out = partial + (((long long)u * 2 + cta) * (2 * half) + col0) * 128 + (warp & 3) * 32 + lane;
-#pragma unroll
-            for (int i = 0; i < 128; ++i)
-                if (i < 64 || wide) out[i * 128] = sum[i];
-            continue;
-        }
-        // the stages behind the tile's: two blocks each. Wide: warps 0-3 have the first one's, warps 4-7 the second one's.
-        const unsigned k = n.k + (wide ? warp >> 2 : 0), s = k % kStages;
-        n.k += wide ? 2 : 1;
-        ok = ok && warp_wait(&bar.full[s], (k / kStages) & 1);
-        place_block(sum, stages + s * kStageBytes + (wide ? 0 : warp >> 2) * kBlockBytes + (warp & 3) * kWarpRows, p != GRAM, c0, c1, lane);
-        if (wide) place_block(sum + 64, stages + s * kStageBytes + kBlockBytes + (warp & 3) * kWarpRows, p != GRAM, c0, c1, lane);
-        send_stage(to, 2 * ti + cta, (tj * 2 * half + (wide ? col0 : 0)) >> 6, stages + s * kStageBytes, &bar.empty[s], wide, warp, lane);
+            // the stages behind the tile's: two blocks each. Wide: warps 0-3 have the first one's, warps 4-7 the second one's.
+            const unsigned k = n.k + (wide ? warp >> 2 : 0), s = k % kStages;
+            n.k += wide ? 2 : 1;
+            ok = ok && warp_wait(&bar.full[s], (k / kStages) & 1);
+            place_block(sum, stages + s * kStageBytes + (wide ? 0 : warp >> 2) * kBlockBytes + (warp & 3) * kWarpRows, p != GRAM, c0, c1, lane);
+            if (wide) place_block(sum + 64, stages + s * kStageBytes + kBlockBytes + (warp & 3) * kWarpRows, p != GRAM, c0, c1, lane);
+            send_stage(to, 2 * ti + cta, (tj * 2 * half + (wide ? col0 : 0)) >> 6, stages + s * kStageBytes, &bar.empty[s], wide, warp, lane);
         }
     }
 }
