@@ -129,6 +129,9 @@ __device__ __forceinline__ Stat warp_merge(Stat a, float k) {
     }
     return a;
 }
+// e^(x / T) by the approximate base-2 exponential (error 2^-22 of itself) of x k rounded to fp32, 2^-24 |x k|: terms that count have
+// |x k| of a few, up to log2 of the row's length, and log p comes out to 1e-7, as with expf of a rounded x / T (1 x 50257:
+// 1.0e-7 against 0.6e-7 of plain fp32 operations, 5e-7 seen); one multiplication and one special-function instruction a term.
 __device__ __forceinline__ void add_element(float z, float base, float k, float& s, float& t) {
     const float x = z - base;
     const float e = ex2_approx(x * k);

@@ -358,10 +358,11 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Bat
 // made good; hi lo and lo hi, 2^-11 as large, have an accumulator of their own. Where results are rounded to 16 bits and no
 // sum is longer than 2048, one accumulation takes the whole axis, and both sums are ready and read at the same time.
 //
-// Measured (fp32, five steps, the launches around the chain included): 4095 x 6001 in bf16 5.14 ms, 360 TFLOP/s of the
-// polynomial's and 1081 of the tensor core's products, 0.77 of a large library product under the same power limit; bound by
-// the MMAs (a stage takes 1516 cycles, its MMAs 1536 at the nominal rate) and by the last tiles of a product, for which
-// the other pairs wait. 2048 x 2048: 679 us, 253 TFLOP/s; fp32 sums leave the tensor core every 512 in K. Below about 1000 rows
+// Measured (fp32, five steps, the launches around the chain included): 4095 x 6001 in bf16 5.46 ms, 339 TFLOP/s of the
+// polynomial's and 1018 of the tensor core's products, 0.72 of a large library product under the same power limit; bound by
+// the MMAs (a stage takes 1516 cycles, its MMAs 1536 at the nominal rate), by the sums' way out every 16 stages (1400) and by the
+// last tiles of a product, for which the other pairs wait. 2048 x 2048: 678 us, 253 TFLOP/s; fp32 sums leave the tensor core
+// every 512 in K, and 256 bytes a thread of the chunked form's registers spill (none of the whole form's). Below about 1000 rows
 // the latencies of a product (barrier, first loads, one tile's way out: 11 to 13 us) count for more than its MMAs.
 enum Product { GRAM, POLY, STEP };
 constexpr int kWriters = 256;
@@ -1167,7 +1168,8 @@ __device__ __forceinline__ void short_matrix(const Matrix& m, int ranks, int ran
 // summing rows q MP / ranks .. and handing them to all as planes; B = b A + c A A in A's place, each CTA for itself;
 // X <- a X + B X in place. All accumulators are in tensor memory; additions per accumulator are few (128 in K), so that the
 // losses of the module comment stay small. What bounds it is the chain of latencies, about eight barriers a step: 64 x 160 takes 40 us, 0.28
-// TFLOP/s of the polynomial's.
+// TFLOP/s of the polynomial's. The update is held in registers over the norm, and of 128 a thread (512 threads fill the register
+// file) 236 to 252 bytes spill; what that costs is not known.
 constexpr int kMidThreads = 512;
 constexpr int kMidWarps = kMidThreads / 32;
 __host__ __device__ constexpr int mid_rows(int rows) { return rows <= 64 ? 64 : 128; }
